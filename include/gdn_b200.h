@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define GDN_ABI_VERSION 7
+#define GDN_ABI_VERSION 8
 
 enum gdn_status_code {
   GDN_OK = 0,
@@ -51,6 +51,11 @@ enum gdn_status_code {
 #define GDN_STATUS_BAD_SLOT 0x1
 #define GDN_STATUS_BAD_SEQLEN 0x2
 #define GDN_STATUS_TIMEOUT 0x4 /* a bounded device-side wait gave up; outputs invalid */
+#define GDN_STATUS_BAD_TREE 0x8     /* a parent or an accepted node that is not one */
+#define GDN_STATUS_BAD_POSITION 0x10 /* a position outside the rotation table */
+
+/* Most nodes of one drafted tree (the tree operators' ancestor sets are 64 bits). */
+#define GDN_MAX_TREE_NODES 64
 
 enum gdn_dtype { GDN_DTYPE_F32 = 0, GDN_DTYPE_BF16 = 1 };
 
@@ -305,6 +310,165 @@ int gdn_decode_fused_static(const void* mixed, int64_t mixed_row_stride,
                             const int64_t* ids, const void* norm_weight, float norm_eps,
                             void* out, int32_t bs, int32_t num_k_heads, int32_t num_v_heads,
                             int32_t head_dim, float scale, int32_t* status, void* stream);
+
+/*
+ * Trees of drafted tokens (no counterpart in the reference, whose speculative
+ * decoding excludes this model: a rejected token cannot be taken out of a
+ * recurrent state).  The operators below compute all nodes of each sequence's
+ * tree without touching the stored state, and take an accepted path over
+ * afterwards.  Shared by all of them:
+ *  - sequence r owns rows [cu_seqlens[r], cu_seqlens[r+1]) (int32 [n_seqs + 1]
+ *    on the device, non-decreasing, the last entry at most n_tokens); rows
+ *    behind the last sequence are left as they were.  A sequence may be empty.
+ *  - parents: int32 [n_tokens]; a row's parent as a number within its sequence,
+ *    smaller than its own, or -1 for a node that follows the stored context
+ *    directly.  A node sees the context, its ancestors and itself.
+ *  - max_nodes bounds every sequence's rows, at most GDN_MAX_TREE_NODES.
+ *  - A malformed sequence (cu_seqlens, or more than max_nodes rows) is skipped
+ *    and flagged GDN_STATUS_BAD_SEQLEN; a parent or accepted node that is not one
+ *    is flagged GDN_STATUS_BAD_TREE, outputs of its sequence are then
+ *    unspecified and its state is left alone.  Nothing is read out of bounds.
+ *  - A row that holds NaN or infinities makes its own outputs and its
+ *    descendants' NaN (or infinite), never those of other nodes.
+ */
+
+/*
+ * (a)+(b) conv + SiLU along each node's ancestors, back into the slot's stored
+ * window, and the gate, in one launch.  The window is not rolled (gdn_commit_tree
+ * does that).  A chain's rows have the bits of gdn_conv_gate_varlen.
+ * Arguments as gdn_conv_gate_varlen, with the tree's.
+ */
+int gdn_conv_gate_tree(const void* x, int64_t x_row_stride,
+                       const void* conv_pool, int64_t slot_stride,
+                       int64_t num_slots, const int64_t* ids,
+                       const int32_t* cu_seqlens, int32_t n_seqs,
+                       const int32_t* parents, int32_t max_nodes,
+                       int64_t n_tokens, int32_t channels, int32_t kernel,
+                       const void* weight, void* y, int64_t y_row_stride,
+                       const void* b, const void* a, int64_t ab_row_stride,
+                       int32_t num_v_heads, const void* a_log,
+                       const void* dt_bias, int32_t param_dtype,
+                       float* g, void* beta, int32_t* status, void* stream);
+
+/*
+ * (d) The gated delta rule (the recurrence of gdn_recurrent_inplace) along each
+ * node's ancestors from the slot's stored state, which is only read.
+ * Arguments as gdn_recurrent_inplace with n_tokens rows; s_pool is not written.
+ * With z, out receives norm_weight * o * rsqrt(mean(o^2) + norm_eps) * silu(z)
+ * in fp32, rounded once.  v and z rows: even strides, 4-byte aligned.
+ */
+int gdn_delta_rule_tree(const void* q, int64_t q_row_stride,
+                        const void* k, int64_t k_row_stride,
+                        const void* v, int64_t v_row_stride,
+                        const float* g, const void* beta,
+                        const float* s_pool, int64_t slot_stride, int64_t num_slots,
+                        const int64_t* ids, const int32_t* cu_seqlens, int32_t n_seqs,
+                        const int32_t* parents, int32_t max_nodes, int64_t n_tokens,
+                        void* out, int32_t num_k_heads, int32_t num_v_heads,
+                        int32_t head_k_dim, int32_t head_v_dim, float scale,
+                        const void* z, int64_t z_row_stride, const void* norm_weight,
+                        float norm_eps, int32_t* status, void* stream);
+
+/*
+ * Take the accepted path of every sequence into its slot: accepted[r] (int32
+ * [n_seqs]) is its last accepted node, -1 for none (the slot keeps its state).
+ * The recurrent state runs through the path's tokens (k, v, g, beta as given to
+ * gdn_delta_rule_tree) and the conv window keeps the last kernel - 1 of (window,
+ * the path's rows of x, the conv's input).  Both pools are indexed by ids.
+ */
+int gdn_commit_tree(const void* x, int64_t x_row_stride,
+                    const void* k, int64_t k_row_stride,
+                    const void* v, int64_t v_row_stride,
+                    const float* g, const void* beta,
+                    void* conv_pool, int64_t conv_slot_stride,
+                    int32_t channels, int32_t kernel,
+                    float* s_pool, int64_t slot_stride, int64_t num_slots,
+                    const int64_t* ids, const int32_t* cu_seqlens, int32_t n_seqs,
+                    const int32_t* parents, const int32_t* accepted,
+                    int32_t max_nodes, int64_t n_tokens,
+                    int32_t num_k_heads, int32_t num_v_heads,
+                    int32_t head_k_dim, int32_t head_v_dim,
+                    int32_t* status, void* stream);
+
+/*
+ * RMS norm of every query and key head, the position rotation, and keys and
+ * values into the paged cache, in one launch: what stands between the hybrid
+ * model's attention projection and its attention (qwen3_5.py:654-694, 712-777;
+ * layers/rotary_embedding.py:31-70; layers/attention.py:19-49).
+ *   x^ = x * rsqrt(mean(x^2) + eps) * (unit_offset ? 1 + w : w);  the first
+ *   rotary_dim elements are rotated by halves: y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin
+ * fp32 arithmetic, rounded once.  q, k, v: bf16 rows of their heads (row strides
+ * given); q_weight, k_weight: bf16 [head_dim]; cos_sin: fp32 [max_position,
+ * rotary_dim], cosines then sines; positions: int64 [n_tokens], one outside the
+ * table is flagged GDN_STATUS_BAD_POSITION and its row's queries and keys are not
+ * written.  k_cache / v_cache: bf16, element (block, token, head, d) at
+ * block*block_stride + token*token_stride + head*head_stride + d, both alike;
+ * slot_mapping: int32 [n_tokens], block * block_size + token, -1 to store
+ * nothing; one outside the cache is flagged GDN_STATUS_BAD_SLOT and not stored.
+ * q_out: bf16 [n_tokens, num_q_heads, head_dim].  head_dim 64, 128 or 256,
+ * rotary_dim a multiple of 16; everything 16-byte aligned.
+ */
+int gdn_qk_norm_rope_cache(const void* q, int64_t q_row_stride,
+                           const void* k, int64_t k_row_stride,
+                           const void* v, int64_t v_row_stride,
+                           const void* q_weight, const void* k_weight,
+                           float eps, int32_t unit_offset,
+                           const float* cos_sin, int64_t max_position,
+                           int32_t rotary_dim, const int64_t* positions,
+                           void* k_cache, void* v_cache, int64_t block_stride,
+                           int64_t token_stride, int64_t head_stride,
+                           int64_t num_blocks, int32_t block_size,
+                           const int32_t* slot_mapping, void* q_out,
+                           int64_t n_tokens, int32_t num_q_heads,
+                           int32_t num_kv_heads, int32_t head_dim,
+                           int32_t* status, void* stream);
+
+/*
+ * Attention of every node over its sequence's paged cache (the layout of
+ * gdn_qk_norm_rope_cache): positions [0, context_lens[r]) and, at
+ * context_lens[r] + j, the nodes j on its path, whose keys and values the
+ * caller has stored there.  One node per sequence is the decode step, a chain
+ * the causal form (the role of layers/attention.py:116-128).
+ * q: bf16 [n_tokens] rows of num_q_heads heads; block_tables: int32 [n_seqs]
+ * rows of max_blocks pages (row stride table_stride); context_lens: int32
+ * [n_seqs]; max_len bounds context_lens[r] + the sequence's rows, a longer one
+ * is skipped and flagged GDN_STATUS_BAD_SEQLEN.  A page outside the cache is
+ * flagged GDN_STATUS_BAD_SLOT, never read.  scores are scaled by `scale`.
+ * out: bf16 [n_tokens, num_q_heads, head_dim].  head_dim 64, 128 or 256.
+ * workspace: device scratch of gdn_attention_tree_workspace_bytes() bytes (0:
+ * none needed), 16-byte aligned, used only during the call.
+ */
+int64_t gdn_attention_tree_workspace_bytes(int64_t n_tokens, int32_t n_seqs,
+                                           int32_t num_q_heads, int32_t num_kv_heads,
+                                           int32_t head_dim, int32_t max_nodes,
+                                           int32_t max_len);
+
+int gdn_attention_tree(const void* q, int64_t q_row_stride,
+                       const void* k_cache, const void* v_cache,
+                       int64_t block_stride, int64_t token_stride, int64_t head_stride,
+                       int64_t num_blocks, int32_t block_size,
+                       const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+                       const int32_t* context_lens, const int32_t* cu_seqlens,
+                       int32_t n_seqs, const int32_t* parents, int32_t max_nodes,
+                       int64_t n_tokens, int32_t max_len, void* out,
+                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                       float scale, void* workspace, int64_t workspace_bytes,
+                       int32_t* status, void* stream);
+
+/*
+ * Positions (int64 [n_rows]: context_lens[r] + the node's depth) and cache
+ * slots (int32 [n_rows]) of all nodes.  accepted == NULL: node i waits at logical
+ * position context_lens[r] + i; else (int32 [n_seqs], as gdn_commit_tree) a node
+ * on the accepted path gets the slot of context_lens[r] + its depth, any other
+ * -1.  A missing page (-1, or past max_blocks) gives -1, flagged
+ * GDN_STATUS_BAD_SLOT; rows behind the last sequence get position 0, slot -1.
+ */
+int gdn_tree_slot_map(const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+                      const int32_t* context_lens, const int32_t* cu_seqlens,
+                      int32_t n_seqs, const int32_t* parents, const int32_t* accepted,
+                      int32_t max_nodes, int32_t block_size, int64_t n_rows,
+                      int64_t* positions, int32_t* slot_mapping,
+                      int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,9 @@ GDN_ERR_CUDA = 3
 GDN_STATUS_BAD_SLOT = 0x1
 GDN_STATUS_BAD_SEQLEN = 0x2
 GDN_STATUS_TIMEOUT = 0x4
+GDN_STATUS_BAD_TREE = 0x8
+GDN_STATUS_BAD_POSITION = 0x10
+GDN_MAX_TREE_NODES = 64
 GDN_DTYPE_F32 = 0
 GDN_DTYPE_BF16 = 1
 
@@ -47,6 +50,18 @@ SIGNATURES = {
                          i64, vp, vp, f32, vp, i32, i32, i32, i32, f32, vp, vp, vp],
     "gdn_decode_fused_static": [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i32, vp, vp, i32, vp,
                                 i64, i64, vp, vp, f32, vp, i32, i32, i32, i32, f32, vp, vp],
+    "gdn_conv_gate_tree": [vp, i64, vp, i64, i64, vp, vp, i32, vp, i32, i64, i32, i32, vp, vp, i64,
+                           vp, vp, i64, i32, vp, vp, i32, vp, vp, vp, vp],
+    "gdn_delta_rule_tree": [vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, i64, vp, vp, i32, vp, i32,
+                            i64, vp, i32, i32, i32, i32, f32, vp, i64, vp, f32, vp, vp],
+    "gdn_commit_tree": [vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, i32, i32, vp, i64, i64, vp, vp,
+                        i32, vp, vp, i32, i64, i32, i32, i32, i32, vp, vp],
+    "gdn_qk_norm_rope_cache": [vp, i64, vp, i64, vp, i64, vp, vp, f32, i32, vp, i64, i32, vp, vp,
+                               vp, i64, i64, i64, i64, i32, vp, vp, i64, i32, i32, i32, vp, vp],
+    "gdn_attention_tree_workspace_bytes": [i64, i32, i32, i32, i32, i32, i32],
+    "gdn_attention_tree": [vp, i64, vp, vp, i64, i64, i64, i64, i32, vp, i64, i32, vp, vp, i32, vp,
+                           i32, i64, i32, vp, i32, i32, i32, f32, vp, i64, vp, vp],
+    "gdn_tree_slot_map": [vp, i64, i32, vp, vp, i32, vp, vp, i32, i32, i64, vp, vp, vp, vp],
 }
 
 _LIB = None
@@ -66,7 +81,8 @@ def load() -> C.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = {"gdn_last_error": C.c_char_p, "gdn_set_wait_limit": None,
-                      "gdn_chunk_prefill_workspace_bytes": C.c_int64}.get(name, C.c_int)
+                      "gdn_chunk_prefill_workspace_bytes": C.c_int64,
+                      "gdn_attention_tree_workspace_bytes": C.c_int64}.get(name, C.c_int)
     _LIB = lib
     return lib
 

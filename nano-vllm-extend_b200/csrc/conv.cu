@@ -30,6 +30,7 @@
 // prefills bit for bit).
 #include "common.cuh"
 #include "tc_util.cuh"
+#include "tree.cuh"
 
 namespace gdn {
 
@@ -314,6 +315,120 @@ __global__ void __launch_bounds__(kConvThreads) conv_state_writeback_kernel(
   for (int j = 0; j < T; ++j) sp[j] = nw[j];
 }
 
+// ---------------------------------------------------------------------------
+// trees of drafted tokens: a node's window runs along its ancestors, back into
+// the slot's stored taps, which stay as they are
+// ---------------------------------------------------------------------------
+//
+// y[n] = silu(sum_{i<K} w[K-1-i] * x[i-th ancestor of n]); above the root the
+// stored taps, newest first.  A CTA owns rows_per_cta rows x 1024 channels (or
+// 128 unaligned ones); its first warp walks every row's K-1 ancestors once and
+// leaves, per row and tap, the row to read or the stored tap.  Values come from
+// conv_point(), so a chain's rows have the bits of the varlen conv.
+constexpr int kTreeConvRows = 16;
+
+template <int K, bool VEC>
+__global__ void __launch_bounds__(kConvThreads) conv_tree_kernel(
+    const bf16* __restrict__ x, int64_t xs, const bf16* __restrict__ pool, int64_t slot_stride,
+    int64_t num_slots, const int64_t* __restrict__ ids, const int32_t* __restrict__ cu,
+    int n_seqs, const int32_t* __restrict__ parents, int max_nodes, int64_t n_tokens, int C,
+    const bf16* __restrict__ w, bf16* __restrict__ y, int64_t ys, int rows_per_cta,
+    int32_t* status, const GateArgs gate) {
+  constexpr int T = K - 1;
+  constexpr int V = VEC ? 8 : 1;
+  const int64_t t0 = (int64_t)blockIdx.x * rows_per_cta;
+  const int rows = (int)min((int64_t)rows_per_cta, n_tokens - t0);
+  // per row: its slot (-1: leave the row), and per tap i the flat row of the
+  // i-th ancestor, or -1 - j for the stored tap j
+  __shared__ int64_t s_slot[kTreeConvRows];
+  __shared__ int64_t s_src[kTreeConvRows][K];
+  const int c0 = (blockIdx.y * kConvThreads + threadIdx.x) * V;
+  const bool gate_cta = blockIdx.y == gridDim.y - 1;
+  float wv[V * K];
+  if (!gate_cta && c0 < C) {
+    if constexpr (VEC) {
+      const uint4* wp = reinterpret_cast<const uint4*>(w + (int64_t)c0 * K);
+#pragma unroll
+      for (int j = 0; j < K; ++j) unpack8(wp[j], wv + 8 * j);
+    } else {
+#pragma unroll
+      for (int i = 0; i < K; ++i) wv[i] = bf2f(w[(int64_t)c0 * K + i]);
+    }
+  }
+  if (threadIdx.x < 32) {
+    int r = warp_seq_of(cu, n_seqs, t0);
+    const int lane = threadIdx.x;
+    if (lane < rows) {
+      const int64_t t = t0 + lane;
+      while (r < n_seqs && (int64_t)cu[r + 1] <= t) ++r;
+      int64_t start = 0, slot = -1;
+      int n = 0;
+      if (r < n_seqs && tree_rows(cu, r, n_tokens, max_nodes, status, start, n) && t >= start &&
+          t < start + n) {
+        slot = ids[r];
+        if (!slot_ok(slot, num_slots, status)) slot = -1;
+        int at = (int)(t - start), above = 0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+          s_src[lane][i] = at >= 0 ? start + at : (int64_t)(-1 - (T - 1 - above));
+          if (at < 0) ++above;
+          else at = i + 1 < K ? tree_parent(parents[start + at], at, status) : -1;
+        }
+      }
+      s_slot[lane] = slot;
+    }
+  }
+  __syncthreads();
+  if (gate_cta) {
+    const int total = rows * gate.H;
+    for (int i = threadIdx.x; i < total; i += kConvThreads) {
+      const int rr = i / gate.H;
+      if (s_slot[rr] < 0) continue;
+      const int h = i - rr * gate.H;
+      const int64_t t = t0 + rr;
+      const float al = gate.param_bf16 ? bf2f(static_cast<const bf16*>(gate.a_log)[h])
+                                       : static_cast<const float*>(gate.a_log)[h];
+      const float db = gate.param_bf16 ? bf2f(static_cast<const bf16*>(gate.dt_bias)[h])
+                                       : static_cast<const float*>(gate.dt_bias)[h];
+      float gv, bt;
+      gate_value(bf2f(gate.a[t * gate.ab_stride + h]), bf2f(gate.b[t * gate.ab_stride + h]), al,
+                 db, gv, bt);
+      gate.g[t * gate.H + h] = gv;
+      gate.beta[t * gate.H + h] = f2bf(bt);
+    }
+    return;
+  }
+  if (c0 >= C) return;
+  for (int rr = 0; rr < rows; ++rr) {
+    const int64_t slot = s_slot[rr];
+    if (slot < 0) continue;
+    const bf16* taps = pool + slot * slot_stride + (int64_t)c0 * T;
+    float win[K][V];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int64_t src = s_src[rr][i];
+      if (src >= 0) {
+        if constexpr (VEC) unpack8(*reinterpret_cast<const uint4*>(x + src * xs + c0), win[T - i]);
+        else win[T - i][0] = bf2f(x[src * xs + c0]);
+      } else {
+        const int j = (int)(-1 - src);
+#pragma unroll
+        for (int ch = 0; ch < V; ++ch) win[T - i][ch] = bf2f(taps[ch * T + j]);
+      }
+    }
+    float out[V];
+#pragma unroll
+    for (int ch = 0; ch < V; ++ch) {
+      float wn[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) wn[i] = win[i][ch];
+      out[ch] = conv_point<K>(wn, wv + ch * K);
+    }
+    if constexpr (VEC) *reinterpret_cast<uint4*>(y + (t0 + rr) * ys + c0) = pack8(out);
+    else y[(t0 + rr) * ys + c0] = f2bf(out[0]);
+  }
+}
+
 }  // namespace gdn
 
 using namespace gdn;
@@ -440,4 +555,52 @@ extern "C" int gdn_conv_gate_varlen(const void* x, int64_t x_row_stride, void* c
   return launch_conv_varlen(fn, x, x_row_stride, conv_pool, slot_stride, num_slots, ids,
                             cu_seqlens, n_seqs, n_tokens, channels, kernel, weight, y,
                             y_row_stride, gate, status, stream);
+}
+
+extern "C" int gdn_conv_gate_tree(const void* x, int64_t x_row_stride, const void* conv_pool,
+                                  int64_t slot_stride, int64_t num_slots, const int64_t* ids,
+                                  const int32_t* cu_seqlens, int32_t n_seqs,
+                                  const int32_t* parents, int32_t max_nodes, int64_t n_tokens,
+                                  int32_t channels, int32_t kernel, const void* weight, void* y,
+                                  int64_t y_row_stride, const void* b, const void* a,
+                                  int64_t ab_row_stride, int32_t num_v_heads, const void* a_log,
+                                  const void* dt_bias, int32_t param_dtype, float* g, void* beta,
+                                  int32_t* status, void* stream) {
+  clear_error();
+  const char* fn = "gdn_conv_gate_tree";
+  GDN_REQUIRE(n_seqs >= 0 && n_tokens >= 0 && channels > 0 && num_v_heads > 0,
+              "%s: bad sizes (n_seqs=%d, n_tokens=%lld, channels=%d, heads=%d)", fn, n_seqs,
+              (long long)n_tokens, channels, num_v_heads);
+  GDN_REQUIRE(max_nodes >= 0, "%s: max_nodes %d < 0", fn, max_nodes);
+  GDN_UNSUPPORTED(max_nodes <= kMaxTreeNodes, "%s: %d nodes in a tree (max %d)", fn, max_nodes,
+                  kMaxTreeNodes);
+  GDN_UNSUPPORTED(kernel >= 2 && kernel <= 4, "%s: kernel %d unsupported (2..4)", fn, kernel);
+  GDN_REQUIRE(x_row_stride >= channels && y_row_stride >= channels,
+              "%s: row stride smaller than channels", fn);
+  GDN_REQUIRE(num_slots > 0 && slot_stride >= (int64_t)channels * (kernel - 1),
+              "%s: slot_stride too small", fn);
+  GDN_REQUIRE(ab_row_stride >= num_v_heads, "%s: row stride %lld < heads %d", fn,
+              (long long)ab_row_stride, num_v_heads);
+  GDN_REQUIRE(param_dtype == GDN_DTYPE_F32 || param_dtype == GDN_DTYPE_BF16,
+              "%s: param_dtype must be F32 or BF16", fn);
+  if (n_seqs == 0 || n_tokens == 0 || max_nodes == 0) return GDN_OK;
+  GDN_REQUIRE(x && conv_pool && ids && cu_seqlens && parents && weight && y && b && a && a_log &&
+                  dt_bias && g && beta,
+              "%s: null pointer", fn);
+  const bool vec = channels % 8 == 0 && x_row_stride % 8 == 0 && y_row_stride % 8 == 0 &&
+                   aligned16(x) && aligned16(y) && aligned16(weight);
+  const int per_cta = vec ? kConvThreads * 8 : kConvThreads;
+  const unsigned cy = (unsigned)((channels + per_cta - 1) / per_cta) + 1;   // + the gate's row
+  const int rows = kTreeConvRows;
+  const int64_t tiles = (n_tokens + rows - 1) / rows;
+  GDN_UNSUPPORTED(tiles < (1ll << 31) && cy <= 65535, "%s: too many tokens or channels", fn);
+  const GateArgs gate{(const bf16*)b, (const bf16*)a, ab_row_stride, num_v_heads, a_log, dt_bias,
+                      param_dtype == GDN_DTYPE_BF16, g, (bf16*)beta};
+  cudaStream_t s = (cudaStream_t)stream;
+  const dim3 grid((unsigned)tiles, cy);
+#define GDN_CT(KK, VV)                                                                            if (kernel == KK && vec == VV)                                                                    conv_tree_kernel<KK, VV><<<grid, kConvThreads, 0, s>>>(                                             (const bf16*)x, x_row_stride, (const bf16*)conv_pool, slot_stride, num_slots, ids,              cu_seqlens, n_seqs, parents, max_nodes, n_tokens, channels, (const bf16*)weight,                (bf16*)y, y_row_stride, rows, status, gate);
+  GDN_CT(2, true) GDN_CT(3, true) GDN_CT(4, true)
+  GDN_CT(2, false) GDN_CT(3, false) GDN_CT(4, false)
+#undef GDN_CT
+  return check_launch(fn);
 }

@@ -63,8 +63,12 @@ def _raise_for(v: int) -> int:
         raise IndexError(f"GDN kernel saw a slot id outside the pool (status {v:#x})")
     if v & _lib.GDN_STATUS_TIMEOUT:
         raise _lib.GdnError(f"GDN kernel gave up a bounded device-side wait (status {v:#x})")
+    if v & _lib.GDN_STATUS_BAD_POSITION:
+        raise IndexError(f"GDN kernel saw a position outside the rotation table (status {v:#x})")
     if v & _lib.GDN_STATUS_BAD_SEQLEN:
         raise ValueError(f"GDN kernel saw malformed cu_seqlens / max_seqlen (status {v:#x})")
+    if v & _lib.GDN_STATUS_BAD_TREE:
+        raise ValueError(f"GDN kernel saw a malformed tree of drafted tokens (status {v:#x})")
     return v
 
 
@@ -196,6 +200,34 @@ def check_cu_seqlens(cu, n_rows: int, max_seqlen: int | None = None) -> None:
     if max_seqlen is not None and c.size > 1 and int(np.diff(c).max()) > max_seqlen:
         raise ValueError(f"a sequence of {int(np.diff(c).max())} rows exceeds max_seqlen "
                          f"{max_seqlen}")
+
+
+def check_tree(cu, parents, max_nodes: int, n_rows: int, accepted=None) -> None:
+    """Raise ValueError unless cu starts at 0, never decreases, ends at most at
+    n_rows and gives no sequence more than max_nodes rows, every parent is -1 or an
+    earlier node of its sequence, and (when given) every accepted node is -1
+    or one of its sequence's."""
+    host = lambda t: np.asarray(t.cpu() if isinstance(t, torch.Tensor) else t, np.int64).reshape(-1)
+    c, p = host(cu), host(parents)
+    if c.size == 0 or c[0] != 0 or c[-1] > n_rows or (np.diff(c) < 0).any():
+        raise ValueError(f"cu_seqlens must start at 0, not decrease and end at most at {n_rows}")
+    n = np.diff(c)
+    if n.size and n.max() > max_nodes:
+        raise ValueError(f"a tree of {int(n.max())} nodes exceeds max_nodes {max_nodes}")
+    own = np.arange(c[-1]) - np.repeat(c[:-1], n)
+    bad = (p[:c[-1]] < -1) | (p[:c[-1]] >= own)
+    if bad.any():
+        raise ValueError(f"row {int(np.argmax(bad))} has parent {int(p[np.argmax(bad)])}: -1 or an "
+                         "earlier node of its sequence is wanted")
+    if accepted is not None:
+        a = host(accepted)
+        if ((a < -1) | (a >= n)).any():
+            raise ValueError("an accepted node is not one of its sequence's")
+
+
+def _debug_tree(tree, n_rows: int, accepted=None) -> None:
+    if _DEBUG_CHECKS and not torch.cuda.is_current_stream_capturing():
+        check_tree(tree[0], tree[1], tree[2], n_rows, accepted)
 
 
 def _debug_checks(ids=None, num_slots: int = 0, cu=None, n_rows: int = 0,
@@ -657,4 +689,303 @@ def decode_fused(mixed: torch.Tensor, z: torch.Tensor, b: torch.Tensor, a: torch
         _slot_stride(s_pool), s_pool.shape[0], _p(ids), _p(nw), float(eps), _p(out), bs, HK, HV,
         D, D ** -0.5, _p(cnt), _p(status_word(mixed.device)), _stream_ptr(mixed.device))
     _lib.check(rc, "gdn_decode_fused")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# trees of drafted tokens
+# ---------------------------------------------------------------------------
+#
+# A tree is (cu_seqlens, parents, max_nodes): sequence r owns rows
+# [cu_seqlens[r], cu_seqlens[r + 1]), one per node; parents [N] int32 holds each
+# row's parent as a number within its sequence, smaller than its own, -1 for a
+# node that follows the stored context directly; max_nodes (at most 64) bounds
+# every sequence's rows.  A node sees the context, its ancestors and itself; a
+# chain is the tree with parents -1, 0, 1, ...  Rows behind the last sequence are
+# left as they were.
+#
+# One round of checking drafted tokens: tree_slot_map gives positions and cache
+# slots; each GDN layer runs conv_gate_tree and gated_delta_rule_tree, each
+# attention layer qk_norm_rope_cache and attention_tree; once the accepted nodes are
+# known, each GDN layer runs commit_tree, and for trees that branch each
+# attention layer stores its rows again with the slots of
+# tree_slot_map(accepted=...) (a chain's keys and values already stand right).
+
+
+def _launch(name: str, device: torch.device, *args) -> None:
+    """Call entry point ``name`` with its device's status word and current stream,
+    on that device."""
+    lib = _lib.load()
+    if device.index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, _p(status_word(device)), _stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, _p(status_word(device)), _stream_ptr(device))
+    _lib.check(rc, name)
+
+
+def _one_device(*ts) -> torch.device:
+    dev = ts[0].device
+    for t in ts:
+        assert t is None or (t.is_cuda and t.device == dev), \
+            "GDN operators take CUDA tensors of one device"
+    return dev
+
+
+def _int32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    assert t.dim() == 1 and t.numel() == n, f"{name} must have {n} entries"
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        assert not t.is_floating_point(), f"{name} must hold integers"
+        t = t.to(torch.int32).contiguous()
+    return t
+
+
+def _tree(cu_seqlens, parents, max_nodes, n_seqs: int, n_rows: int):
+    return (_int32(cu_seqlens, n_seqs + 1, "cu_seqlens"), _int32(parents, n_rows, "parents"),
+            int(max_nodes))
+
+
+def _stride(row_stride: int, rows: int, width: int) -> int:
+    """The row stride to pass on; that of a single row means nothing and may be
+    anything, so it becomes the row's width."""
+    return row_stride if rows > 1 else width
+
+
+def _aligned_rows(t: torch.Tensor, row_stride: int, elements: int) -> bool:
+    return t.data_ptr() % (2 * elements) == 0 and row_stride % elements == 0
+
+
+def conv_gate_tree(x: torch.Tensor, state_pool: torch.Tensor, ids: torch.Tensor,
+                   weight: torch.Tensor, cu_seqlens: torch.Tensor, parents: torch.Tensor,
+                   max_nodes: int, b: torch.Tensor, a: torch.Tensor, a_log: torch.Tensor,
+                   dt_bias: torch.Tensor):
+    """:func:`conv_gate_varlen` for trees of drafted tokens: each row's window
+    runs along its ancestors, back into the window stored in ``state_pool[ids[r]]``,
+    which stays as it is (:func:`commit_tree` rolls it).  A chain's rows have the bits
+    of conv_gate_varlen.  Returns (y [N, C], g fp32 [N, Vh], beta bf16 [N, Vh])."""
+    dev = _one_device(x, state_pool, ids, weight, cu_seqlens, parents, b, a, a_log, dt_bias)
+    C = x.shape[-1]
+    w = weight.reshape(C, -1).contiguous()
+    K = w.shape[1]
+    _pool_view_check(state_pool, K - 1, C)
+    assert x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16
+    x2, xs = _rows2d(x, C)
+    N = x2.shape[0]
+    xs = _stride(xs, N, C)
+    ids = _ids64(ids)
+    tree = _tree(cu_seqlens, parents, max_nodes, ids.numel(), N)
+    assert b.dtype == torch.bfloat16 and a.dtype == torch.bfloat16 and a.shape == b.shape
+    vh = a.shape[-1]
+    assert a.numel() == N * vh, "b / a need one row per token"
+    assert a_log.numel() == vh and dt_bias.numel() == vh and a_log.dtype == dt_bias.dtype
+    if a.dim() != 2 or b.dim() != 2 or a.stride(0) != b.stride(0) or a.stride(1) != 1 \
+            or b.stride(1) != 1:
+        a = a.reshape(-1, vh).contiguous()
+        b = b.reshape(-1, vh).contiguous()
+    if a_log.dtype == torch.bfloat16:
+        pdt, a_log, dt_bias = _lib.GDN_DTYPE_BF16, a_log.contiguous(), dt_bias.contiguous()
+    else:
+        pdt, a_log, dt_bias = (_lib.GDN_DTYPE_F32, a_log.float().contiguous(),
+                               dt_bias.float().contiguous())
+    _debug_checks(ids, state_pool.shape[0])
+    _debug_tree(tree, N)
+    y = torch.empty(N, C, dtype=x.dtype, device=dev)
+    g = torch.empty(N, vh, dtype=torch.float32, device=dev)
+    beta = torch.empty(N, vh, dtype=torch.bfloat16, device=dev)
+    _launch("gdn_conv_gate_tree", dev, _p(x2), xs, _p(state_pool), _slot_stride(state_pool),
+            state_pool.shape[0], _p(ids), _p(tree[0]), ids.numel(), _p(tree[1]), tree[2], N, C, K,
+            _p(w), _p(y), C, _p(b), _p(a), _stride(a.stride(0), N, vh), vh, _p(a_log), _p(dt_bias), pdt,
+            _p(g), _p(beta))
+    return y, g, beta
+
+
+def _delta_args(k, v, g, beta, s_pool, ids):
+    """The checks gated_delta_rule_tree and commit_tree share."""
+    N, HK, DK, ks = _heads(k, "k")
+    N_v, HV, DV, vs = _heads(v, "v")
+    assert N_v == N and HV % HK == 0
+    assert k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16
+    g = g.reshape(N, HV)
+    beta = beta.reshape(N, HV)
+    assert g.dtype == torch.float32 and beta.dtype == torch.bfloat16 and g.is_contiguous() and \
+        beta.is_contiguous(), "g (fp32) / beta (bf16) must be contiguous"
+    _state_view_check(s_pool, HV, DK, DV)
+    ids = _ids64(ids)
+    _debug_checks(ids, s_pool.shape[0])
+    return (N, HK, HV, DK, DV, _stride(ks, N, HK * DK), _stride(vs, N, HV * DV), g, beta, ids)
+
+
+def gated_delta_rule_tree(q, k, v, g, beta, s_pool, ids, cu_seqlens, parents, max_nodes: int,
+                          z=None, norm_weight=None, eps: float = 1e-6, out=None) -> torch.Tensor:
+    """The gated delta rule along every node's ancestors, from the state in
+    ``s_pool[ids[r]]``, which stays as it is: row i of the result is what
+    :func:`recurrent_gdn_inplace` would return for it after its ancestors' steps.
+    q/k [N, HK, DK], v [N, HV, DV] (row views allowed), g fp32 / beta bf16 [N, HV].
+    Returns out [N, HV, DV]; with ``z`` ([N, HV, DV]) and ``norm_weight`` the gated
+    RMSNorm of it, in fp32 up to the one rounding at the end (the single-step
+    operators round three times on the way)."""
+    dev = _one_device(q, k, v, g, beta, s_pool, ids, cu_seqlens, parents, z, norm_weight)
+    N, HK, HV, DK, DV, ks, vs, g, beta, ids = _delta_args(k, v, g, beta, s_pool, ids)
+    N_q, HK_q, DK_q, qs = _heads(q, "q")
+    assert (N_q, HK_q, DK_q) == (N, HK, DK) and q.dtype == torch.bfloat16
+    tree = _tree(cu_seqlens, parents, max_nodes, ids.numel(), N)
+    _debug_tree(tree, N)
+    if not _aligned_rows(v, vs, 2):
+        v, vs = v.clone(memory_format=torch.contiguous_format), HV * DV
+    z3, zs, nw = _norm_args(z, norm_weight, N, HV, DV)
+    zs = _stride(zs, N, HV * DV)
+    if z3 is not None and not _aligned_rows(z3, zs, 2):
+        z3, zs = z3.clone(memory_format=torch.contiguous_format), HV * DV
+    out = _out_buffer(out, (N, HV, DV), dev)
+    _launch("gdn_delta_rule_tree", dev, _p(q), _stride(qs, N, HK * DK), _p(k), ks, _p(v), vs, _p(g),
+            _p(beta), _p(s_pool), _slot_stride(s_pool), s_pool.shape[0], _p(ids), _p(tree[0]),
+            ids.numel(), _p(tree[1]), tree[2], N, _p(out), HK, HV, DK, DV, DK ** -0.5, _p(z3),
+            zs, _p(nw), float(eps))
+    return out
+
+
+def commit_tree(x, k, v, g, beta, conv_pool, s_pool, ids, cu_seqlens, parents, max_nodes: int,
+                accepted) -> None:
+    """Take each sequence's accepted path into its slot of both pools:
+    ``accepted[r]`` (integers [n_seqs]) is the last accepted node, -1 for none.
+    ``s_pool[ids[r]]`` runs through the path's tokens as
+    :func:`recurrent_gdn_inplace` would one after the other (k, v, g, beta as given
+    to :func:`gated_delta_rule_tree`); ``conv_pool[ids[r]]`` keeps the last K - 1 of
+    its window and the path's rows of ``x`` [N, C], the input of
+    :func:`conv_gate_tree`.  Both pools are updated in place."""
+    dev = _one_device(x, k, v, g, beta, conv_pool, s_pool, ids, cu_seqlens, parents, accepted)
+    N, HK, HV, DK, DV, ks, vs, g, beta, ids = _delta_args(k, v, g, beta, s_pool, ids)
+    C = x.shape[-1]
+    assert x.dtype == torch.bfloat16
+    x2, xs = _rows2d(x, C)
+    assert x2.shape[0] == N
+    assert conv_pool.dim() == 3 and conv_pool.shape[0] == s_pool.shape[0], \
+        "both pools index the same slots"
+    K = conv_pool.shape[2] + 1
+    _pool_view_check(conv_pool, K - 1, C)
+    tree = _tree(cu_seqlens, parents, max_nodes, ids.numel(), N)
+    accepted = _int32(accepted, ids.numel(), "accepted")
+    _debug_tree(tree, N, accepted)
+    _launch("gdn_commit_tree", dev, _p(x2), _stride(xs, N, C), _p(k), ks, _p(v), vs, _p(g), _p(beta),
+            _p(conv_pool), _slot_stride(conv_pool), C, K, _p(s_pool), _slot_stride(s_pool),
+            s_pool.shape[0], _p(ids), _p(tree[0]), ids.numel(), _p(tree[1]), _p(accepted), tree[2],
+            N, HK, HV, DK, DV)
+
+
+def tree_slot_map(block_tables: torch.Tensor, context_lens: torch.Tensor,
+                  cu_seqlens: torch.Tensor, parents: torch.Tensor, max_nodes: int,
+                  block_size: int, n_rows: int, accepted=None):
+    """Positions (int64 [n_rows]) and cache slots (int32 [n_rows]) of all nodes,
+    from block_tables [n_seqs, max_blocks] int32, context_lens [n_seqs] and the
+    trees.  position = context length + depth.  Without ``accepted`` node i's slot is
+    that of logical position context length + i; with it (as :func:`commit_tree`)
+    the accepted path's nodes get the slot of their position and all others -1.
+    Rows behind the last sequence get position 0 and slot -1."""
+    dev = _one_device(block_tables, context_lens, cu_seqlens, parents, accepted)
+    assert block_tables.dim() == 2 and block_tables.dtype == torch.int32 and \
+        (block_tables.shape[1] <= 1 or block_tables.stride(1) == 1), \
+        "block_tables must be int32 [n_seqs, max_blocks] with dense rows"
+    n_seqs, n_blocks = block_tables.shape
+    tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, n_rows)
+    context_lens = _int32(context_lens, n_seqs, "context_lens")
+    if accepted is not None:
+        accepted = _int32(accepted, n_seqs, "accepted")
+    _debug_tree(tree, n_rows, accepted)
+    positions = torch.empty(n_rows, dtype=torch.int64, device=dev)
+    slots = torch.empty(n_rows, dtype=torch.int32, device=dev)
+    _launch("gdn_tree_slot_map", dev, _p(block_tables), _stride(block_tables.stride(0), n_seqs, n_blocks),
+            n_blocks, _p(context_lens), _p(tree[0]), n_seqs, _p(tree[1]), _p(accepted), tree[2],
+            int(block_size), n_rows, _p(positions), _p(slots))
+    return positions, slots
+
+
+def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, HKV: int, D: int):
+    """The strides (block, token, head) that both caches share."""
+    assert k_cache.dim() == 4 and tuple(k_cache.shape[2:]) == (HKV, D) and \
+        k_cache.shape == v_cache.shape, f"caches must be [blocks, block_size, {HKV}, {D}]"
+    assert k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16
+    assert k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1, \
+        "caches must have the same strides and dense heads"
+    # a dimension of one entry may have any stride: it is never stepped along
+    return tuple(k_cache.stride(i) if k_cache.shape[i] > 1 else max(k_cache.stride(i) // 8 * 8, D)
+                 for i in range(3))
+
+
+def qk_norm_rope_cache(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache,
+                       slot_mapping, eps: float = 1e-6, unit_offset: bool = False,
+                       out=None) -> torch.Tensor:
+    """RMS norm of every query and key head, the position rotation, and keys and
+    values into the paged cache.  q [N, HQ, D], k / v [N, HKV, D] bf16 (row views
+    allowed); q_weight / k_weight bf16 [D], used as 1 + w with ``unit_offset`` (the
+    hybrid model's norms); cos_sin fp32 [positions, R], R / 2 cosines then R / 2
+    sines: the first R elements of a head are rotated by halves; positions [N] int64;
+    k_cache / v_cache bf16 [blocks, block_size, HKV, D] (equal strides, dense heads),
+    written at slot_mapping [N] (block * block_size + token, -1: not stored).
+    Returns the rotated queries [N, HQ, D]; fp32 up to the one rounding at the end."""
+    dev = _one_device(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache,
+                      slot_mapping)
+    N, HQ, D, qs = _heads(q, "q")
+    N_k, HKV, D_k, ks = _heads(k, "k")
+    assert (N_k, D_k) == (N, D) and v.shape == k.shape
+    vs = _stride(_heads(v, "v")[3], N, HKV * D)
+    qs, ks = _stride(qs, N, HQ * D), _stride(ks, N, HKV * D)
+    assert q.dtype == k.dtype == v.dtype == torch.bfloat16
+    assert q_weight.dtype == k_weight.dtype == torch.bfloat16
+    assert q_weight.numel() == D and k_weight.numel() == D
+    assert cos_sin.dim() == 2 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous(), \
+        "cos_sin must be a contiguous fp32 [positions, rotary_dim]"
+    assert positions.dim() == 1 and positions.numel() == N and not positions.is_floating_point()
+    positions = _ids64(positions)
+    slot_mapping = _int32(slot_mapping, N, "slot_mapping")
+    bs, ts, hs = _paged_cache(k_cache, v_cache, HKV, D)
+    if not _aligned_rows(q, qs, 8):
+        q, qs = q.clone(memory_format=torch.contiguous_format), HQ * D
+    if not _aligned_rows(k, ks, 8):
+        k, ks = k.clone(memory_format=torch.contiguous_format), HKV * D
+    if not _aligned_rows(v, vs, 8):
+        v, vs = v.clone(memory_format=torch.contiguous_format), HKV * D
+    out = _out_buffer(out, (N, HQ, D), dev)
+    _launch("gdn_qk_norm_rope_cache", dev, _p(q), qs, _p(k), ks, _p(v), vs,
+            _p(q_weight.contiguous()), _p(k_weight.contiguous()), float(eps), int(unit_offset),
+            _p(cos_sin), cos_sin.shape[0], cos_sin.shape[1], _p(positions), _p(k_cache), _p(v_cache), bs, ts, hs, k_cache.shape[0], k_cache.shape[1],
+            _p(slot_mapping), _p(out), N, HQ, HKV, D)
+    return out
+
+
+def attention_tree(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, parents,
+                   max_nodes: int, max_len: int, scale: float | None = None,
+                   out=None) -> torch.Tensor:
+    """Attention of every node over its sequence's paged cache: positions
+    [0, context_lens[r]) and, at context_lens[r] + j, the nodes j on its path
+    (itself included), whose keys and values stand there already
+    (:func:`qk_norm_rope_cache`).  One node per sequence is the plain decode step.
+    q [N, HQ, D] bf16 (row views allowed), caches bf16 [blocks, block_size, HKV, D],
+    block_tables int32 [n_seqs, max_blocks], context_lens [n_seqs]; max_len bounds
+    context_lens[r] + the sequence's nodes (a longer sequence is skipped and
+    flagged).  ``scale`` defaults to D ** -0.5.  Returns out [N, HQ, D]."""
+    dev = _one_device(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, parents)
+    N, HQ, D, qs = _heads(q, "q")
+    qs = _stride(qs, N, HQ * D)
+    assert k_cache.dim() == 4
+    HKV = k_cache.shape[2]
+    assert q.dtype == torch.bfloat16 and HQ % HKV == 0
+    bs, ts, hs = _paged_cache(k_cache, v_cache, HKV, D)
+    assert block_tables.dim() == 2 and block_tables.dtype == torch.int32 and \
+        (block_tables.shape[1] <= 1 or block_tables.stride(1) == 1), \
+        "block_tables must be int32 [n_seqs, max_blocks] with dense rows"
+    n_seqs, n_blocks = block_tables.shape
+    tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, N)
+    context_lens = _int32(context_lens, n_seqs, "context_lens")
+    _debug_tree(tree, N)
+    if not _aligned_rows(q, qs, 8):
+        q, qs = q.clone(memory_format=torch.contiguous_format), HQ * D
+    out = _out_buffer(out, (N, HQ, D), dev)
+    max_len = int(max_len)
+    need = _lib.load().gdn_attention_tree_workspace_bytes(N, n_seqs, HQ, HKV, D, tree[2], max_len)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _launch("gdn_attention_tree", dev, _p(q), qs, _p(k_cache), _p(v_cache), bs, ts,
+            hs, k_cache.shape[0], k_cache.shape[1], _p(block_tables),
+            _stride(block_tables.stride(0), n_seqs, n_blocks), n_blocks, _p(context_lens), _p(tree[0]), n_seqs,
+            _p(tree[1]), tree[2], N, max_len, _p(out), HQ, HKV, D,
+            D ** -0.5 if scale is None else float(scale), _p(ws), need)
     return out
