@@ -355,7 +355,7 @@ int gdn_conv_gate_tree(const void* x, int64_t x_row_stride,
  * node's ancestors from the slot's stored state, which is only read.
  * Arguments as gdn_recurrent_inplace with n_tokens rows; s_pool is not written.
  * With z, out receives norm_weight * o * rsqrt(mean(o^2) + norm_eps) * silu(z)
- * in fp32, rounded once.  v and z rows: even strides, 4-byte aligned.
+ * in fp32, rounded once.  v, z and out: 8-byte aligned, row strides of whole fours.
  */
 int gdn_delta_rule_tree(const void* q, int64_t q_row_stride,
                         const void* k, int64_t k_row_stride,

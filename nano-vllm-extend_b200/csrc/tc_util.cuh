@@ -219,6 +219,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const void* tmap,
       "l"(tmap), "r"(x), "r"(y), "r"(mbar)
       : "memory");
 }
+// The same for a 3-D tensor map.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const void* tmap, int x, int y, int z,
+                                            uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst_smem),
+      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(mbar)
+      : "memory");
+}
 // TMA: 2-D tiled store shared -> global (the tensor map's box), tracked by the
 // issuing thread's bulk group.  Generic-proxy writes of the source must be
 // fenced (fence_async_smem) before the store is issued.

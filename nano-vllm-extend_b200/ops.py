@@ -830,11 +830,11 @@ def gated_delta_rule_tree(q, k, v, g, beta, s_pool, ids, cu_seqlens, parents, ma
     assert (N_q, HK_q, DK_q) == (N, HK, DK) and q.dtype == torch.bfloat16
     tree = _tree(cu_seqlens, parents, max_nodes, ids.numel(), N)
     _debug_tree(tree, N)
-    if not _aligned_rows(v, vs, 2):
+    if not _aligned_rows(v, vs, 4):
         v, vs = v.clone(memory_format=torch.contiguous_format), HV * DV
     z3, zs, nw = _norm_args(z, norm_weight, N, HV, DV)
     zs = _stride(zs, N, HV * DV)
-    if z3 is not None and not _aligned_rows(z3, zs, 2):
+    if z3 is not None and not _aligned_rows(z3, zs, 4):
         z3, zs = z3.clone(memory_format=torch.contiguous_format), HV * DV
     out = _out_buffer(out, (N, HV, DV), dev)
     _launch("gdn_delta_rule_tree", dev, _p(q), _stride(qs, N, HK * DK), _p(k), ks, _p(v), vs, _p(g),
