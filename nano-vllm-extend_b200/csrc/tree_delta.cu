@@ -19,22 +19,26 @@
 // Products are computed transposed, X^T = S_0^T [K; Q]^T with mma.sync: value
 // columns by 8 nodes, so few nodes waste little.  The results' layout is that of the
 // next product's A operand (nodes 2t, 2t + 1 as its k = t, t + 4), so X, d and o
-// never leave the warp's registers.  X is bf16 with fp32 sums: q and k are
-// exact, S_0 enters as two parts of 8 bits each; A, M and d meet in tf32, two parts
-// of 11 bits each (hi hi + lo hi + hi lo).  Norms, decays and the substitution
-// within eight nodes are fp32.
+// never leave the warp's registers.  X is bf16 with fp32 sums: q and k are exact,
+// S_0 enters as two parts of 8 bits each (cutting it to one tf32 part of 11 bits, no
+// instruction per element, saves 2 us of 99); A, M and d meet in tf32, two parts of
+// 11 bits each (hi hi + lo hi + hi lo).  Norms, decays and the substitution within
+// eight nodes are fp32.
 //
 // The chain of a unit (one sequence and v-head) is long and mostly latency:
 // norms, decays, gram factors, X, substitution, norm.  So the states come by TMA
 // (32-column boxes, 128-byte swizzle, which the fragment loads read without bank
 // conflicts) into a ring of ST buffers of a persistent CTA, independent of where
 // the arithmetic stands, and GROUPS groups of warps take the CTA's units in turn,
-// each a whole unit.  A buffer is refilled as soon as its group has formed X.  The
-// next unit's rows and scalars are loaded into registers a unit ahead.  Measured, 256
-// sequences x 32 heads of 3 to 8 nodes: state loaded into registers by its own CTA,
-// two CTAs an SM, 160-228 us (the loads stand still while a CTA computes); ring with
-// two groups of eight warps 174 us (1000 instructions per warp and unit, most of them
-// the same in every warp).  Hence few warps per unit, with 32 columns each.
+// each a whole unit.  A buffer is refilled as soon as its group has formed X.  Rows,
+// values and gates of the next unit are copied into shared memory a unit ahead
+// (cp.async): as loads into registers they made every other wait of the warp a wait
+// for memory (a warp has six scoreboards), 115 us where this takes 99.  Measured
+// so, 256 sequences x 32 heads of 3 to 8 nodes, the floor being 89 us: state loaded
+// into registers by its own CTA, two CTAs an SM, 160-228 us (the loads stand still
+// while a CTA computes); the ring with two groups of eight warps 174 (1000
+// instructions per warp and unit, most of them the same in every warp: hence few
+// warps per unit, with 32 columns each).
 //
 // A node whose own d is not finite (a NaN or infinity in its row) must not reach
 // nodes that do not descend from it: zero coefficients would still turn it into
@@ -56,18 +60,19 @@ struct TreeDelta {
   static constexpr int MT = TN <= 32 ? 2 : 1;
   static constexpr int VC = 2 * MT;                  // value columns of a thread, adjacent
   static constexpr int NW = D / (16 * MT), NT = 32 * NW;
-  static constexpr int GROUPS = TN <= 8 ? (D == 64 ? 4 : 3) : TN <= 16 ? (D == 64 ? 4 : 2) : TN <= 32 ? 2 : 1;
+  static constexpr int GROUPS = D == 64 ? (TN <= 8 ? 4 : TN <= 16 ? 3 : TN <= 32 ? 2 : 1)
+                                        : (TN <= 8 ? 3 : TN <= 32 ? 2 : 1);
   static constexpr int ST = TN <= 32 ? GROUPS : 2;
   // A buffer always serves the same group: when a group waits for a unit's state it
   // has used up the buffer's last one itself, so the parity it waits for is never
   // that of two copies ago.
   static_assert(ST % GROUPS == 0, "a buffer belongs to one group");
-  static constexpr bool AHEAD = TN <= 8;             // rows loaded a unit ahead
-  static constexpr int KP = D + 16;                  // pitches: conflict-free fragment loads
+  static constexpr bool AHEAD = TN <= 32;            // values and gates copied a unit ahead
+  static constexpr int KP = D + 8;                   // pitches: conflict-free fragment loads
   static constexpr int AP = TN + 4;
   static constexpr int MP = TN == 8 ? 8 : TN + 8;
   struct Group {
-    __align__(16) bf16 kq[2 * TN][KP];               // keys, then queries (k order: see frag)
+    __align__(16) bf16 kq[2 * TN][KP];               // keys, then queries
     float at[TN][AP];                                // at[i][j] = -A_ji
     float m[TN][MP];                                 // M
     float dec[TN][TN + 1];                           // D_ij, zero where j is no ancestor of i
@@ -75,6 +80,8 @@ struct TreeDelta {
     float norm[2 * TN];                              // 1 / |k|, scale / |q|
     __align__(16) float ssum[TN][NW];
     int par[2][TN];                                  // alternating: slow warps may still walk the last unit's
+    // values and gates: each thread's own pieces, [node of the thread][thread]
+    __align__(16) unsigned char vals[2][AHEAD ? TN / 4 * NT * MT * 4 : 16];
   };
   struct Smem {
     __align__(1024) unsigned char state[ST][D * D * 4];
@@ -83,9 +90,8 @@ struct TreeDelta {
   };
 };
 
-// Eight elements of a head row (vec: 16-byte aligned).
-__device__ __forceinline__ uint4 load8(const bf16* p, bool vec) {
-  if (vec) return *reinterpret_cast<const uint4*>(p);
+// Eight elements of an unaligned head row.
+__device__ __forceinline__ uint4 load8(const bf16* p) {
   uint4 u;
   bf16* h = reinterpret_cast<bf16*>(&u);
 #pragma unroll
@@ -96,11 +102,18 @@ __device__ __forceinline__ uint4 load8(const bf16* p, bool vec) {
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-// (x, y) as bf16 pairs, hi + lo, both cut: 16 bits of each.
-__device__ __forceinline__ void cut2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-  lo = __byte_perm(__float_as_uint(x - __uint_as_float(__float_as_uint(x) & 0xffff0000u)),
-                   __float_as_uint(y - __uint_as_float(__float_as_uint(y) & 0xffff0000u)), 0x7632);
+// The upper halves of two fp32 words: (x, y) cut to a bf16 pair.
+__device__ __forceinline__ uint32_t cut2(float x, float y) {
+  return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+}
+// What that leaves of each.
+__device__ __forceinline__ void rest2(float x, float y, float& rx, float& ry) {
+  const unsigned long long h = tc::f2pack(
+      __uint_as_float((__float_as_uint(x) & 0xffff0000u) ^ 0x80000000u),
+      __uint_as_float((__float_as_uint(y) & 0xffff0000u) ^ 0x80000000u));
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(tc::f2pack(x, y)), "l"(h));
+  tc::f2unpack(r, rx, ry);
 }
 
 // Substitution within eight nodes (lane t of a quad holds nodes 2t, 2t + 1; r[0],
@@ -162,7 +175,8 @@ struct DeltaArgs {
   int max_nodes;
   int64_t n_tokens;
   bf16* out;
-  int HK, HV, units;
+  int HV, units;
+  unsigned rep_magic;   // ceil(2^32 / v-heads per k-head), so that h * it >> 32 is the k-head (h < 2^16); 0: one
   float scale;
   const bf16* z;
   int64_t zs;
@@ -204,9 +218,12 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
   constexpr int NT = P::NT, NW = P::NW, ST = P::ST, GROUPS = P::GROUPS, MT = P::MT, VC = P::VC;
   constexpr int KB = D / 16, KT = TN / 8;
   constexpr int PC = D / 8, PPT = 2 * TN * PC / NT;   // 16-byte pieces of q / k per thread
-  // gram tiles of 16 rows x 8 columns that hold a column <= some row, per half (keys, queries)
-  constexpr int MH = TN / 16, TH = MH * (MH + 1), GT = TN == 8 ? 1 : (2 * TH + NW - 1) / NW;
-  static_assert(2 * TN * PC % NT == 0 && TN <= NT, "thread layout");
+  constexpr int NPP = NT / PC;                       // rows from one piece of a thread to the next
+  // gram tiles of 16 rows x 8 columns: [K; Q] K^T where some column <= some row, TH per
+  // half, then the diagonal ones of Q Q^T, for the norms
+  constexpr int MH = TN / 16, TH = MH * (MH + 1), TILES = TN == 8 ? 2 : 2 * TH + 2 * MH;
+  constexpr int GT = (TILES + NW - 1) / NW;
+  static_assert(PPT % 2 == 0 && NT % PC == 0 && 2 * TN * PC % NT == 0 && TN <= NT, "thread layout");
   extern __shared__ unsigned char smem_raw[];
   auto& sm = *reinterpret_cast<typename P::Smem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -239,9 +256,8 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
     return d;
   };
   // the state of the CTA's i-th unit into its buffer (one thread)
-  const auto fetch = [&](int i, const DeltaAt& at, const DeltaRaw& r) {
+  const auto fetch = [&](int i, const DeltaUnit& d) {
     if (i >= count) return;
-    const DeltaUnit d = unit_of(i, at, r, nullptr);
     const uint32_t bar = tc::smem_u32(&sm.full[i % ST]);
     if (d.n == 0) {
       tc::mbar_arrive(bar);
@@ -262,37 +278,75 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
   DeltaAt at_cur = first.step(group, a.HV), at_nxt = at_cur.step(GROUPS, a.HV);
   const DeltaRaw raw_cur = raw_of(at_cur), raw_nxt = raw_of(at_nxt);
   __syncthreads();
-  if (tid == 0) {
-    fetch(group, at_cur, raw_cur);
-    for (int i = group + GROUPS; i < ST; i += GROUPS) {
-      const DeltaAt at = first.step(i, a.HV);
-      fetch(i, at, raw_of(at));
-    }
-  }
-
-  // a unit's rows and scalars, loaded ahead
-  uint4 piece[PPT];
-  int my_par = -1;
-  float my_g = 0.f, my_beta = 0.f;
-  uint32_t vr[KT][2][MT], zr[KT][2][MT];
-  const int c = warp * 16 * MT + VC * gr;            // this thread's value columns: c .. c + VC - 1
-  const auto load_rows = [&](const DeltaUnit& d) {
-    const int hk = d.h / (a.HV / a.HK);
-#pragma unroll
-    for (int i = 0; i < PPT; ++i) {
-      const int p = tid + i * NT, row = p / PC, node = row % TN, ch = (p - row * PC) * 8;
-      piece[i] = make_uint4(0, 0, 0, 0);
-      if (node < d.n)
-        piece[i] = load8((row < TN ? a.k + (d.start + node) * a.ks : a.q + (d.start + node) * a.qs) +
-                             (int64_t)hk * D + ch, a.vec);
-    }
-    if (tid < d.n) {
-      my_par = a.parents[d.start + tid];
-      my_g = a.g[(d.start + tid) * a.HV + d.h];
-      my_beta = bf2f(a.beta[(d.start + tid) * a.HV + d.h]);
+  // bounded: the state of the CTA's i-th unit has arrived
+  const auto await_state = [&](int i) {
+    const uint32_t bar = tc::smem_u32(&sm.full[i % ST]);
+    if (!tc::mbar_wait(bar, (i / ST) & 1, kDeltaWait)) {
+      if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
+      tc::mbar_wait(bar, (i / ST) & 1, kDeltaWait);
     }
   };
-  const auto load_vals = [&](uint32_t (&r)[KT][2][MT], const bf16* p, int64_t stride,
+
+  // a unit's scalars, loaded ahead
+  int my_par = -1;
+  float my_g = 0.f, my_beta = 0.f;
+  const int c = warp * 16 * MT + VC * gr;            // this thread's value columns: c .. c + VC - 1
+  // q / k rows to shared memory (zero rows behind the last node), a thread's first
+  // pieces keys, the others queries; and the nodes' scalars to registers
+  const int node0 = tid / PC, ch = tid % PC * 8;
+  const int64_t koff = node0 * a.ks + ch, qoff = node0 * a.qs + ch;
+  const auto load_rows = [&](const DeltaUnit& d) {
+    const int hk = a.rep_magic ? (int)__umulhi((unsigned)d.h, a.rep_magic) : d.h;
+    const bf16* kp = a.k + d.start * a.ks + hk * D + koff;
+    const bf16* qp = a.q + d.start * a.qs + hk * D + qoff;
+#pragma unroll
+    for (int i = 0; i < PPT / 2; ++i) {
+      const int node = node0 + i * NPP;
+      bf16 *kd = &gs.kq[node][ch], *qd = &gs.kq[TN + node][ch];
+      if (a.vec) {
+        const uint32_t bytes = node < d.n ? 16u : 0u;
+        tc::cp_async16(tc::smem_u32(kd), bytes ? kp + i * NPP * a.ks : a.k, bytes);
+        tc::cp_async16(tc::smem_u32(qd), bytes ? qp + i * NPP * a.qs : a.q, bytes);
+      } else {
+        uint4 u = make_uint4(0, 0, 0, 0), w = u;
+        if (node < d.n) {
+          u = load8(kp + i * NPP * a.ks);
+          w = load8(qp + i * NPP * a.qs);
+        }
+        *reinterpret_cast<uint4*>(kd) = u;
+        *reinterpret_cast<uint4*>(qd) = w;
+      }
+    }
+    tc::cp_async_commit();
+    if (tid < d.n) {
+      const int64_t at = (d.start + tid) * a.HV + d.h;
+      my_par = a.parents[d.start + tid];
+      my_g = a.g[at];
+      my_beta = bf2f(a.beta[at]);
+    }
+  };
+  // values (which 0) or gates (1) of a unit: copied into the thread's own pieces of
+  // shared memory (which ties up no register while it is under way), and read back; or,
+  // where there is no room for that, loaded
+  const auto copy_vals = [&](int which, const bf16* p, int64_t stride, const DeltaUnit& d) {
+    if constexpr (P::AHEAD) {
+      const bf16* base = p + d.start * stride + (int64_t)d.h * D + c;
+#pragma unroll
+      for (int j = 0; j < TN / 4; ++j) {
+        const int node = j / 2 * 8 + 2 * tq + j % 2;
+        const uint32_t dst = tc::smem_u32(&gs.vals[which][(j * NT + tid) * MT * 4]);
+        const uint32_t bytes = node < d.n ? MT * 4u : 0u;
+        const bf16* src = bytes ? base + node * stride : p;
+        if constexpr (MT == 2)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                       : "memory");
+        else
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                       : "memory");
+      }
+    }
+  };
+  const auto load_vals = [&](uint32_t (&r)[KT][2][MT], int which, const bf16* p, int64_t stride,
                              const DeltaUnit& d) {
     const bf16* base = p + d.start * stride + (int64_t)d.h * D + c;
 #pragma unroll
@@ -300,86 +354,83 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int node = t8 * 8 + 2 * tq + e;
-        const bool on = node < d.n;
+        const unsigned char* src =
+            P::AHEAD ? &gs.vals[which][((t8 * 2 + e) * NT + tid) * MT * 4]
+                     : reinterpret_cast<const unsigned char*>(base + node * stride);
+        const bool on = P::AHEAD || node < d.n;
         if constexpr (MT == 2) {
           uint2 u = make_uint2(0u, 0u);
-          if (on) u = *reinterpret_cast<const uint2*>(base + node * stride);
+          if (on) u = *reinterpret_cast<const uint2*>(src);
           r[t8][e][0] = u.x;
           r[t8][e][1] = u.y;
         } else {
-          r[t8][e][0] = on ? *reinterpret_cast<const uint32_t*>(base + node * stride) : 0u;
+          r[t8][e][0] = on ? *reinterpret_cast<const uint32_t*>(src) : 0u;
         }
       }
   };
-  // k-elements of row r, block kb, as this lane's fragments take them (k 2t, 2t + 1
-  // and 2t + 8, 2t + 9): in shared memory those four of each 16 are adjacent
-  const auto frag = [&](int r, int kb) {
-    return *reinterpret_cast<const uint2*>(&gs.kq[r][kb * 16 + 4 * tq]);
+  // B fragments of eight-row tiles r0 and r0 + 8, block kb: (k low, k high) of each
+  const uint32_t kq0 = tc::smem_u32(&gs.kq[0][0]);
+  const uint32_t b_lane = kq0 + (((lane >> 4) * 8 + (lane & 7)) * P::KP + ((lane >> 3) & 1) * 8) * 2;
+  const auto frag2 = [&](int r0, int kb, uint32_t (&b)[4]) {
+    mm::ldsm4(b, b_lane + (r0 * P::KP + kb * 16) * 2);
   };
-  // gram tile -> first row, first column
+  // gram tile -> first row, first column's row
   const auto tile_at = [&](int tile, int& row0, int& col0) {
     if constexpr (TN == 8) {
-      row0 = col0 = 0;
-      return tile == 0;
-    } else {
+      row0 = 0;
+      col0 = tile * 8;
+    } else if (tile < 2 * TH) {
       const int half = tile / TH, rem = tile - half * TH;
       int mt = 0;
       while ((mt + 1) * (mt + 2) <= rem) ++mt;
       row0 = half * TN + mt * 16;
       col0 = (rem - mt * (mt + 1)) * 8;
-      return tile < 2 * TH;
+    } else {
+      row0 = TN + (tile - 2 * TH) / 2 * 16;
+      col0 = TN + (tile - 2 * TH) * 8;
     }
+    return tile < TILES;
   };
   float nwv[VC];
 #pragma unroll
   for (int e = 0; e < VC; ++e) nwv[e] = NORM ? bf2f(a.nw[c + e]) : 1.f;
 
   int32_t* const flags = tid == 0 ? a.status : nullptr;
-  DeltaAt at_fill = at_cur.step(ST, a.HV);
+  DeltaRaw after = raw_nxt;
   DeltaUnit cur = unit_of(group, at_cur, raw_cur, flags);
   DeltaUnit nxt = unit_of(group + GROUPS, at_nxt, raw_nxt, flags);
-  if constexpr (P::AHEAD) {
-    load_rows(cur);
-    load_vals(vr, a.v, a.vs, cur);
-    if constexpr (NORM) load_vals(zr, a.z, a.zs, cur);
+  if (tid == 0) {
+    fetch(group, cur);
+    if constexpr (ST > GROUPS) fetch(group + GROUPS, nxt);
   }
+  // three groups of copies are under way per thread and unit, in this order: rows,
+  // values, gates; waiting for all but the last two is waiting for the next one
+  load_rows(cur);
+  copy_vals(0, a.v, a.vs, cur);
+  tc::cp_async_commit();
+  if constexpr (NORM) copy_vals(1, a.z, a.zs, cur);
+  tc::cp_async_commit();
+  const auto refill = [&](int i) {                   // unit i has used up its buffer
+    if constexpr (ST == GROUPS) fetch(i + ST, nxt);
+    else fetch(i + ST, unit_of(i + ST, at_nxt.step(ST - GROUPS, a.HV), raw_of(at_nxt.step(ST - GROUPS, a.HV)), nullptr));
+  };
   for (int i = group; i < count; i += GROUPS) {
     const DeltaAt at_after = at_nxt.step(GROUPS, a.HV);
-    const DeltaRaw after = raw_of(at_after), fill = raw_of(at_fill);
-    const uint32_t bar = tc::smem_u32(&sm.full[i % ST]);
+    if (at_after.seq != at_nxt.seq) after = raw_of(at_after);
     const int n = cur.n;
     int* par = gs.par[(i / GROUPS) & 1];
     if (n == 0) {                                    // nothing to compute: the buffer is free at once
       if (tid == 0) {
-        if (!tc::mbar_wait(bar, (i / ST) & 1, kDeltaWait) && a.status)
-          atomicOr(a.status, GDN_STATUS_TIMEOUT);
-        fetch(i + ST, at_fill, fill);
+        await_state(i);
+        refill(i);
       }
-      if constexpr (P::AHEAD) {
-        load_rows(nxt);
-        load_vals(vr, a.v, a.vs, nxt);
-        if constexpr (NORM) load_vals(zr, a.z, a.zs, nxt);
-      }
+      tc::cp_async_wait<0>();                        // the next unit's rows go where these went
+      load_rows(nxt);
+      copy_vals(0, a.v, a.vs, nxt);
+      tc::cp_async_commit();
+      if constexpr (NORM) copy_vals(1, a.z, a.zs, nxt);
+      tc::cp_async_commit();
     } else {
-      if constexpr (!P::AHEAD) load_rows(cur);
-      // q / k rows to shared memory (zero rows behind the last node) and their norms
-#pragma unroll
-      for (int j = 0; j < PPT; ++j) {
-        const int p = tid + j * NT, row = p / PC, pc = p - row * PC;
-        float f[8], ss = 0.f;
-        unpack8(piece[j], f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
-#pragma unroll
-        for (int o = PC / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (pc == 0) gs.norm[row] = rsqrtf(ss + 1e-6f) * (row < TN ? 1.f : a.scale);
-        // elements 2t, 2t + 1 of the piece go to place 4t (first half of 16) or 4t + 2
-        bf16* dst = &gs.kq[row][(pc >> 1) * 16 + (pc & 1) * 2];
-        *reinterpret_cast<uint32_t*>(dst) = piece[j].x;
-        *reinterpret_cast<uint32_t*>(dst + 4) = piece[j].y;
-        *reinterpret_cast<uint32_t*>(dst + 8) = piece[j].z;
-        *reinterpret_cast<uint32_t*>(dst + 12) = piece[j].w;
-      }
       for (int j = tid; j < TN * (TN + 1); j += NT) (&gs.dec[0][0])[j] = 0.f;
       if (tid < TN) {
         const bool on = tid < n;
@@ -387,9 +438,8 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
         gs.eg[tid] = on ? expf(my_g) : 0.f;
         gs.beta[tid] = on ? my_beta : 0.f;
       }
-      if constexpr (P::AHEAD) load_rows(nxt);
-      else load_vals(vr, a.v, a.vs, cur);
-      group_sync();
+      tc::cp_async_wait<2>();
+      group_sync();                                  // rows and scalars are there
 
       // decays: thread j walks from node j to the root
       if (tid < TN) {
@@ -404,7 +454,7 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
           }
         gs.d0[tid] = tid < n ? d : 0.f;
       }
-      // gram tiles [K; Q] K^T, the last warps first: the first ones walk the trees
+      // gram tiles, the last warps first: the first ones walk the trees
       float gram[GT][4];
 #pragma unroll
       for (int j = 0; j < GT; ++j) {
@@ -412,20 +462,29 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
 #pragma unroll
         for (int e = 0; e < 4; ++e) gram[j][e] = 0.f;
         if (tile_at(NW - 1 - warp + j * NW, row0, col0)) {
+          const uint32_t a_addr = kq0 + ((row0 + (lane & 15)) * P::KP + (lane >> 4) * 8) * 2;
+          const uint32_t b_addr = kq0 + ((col0 + (lane & 7)) * P::KP + (lane >> 3) * 8) * 2;
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            const uint2 fa = frag(row0 + gr, kb), fb = frag(row0 + gr + 8, kb), fc = frag(col0 + gr, kb);
-            const uint32_t fr[4] = {fa.x, fb.x, fa.y, fb.y};
-            mm::mma16816(gram[j], fr, fc.x, fc.y);
+          for (int kb = 0; kb < KB; kb += 2) {
+            uint32_t f[4], b[4];
+            mm::ldsm4(b, b_addr + kb * 32);
+            mm::ldsm4(f, a_addr + kb * 32);
+            mm::mma16816(gram[j], f, b[0], b[1]);
+            mm::ldsm4(f, a_addr + kb * 32 + 32);
+            mm::mma16816(gram[j], f, b[2], b[3]);
+          }
+          // the diagonal: norms
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = row0 + gr + (e >> 1) * 8;
+            if (row == col0 + 2 * tq + (e & 1))
+              gs.norm[row] = rsqrtf(gram[j][e] + 1e-6f) * (row < TN ? 1.f : a.scale);
           }
         }
       }
 
       // X^T = S_0^T [K; Q]^T
-      if (!tc::mbar_wait(bar, (i / ST) & 1, kDeltaWait)) {
-        if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
-        tc::mbar_wait(bar, (i / ST) & 1, kDeltaWait);
-      }
+      await_state(i);
       float acc[2 * KT][MT][4];
 #pragma unroll
       for (int t8 = 0; t8 < 2 * KT; ++t8)
@@ -447,33 +506,43 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
             if constexpr (VC == 4) *reinterpret_cast<float4*>(s[j]) = *reinterpret_cast<const float4*>(p);
             else *reinterpret_cast<float2*>(s[j]) = *reinterpret_cast<const float2*>(p);
           }
+          float l[4][VC];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < VC; e += 2) rest2(s[j][e], s[j][e + 1], l[j][e], l[j][e + 1]);
           uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              cut2(s[(e >> 1) * 2][2 * mt + (e & 1)], s[(e >> 1) * 2 + 1][2 * mt + (e & 1)], hi[mt][e],
-                   lo[mt][e]);
-#pragma unroll
-          for (int t8 = 0; t8 < 2 * KT; ++t8) {
-            const uint2 b = frag(t8 * 8 + gr, kb);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mm::mma16816(acc[t8][mt], hi[mt], b.x, b.y);
-              mm::mma16816(acc[t8][mt], lo[mt], b.x, b.y);
+            for (int e = 0; e < 4; ++e) {
+              const int j = (e >> 1) * 2, col = 2 * mt + (e & 1);
+              hi[mt][e] = cut2(s[j][col], s[j + 1][col]);
+              lo[mt][e] = cut2(l[j][col], l[j + 1][col]);
             }
+#pragma unroll
+          for (int t8 = 0; t8 < 2 * KT; t8 += 2) {
+            uint32_t b[4];
+            frag2(t8 * 8, kb, b);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                mm::mma16816(acc[t8 + u][mt], hi[mt], b[2 * u], b[2 * u + 1]);
+                mm::mma16816(acc[t8 + u][mt], lo[mt], b[2 * u], b[2 * u + 1]);
+              }
           }
         }
       }
-      if constexpr (!P::AHEAD && NORM) load_vals(zr, a.z, a.zs, cur);
-      group_sync();                                  // decays complete, the buffer is free
-      if (tid == 0) fetch(i + ST, at_fill, fill);
+      group_sync();                                  // decays complete; state and rows are used up
+      if (tid == 0) refill(i);
+      load_rows(nxt);
 
       // gram tiles -> the factors -A and M
 #pragma unroll
       for (int j = 0; j < GT; ++j) {
         int row0, col0;
-        if (tile_at(NW - 1 - warp + j * NW, row0, col0)) {
+        if (tile_at(NW - 1 - warp + j * NW, row0, col0) && col0 < TN) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int row = row0 + gr + (e >> 1) * 8, ci = col0 + 2 * tq + (e & 1), node = row % TN;
@@ -485,6 +554,9 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
         }
       }
       // right sides (keys) and the state's part of the outputs (queries)
+      tc::cp_async_wait<2>();
+      uint32_t vr[KT][2][MT], zr[KT][2][MT];
+      load_vals(vr, 0, a.v, a.vs, cur);
 #pragma unroll
       for (int t8 = 0; t8 < KT; ++t8)
 #pragma unroll
@@ -501,7 +573,8 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
             acc[KT + t8][mt][2 + e] *= fq;
           }
         }
-      if constexpr (P::AHEAD) load_vals(vr, a.v, a.vs, nxt);
+      copy_vals(0, a.v, a.vs, nxt);
+      tc::cp_async_commit();
       group_sync();                                  // the factors are complete
 
       unsigned long long bad = 0;
@@ -590,6 +663,8 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
             ss += __shfl_xor_sync(0xffffffffu, ss, 16);
             if (gr == 0) gs.ssum[t8 * 8 + 2 * tq + e][warp] = ss;
           }
+        tc::cp_async_wait<2>();
+        load_vals(zr, 1, a.z, a.zs, cur);
         group_sync();
       }
       bf16* obase = a.out + (cur.start * a.HV + cur.h) * D + c;
@@ -622,12 +697,12 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
           else
             *reinterpret_cast<uint32_t*>(to) = mm::pack2(o[0], o[1]);
         }
-      if constexpr (P::AHEAD && NORM) load_vals(zr, a.z, a.zs, nxt);
+      if constexpr (NORM) copy_vals(1, a.z, a.zs, nxt);
+      tc::cp_async_commit();
     }
     cur = nxt;
     nxt = unit_of(i + 2 * GROUPS, at_after, after, flags);
     at_nxt = at_after;
-    at_fill = at_fill.step(GROUPS, a.HV);
   }
 }
 
@@ -691,7 +766,8 @@ extern "C" int gdn_delta_rule_tree(const void* q, int64_t q_row_stride, const vo
                       ((uintptr_t)v | (uintptr_t)z | (uintptr_t)out) % 8 == 0,
                   "%s: v, z and out must be 8-byte aligned with row strides of whole fours", fn);
   const int64_t units = (int64_t)n_seqs * num_v_heads;
-  GDN_UNSUPPORTED(units < (1ll << 30), "%s: too many (sequence, head) units", fn);
+  GDN_UNSUPPORTED(units < (1ll << 30) && num_v_heads <= 65535, "%s: too many (sequence, head) units",
+                  fn);
   // the pool's view as rows of value columns, [slots][HV * DK][DV]
   const EncodeTiledFn encode = encode_tiled();
   const cuuint64_t dims[3] = {(cuuint64_t)head_v_dim, (cuuint64_t)num_v_heads * head_k_dim,
@@ -707,9 +783,11 @@ extern "C" int gdn_delta_rule_tree(const void* q, int64_t q_row_stride, const vo
     set_error("%s: the pool's tensor map could not be encoded", fn);
     return GDN_ERR_CUDA;
   }
+  const int rep = num_v_heads / num_k_heads;
   const DeltaArgs a{(const bf16*)q, (const bf16*)k, (const bf16*)v, q_row_stride, k_row_stride,
                     v_row_stride, g, (const bf16*)beta, num_slots, ids, cu_seqlens, parents,
-                    max_nodes, n_tokens, (bf16*)out, num_k_heads, num_v_heads, (int)units, scale,
+                    max_nodes, n_tokens, (bf16*)out, num_v_heads, (int)units,
+                    rep == 1 ? 0u : (unsigned)(((1ull << 32) + rep - 1) / rep), scale,
                     (const bf16*)z, z_row_stride, (const bf16*)norm_weight, norm_eps,
                     aligned16(q) && aligned16(k) && q_row_stride % 8 == 0 && k_row_stride % 8 == 0,
                     status};

@@ -179,6 +179,30 @@ def test_delta_rule(ops, HK, HV, D, lens, chain, norm):
     assert ops.check_status() == 0
 
 
+@pytest.mark.parametrize("HK,HV,D,nodes", [(2, 8, 128, 8), (2, 4, 64, 8), (2, 4, 128, 13),
+                                          (1, 3, 64, 16), (1, 3, 128, 30), (2, 2, 64, 64),
+                                          (1, 2, 128, 40)])
+def test_delta_rule_many_units(ops, HK, HV, D, nodes):
+    """Many units per CTA, so every buffer is used again and again; empty sequences and
+    a slot that is not one among them."""
+    r = np.random.default_rng(D + nodes)
+    lens = [int(x) for x in r.integers(0, nodes + 1, 150)]
+    lens[0], lens[7], lens[8], lens[20] = nodes, 0, 0, 3
+    c = Gdn(HK, HV, D, lens, seed=nodes)
+    out = torch.zeros(c.N, HV, D, dtype=torch.bfloat16, device=DEV)
+    ids = c.d_ids.clone()
+    c.d_ids[20] = c.slots
+    c.delta(ops, True, out=out)
+    with pytest.raises(IndexError):
+        ops.check_status()
+    start = sum(lens[:20])
+    assert (out[start:start + 3] == 0).all()
+    c.d_ids = ids
+    close(c.delta(ops, True), c.delta_ref(True), 2.0 ** -12)
+    again = c.delta(ops, True)
+    assert torch.equal(again, c.delta(ops, True)) and ops.check_status() == 0
+
+
 @pytest.mark.parametrize("D", [128, 64])
 def test_delta_rule_extreme_gates(ops, D):
     """No decay, total decay (-inf and far below exp's range), write strengths 0 and 1."""
