@@ -14,14 +14,18 @@
 // A CTA owns one (sequence, v-head); a warp owns 16 value columns and keeps its
 // part of the state in registers from the one read to the one write: a lane
 // holds 4 columns (float4) of DK / 8 rows.  S^T k^ then needs a sum over the 8
-// lanes of a column group only, by shuffles: no CTA barrier between tokens.
-// Keys and values are staged for eight tokens at a time.  The conv windows are
-// rolled by further CTAs of the same launch.
+// lanes of a column group only, by shuffles, and |k| likewise: no CTA barrier
+// between tokens.  What is small is asked for before the state, behind which it would
+// queue; in trees of up to kStaged nodes that is every node's key and value, whatever
+// path is accepted, so that nothing waits for the path (268 -> 199 us for 256
+// sequences x 32 heads of 3 to 8 nodes, floor 168).  Larger trees stage their path's
+// rows, kStaged at a time.  The conv windows are rolled by further CTAs of the same launch.
+#include "tc_util.cuh"
 #include "tree.cuh"
 
 namespace gdn {
 
-constexpr int kCommitTokens = 8;
+constexpr int kStaged = 16;
 
 struct CommitConv {
   const bf16* x;
@@ -29,21 +33,46 @@ struct CommitConv {
   bf16* pool;
   int64_t slot_stride;
   int channels, kernel, ctas;   // ctas: CTAs per sequence
+  bool vec;                     // eight channels per thread (16-byte aligned)
 };
 
+// Eight channels' windows of T taps: M path rows (the newest first) enter.
+template <int T, int M>
+__device__ __forceinline__ void roll8(bf16* sp, const uint4 (&rows)[3]) {
+  uint4 old[T], out[T];
+#pragma unroll
+  for (int j = 0; j < T; ++j) old[j] = reinterpret_cast<const uint4*>(sp)[j];
+  const bf16* o = reinterpret_cast<const bf16*>(old);
+  bf16* n = reinterpret_cast<bf16*>(out);
+#pragma unroll
+  for (int ch = 0; ch < 8; ++ch)
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+      n[ch * T + j] = j + M < T ? o[ch * T + j + M] : reinterpret_cast<const bf16*>(&rows[T - 1 - j])[ch];
+#pragma unroll
+  for (int j = 0; j < T; ++j) reinterpret_cast<uint4*>(sp)[j] = out[j];
+}
+
+template <int T>
+__device__ __forceinline__ void roll8(bf16* sp, const uint4 (&rows)[3], int m) {
+  if (m >= T) roll8<T, T>(sp, rows);
+  else if (m == 1) roll8<T, 1>(sp, rows);
+  else if constexpr (T > 2) roll8<T, 2>(sp, rows);
+}
+
 template <int DK, int DV>
-__global__ void __launch_bounds__(DV * 2) commit_tree_kernel(
+__global__ void __launch_bounds__(DV * 2, DV == 128 ? 2 : 4) commit_tree_kernel(
     const bf16* __restrict__ k, int64_t ks, const bf16* __restrict__ v, int64_t vs,
     const float* __restrict__ g, const bf16* __restrict__ beta, float* __restrict__ pool,
     int64_t slot_stride, int64_t num_slots, const int64_t* __restrict__ ids,
     const int32_t* __restrict__ cu, const int32_t* __restrict__ parents,
     const int32_t* __restrict__ accepted, int max_nodes, int64_t n_tokens, int n_seqs, int HK,
-    int HV, const CommitConv conv, int32_t* status) {
-  constexpr int NT = DV * 2, NW = NT / 32, RPL = DK / 8, KP = RPL + 4;
-  __shared__ __align__(16) float sk[kCommitTokens][8 * KP];   // row group rl at rl * KP
-  __shared__ __align__(16) float sv[kCommitTokens][DV];
-  __shared__ float seg[kCommitTokens], sbeta[kCommitTokens];
-  __shared__ int spar[kMaxTreeNodes], spath[kMaxTreeNodes], sdepth;
+    int HV, bool vec, const CommitConv conv, int32_t* status) {
+  constexpr int NT = DV * 2, RPL = DK / 8, PK = DK / 8;
+  __shared__ __align__(16) bf16 sk[kStaged][DK];
+  __shared__ __align__(16) bf16 sv[kStaged][DV];
+  __shared__ float sg[kMaxTreeNodes], sbeta[kMaxTreeNodes];
+  __shared__ int spar[kMaxTreeNodes];
 
   const int64_t units = (int64_t)n_seqs * HV;
   const bool is_conv = blockIdx.x >= units;
@@ -52,125 +81,167 @@ __global__ void __launch_bounds__(DV * 2) commit_tree_kernel(
   int64_t start;
   int n;
   const int64_t slot = ids[seq];
-  if (!tree_rows(cu, seq, n_tokens, max_nodes, status, start, n)) return;
   const int last = accepted[seq];
+  if (!tree_rows(cu, seq, n_tokens, max_nodes, status, start, n)) return;
   if (last < -1 || last >= n) {
     if (status) atomicOr(status, GDN_STATUS_BAD_TREE);
     return;
   }
   if (last < 0) return;
   if (!slot_ok(slot, num_slots, status)) return;
-  // a malformed tree leaves both pools alone (every CTA of the sequence sees all of it)
-  bool malformed = false;
-  if (tid < n) {
-    const int p = parents[start + tid];
-    malformed = p < -1 || p >= tid;
-    spar[tid] = p;
+  const int h = is_conv ? 0 : (int)(blockIdx.x - (int64_t)seq * HV), hk = h / (HV / HK);
+
+  int my_par = -1;
+  if (tid < n) my_par = parents[start + tid];
+  // m rows of keys and values into the staging buffers, all threads together
+  const auto stage = [&](int m, const auto& node_of) {
+    for (int i = tid; i < m * 2 * PK; i += NT) {
+      const int r = i / (2 * PK), pc = i - r * 2 * PK, c8 = pc % PK * 8;
+      const int64_t row = start + node_of(r);
+      const bf16* src = pc < PK ? k + row * ks + (int64_t)hk * DK + c8
+                                : v + row * vs + (int64_t)h * DV + c8;
+      bf16* dst = pc < PK ? &sk[r][c8] : &sv[r][c8];
+      if (vec) {
+        tc::cp_async16(tc::smem_u32(dst), src, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dst[e] = src[e];
+      }
+    }
+  };
+  if (!is_conv) {
+    if (n <= kStaged) stage(n, [](int r) { return r; });
+    if (tid < n) {
+      sg[tid] = g[(start + tid) * HV + h];
+      sbeta[tid] = bf2f(beta[(start + tid) * HV + h]);
+    }
   }
-  if (__syncthreads_or(malformed)) {
+
+  const int warp = tid >> 5, lane = tid & 31, cl = lane & 3, rl = lane >> 2;
+  const int c = warp * 16 + 4 * cl;
+  float* sp = pool + slot * slot_stride + (int64_t)h * DK * DV + (int64_t)(rl * RPL) * DV + c;
+  float4 s[RPL];
+  if (!is_conv) {
+#pragma unroll
+    for (int i = 0; i < RPL; ++i) s[i] = __ldcs(reinterpret_cast<const float4*>(sp + i * DV));
+  }
+
+  // a malformed tree leaves both pools alone (every CTA of the sequence sees all of it)
+  if (tid < n) spar[tid] = my_par;
+  tc::cp_async_commit();
+  tc::cp_async_wait<0>();
+  if (__syncthreads_or(tid < n && (my_par < -1 || my_par >= tid))) {
     if (status && tid == 0) atomicOr(status, GDN_STATUS_BAD_TREE);
     return;
   }
 
   if (is_conv) {
-    const int c = (int)((blockIdx.x - units) % conv.ctas) * NT + tid;
-    if (c >= conv.channels) return;
     const int T = conv.kernel - 1;
-    bf16* sp = conv.pool + slot * conv.slot_stride + (int64_t)c * T;
-    bf16 nw[3];
+    const int c0 = ((int)((blockIdx.x - units) % conv.ctas) * NT + tid) * (conv.vec ? 8 : 1);
+    if (c0 >= conv.channels) return;
+    bf16* to = conv.pool + slot * conv.slot_stride + (int64_t)c0 * T;
     int at = last, m = 0;              // the path's newest T rows, newest first
-    for (; m < T && at >= 0; ++m) {
-      nw[m] = conv.x[(start + at) * conv.xs + c];
-      at = spar[at];
+    if (conv.vec) {
+      uint4 rows[3];
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < T && at >= 0) {
+          rows[j] = *reinterpret_cast<const uint4*>(conv.x + (start + at) * conv.xs + c0);
+          at = spar[at];
+          ++m;
+        }
+      if (T == 3) roll8<3>(to, rows, m);
+      else if (T == 2) roll8<2>(to, rows, m);
+      else roll8<1>(to, rows, m);
+      return;
     }
-    bf16 old[3];
-    for (int j = 0; j + m < T; ++j) old[j] = sp[j + m];
-    for (int j = 0; j < T; ++j) sp[j] = j + m < T ? old[j] : nw[T - 1 - j];
+    bf16 nw[3], old[3];
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < T && at >= 0) {
+        nw[j] = conv.x[(start + at) * conv.xs + c0];
+        at = spar[at];
+        ++m;
+      }
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < T) old[j] = to[j];
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < T) {
+        // tap j: old tap j + m, or the path's row T - 1 - j
+        bf16 x = nw[0];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          if (j + m < T && i == j + m) x = old[i];
+          if (j + m >= T && i == T - 1 - j) x = nw[i];
+        }
+        to[j] = x;
+      }
     return;
   }
 
-  const int h = (int)(blockIdx.x - (int64_t)seq * HV), hk = h / (HV / HK);
-  const int warp = tid >> 5, lane = tid & 31, cl = lane & 3, rl = lane >> 2;
-  const int c = warp * 16 + 4 * cl;
-  float* sp = pool + slot * slot_stride + (int64_t)h * DK * DV + (int64_t)(rl * RPL) * DV + c;
-  float4 s[RPL];
-#pragma unroll
-  for (int i = 0; i < RPL; ++i) s[i] = __ldcs(reinterpret_cast<const float4*>(sp + i * DV));
+  // the path as bits: parents come before their children, so its order is theirs
+  unsigned long long path = 0;
+  for (int at = last; at >= 0; at = spar[at]) path |= 1ull << at;
 
-  if (tid == 0) {
-    int m = 0;
-    for (int at = last; at >= 0; at = spar[at]) ++m;
-    sdepth = m;
-    for (int at = last; at >= 0; at = spar[at]) spath[--m] = at;
-  }
-  __syncthreads();
-  const int depth = sdepth;
-
-  for (int t0 = 0; t0 < depth; t0 += kCommitTokens) {
-    const int m = min(kCommitTokens, depth - t0);
-    for (int i = warp; i < m; i += NW) {      // a warp per token
-      const int64_t row = start + spath[t0 + i];
-      float x[DK / 32], ss = 0.f;
+  const auto token = [&](int node, int row) {
+    float kr[RPL];
 #pragma unroll
-      for (int e = 0; e < DK / 32; ++e) {
-        x[e] = bf2f(k[row * ks + (int64_t)hk * DK + lane + 32 * e]);
-        ss = fmaf(x[e], x[e], ss);
-      }
-      const float nk = rsqrtf(warp_sum(ss) + 1e-6f);
+    for (int r = 0; r < RPL; r += 8)
+      unpack8(*reinterpret_cast<const uint4*>(&sk[row][rl * RPL + r]), kr + r);
+    float ss = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < DK / 32; ++e) {
-        const int r = lane + 32 * e;
-        sk[i][(r / RPL) * KP + r % RPL] = x[e] * nk;
-      }
-#pragma unroll
-      for (int e = 0; e < DV / 32; ++e)
-        sv[i][lane + 32 * e] = bf2f(v[row * vs + (int64_t)h * DV + lane + 32 * e]);
-      if (lane == 0) {
-        seg[i] = expf(g[row * HV + h]);
-        sbeta[i] = bf2f(beta[row * HV + h]);
-      }
+    for (int r = 0; r < RPL; ++r) {
+      ss = fmaf(kr[r], kr[r], ss);
+      a.x = fmaf(s[r].x, kr[r], a.x);
+      a.y = fmaf(s[r].y, kr[r], a.y);
+      a.z = fmaf(s[r].z, kr[r], a.z);
+      a.w = fmaf(s[r].w, kr[r], a.w);
     }
-    __syncthreads();
-    for (int i = 0; i < m; ++i) {
-      const float* kr = &sk[i][rl * KP];
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int r = 0; r < RPL; r += 4) {
-        const float4 kk = *reinterpret_cast<const float4*>(kr + r);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float ke = e == 0 ? kk.x : e == 1 ? kk.y : e == 2 ? kk.z : kk.w;
-          a.x = fmaf(s[r + e].x, ke, a.x);
-          a.y = fmaf(s[r + e].y, ke, a.y);
-          a.z = fmaf(s[r + e].z, ke, a.z);
-          a.w = fmaf(s[r + e].w, ke, a.w);
-        }
-      }
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        a.x += __shfl_xor_sync(0xffffffffu, a.x, o);
-        a.y += __shfl_xor_sync(0xffffffffu, a.y, o);
-        a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
-        a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
-      }
-      const float eg = seg[i], bt = sbeta[i];
-      const float4 vv = *reinterpret_cast<const float4*>(&sv[i][c]);
-      const float4 d = make_float4(bt * (vv.x - eg * a.x), bt * (vv.y - eg * a.y),
-                                   bt * (vv.z - eg * a.z), bt * (vv.w - eg * a.w));
-#pragma unroll
-      for (int r = 0; r < RPL; r += 4) {
-        const float4 kk = *reinterpret_cast<const float4*>(kr + r);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float ke = e == 0 ? kk.x : e == 1 ? kk.y : e == 2 ? kk.z : kk.w;
-          s[r + e].x = fmaf(ke, d.x, s[r + e].x * eg);
-          s[r + e].y = fmaf(ke, d.y, s[r + e].y * eg);
-          s[r + e].z = fmaf(ke, d.z, s[r + e].z * eg);
-          s[r + e].w = fmaf(ke, d.w, s[r + e].w * eg);
-        }
-      }
+    for (int o = 4; o < 32; o <<= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      a.x += __shfl_xor_sync(0xffffffffu, a.x, o);
+      a.y += __shfl_xor_sync(0xffffffffu, a.y, o);
+      a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
+      a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
     }
-    if (t0 + kCommitTokens < depth) __syncthreads();   // the staging buffers are free
+    const float nk = rsqrtf(ss + 1e-6f);
+    const float eg = expf(sg[node]), bt = sbeta[node] * nk, en = eg * nk;
+    const uint2 vu = *reinterpret_cast<const uint2*>(&sv[row][c]);
+    const float4 d = make_float4(bt * (__uint_as_float(vu.x << 16) - en * a.x),
+                                 bt * (__uint_as_float(vu.x & 0xffff0000u) - en * a.y),
+                                 bt * (__uint_as_float(vu.y << 16) - en * a.z),
+                                 bt * (__uint_as_float(vu.y & 0xffff0000u) - en * a.w));
+#pragma unroll
+    for (int r = 0; r < RPL; ++r) {
+      s[r].x = fmaf(kr[r], d.x, s[r].x * eg);
+      s[r].y = fmaf(kr[r], d.y, s[r].y * eg);
+      s[r].z = fmaf(kr[r], d.z, s[r].z * eg);
+      s[r].w = fmaf(kr[r], d.w, s[r].w * eg);
+    }
+  };
+  if (n <= kStaged) {
+    for (; path; path &= path - 1) {
+      const int node = __ffsll(path) - 1;
+      token(node, node);
+    }
+  } else {
+    while (path) {
+      const int m = min(kStaged, __popcll(path));
+      stage(m, [&](int r) {
+        unsigned long long p = path;
+        for (int i = 0; i < r; ++i) p &= p - 1;
+        return __ffsll(p) - 1;
+      });
+      tc::cp_async_commit();
+      tc::cp_async_wait<0>();
+      __syncthreads();
+      for (int r = 0; r < m; ++r, path &= path - 1) token(__ffsll(path) - 1, r);
+      __syncthreads();                               // the staging buffers are free
+    }
   }
 #pragma unroll
   for (int i = 0; i < RPL; ++i) __stcs(reinterpret_cast<float4*>(sp + i * DV), s[i]);
@@ -217,9 +288,12 @@ extern "C" int gdn_commit_tree(const void* x, int64_t x_row_stride, const void* 
                   accepted,
               "%s: null pointer", fn);
   GDN_REQUIRE(aligned16(s_pool), "%s: s_pool must be 16-byte aligned", fn);
-  const int nt = head_v_dim * 2;
+  const bool cvec = channels % 8 == 0 && x_row_stride % 8 == 0 && conv_slot_stride % 8 == 0 &&
+                    aligned16(x) && aligned16(conv_pool);
+  const bool vec = k_row_stride % 8 == 0 && v_row_stride % 8 == 0 && aligned16(k) && aligned16(v);
+  const int per_cta = head_v_dim * 2 * (cvec ? 8 : 1);
   const CommitConv conv{(const bf16*)x, x_row_stride, (bf16*)conv_pool, conv_slot_stride, channels,
-                        kernel, (channels + nt - 1) / nt};
+                        kernel, (channels + per_cta - 1) / per_cta, cvec};
   const int64_t ctas = (int64_t)n_seqs * (num_v_heads + conv.ctas);
   GDN_UNSUPPORTED(ctas < (1ll << 31), "%s: too many (sequence, head) units", fn);
   cudaStream_t s = (cudaStream_t)stream;
@@ -227,7 +301,7 @@ extern "C" int gdn_commit_tree(const void* x, int64_t x_row_stride, const void* 
   commit_tree_kernel<D, D><<<(unsigned)ctas, 2 * D, 0, s>>>(                                     \
       (const bf16*)k, k_row_stride, (const bf16*)v, v_row_stride, g, (const bf16*)beta, s_pool,  \
       slot_stride, num_slots, ids, cu_seqlens, parents, accepted, max_nodes, n_tokens, n_seqs,   \
-      num_k_heads, num_v_heads, conv, status)
+      num_k_heads, num_v_heads, vec, conv, status)
   if (head_v_dim == 128) GDN_CM(128);
   else GDN_CM(64);
 #undef GDN_CM
