@@ -321,39 +321,39 @@ __global__ void __launch_bounds__(kConvThreads) conv_state_writeback_kernel(
 // ---------------------------------------------------------------------------
 //
 // y[n] = silu(sum_{i<K} w[K-1-i] * x[i-th ancestor of n]); above the root the
-// stored taps, newest first.  A CTA owns rows_per_cta rows x 1024 channels (or
+// stored taps, newest first.  A CTA owns rows_per_cta rows x 512 channels (or
 // 128 unaligned ones); its first warp walks every row's K-1 ancestors once and
-// leaves, per row and tap, the row to read or the stored tap.  Values come from
-// conv_point(), so a chain's rows have the bits of the varlen conv.
+// leaves, per row and tap, the row to read.  Values come from conv_point(), so a
+// chain's rows have the bits of the varlen conv.
+//
+// 2 + 2 bytes per element of HBM; the ancestors' rows come from L1 / L2, a row ahead,
+// and without a branch: above the root a row stands in for the stored tap, which the
+// few rows concerned then fetch.  Bound by its instructions (some 20 per output: four
+// rows unpacked, addresses, SiLU): 5.2k rows of 8192 channels take 68 us, floor 27,
+// first form 84.
 constexpr int kTreeConvRows = 16;
 
-template <int K, bool VEC>
-__global__ void __launch_bounds__(kConvThreads) conv_tree_kernel(
+template <int K, int V>   // channels per thread: 4 (8-byte accesses) or 1
+__global__ void __launch_bounds__(kConvThreads, 9) conv_tree_kernel(
     const bf16* __restrict__ x, int64_t xs, const bf16* __restrict__ pool, int64_t slot_stride,
     int64_t num_slots, const int64_t* __restrict__ ids, const int32_t* __restrict__ cu,
     int n_seqs, const int32_t* __restrict__ parents, int max_nodes, int64_t n_tokens, int C,
     const bf16* __restrict__ w, bf16* __restrict__ y, int64_t ys, int rows_per_cta,
     int32_t* status, const GateArgs gate) {
   constexpr int T = K - 1;
-  constexpr int V = VEC ? 8 : 1;
   const int64_t t0 = (int64_t)blockIdx.x * rows_per_cta;
   const int rows = (int)min((int64_t)rows_per_cta, n_tokens - t0);
-  // per row: its slot (-1: leave the row), and per tap i the flat row of the
-  // i-th ancestor, or -1 - j for the stored tap j
+  // per row: its slot (-1: leave the row), how many of its K taps are rows, and
+  // those rows' offsets in x (its own where the root is passed)
   __shared__ int64_t s_slot[kTreeConvRows];
   __shared__ int64_t s_src[kTreeConvRows][K];
+  __shared__ int s_found[kTreeConvRows];
   const int c0 = (blockIdx.y * kConvThreads + threadIdx.x) * V;
   const bool gate_cta = blockIdx.y == gridDim.y - 1;
   float wv[V * K];
   if (!gate_cta && c0 < C) {
-    if constexpr (VEC) {
-      const uint4* wp = reinterpret_cast<const uint4*>(w + (int64_t)c0 * K);
 #pragma unroll
-      for (int j = 0; j < K; ++j) unpack8(wp[j], wv + 8 * j);
-    } else {
-#pragma unroll
-      for (int i = 0; i < K; ++i) wv[i] = bf2f(w[(int64_t)c0 * K + i]);
-    }
+    for (int i = 0; i < V * K; ++i) wv[i] = bf2f(w[(int64_t)c0 * K + i]);
   }
   if (threadIdx.x < 32) {
     int r = warp_seq_of(cu, n_seqs, t0);
@@ -367,13 +367,14 @@ __global__ void __launch_bounds__(kConvThreads) conv_tree_kernel(
           t < start + n) {
         slot = ids[r];
         if (!slot_ok(slot, num_slots, status)) slot = -1;
-        int at = (int)(t - start), above = 0;
+        int at = (int)(t - start), found = 0;
 #pragma unroll
         for (int i = 0; i < K; ++i) {
-          s_src[lane][i] = at >= 0 ? start + at : (int64_t)(-1 - (T - 1 - above));
-          if (at < 0) ++above;
-          else at = i + 1 < K ? tree_parent(parents[start + at], at, status) : -1;
+          s_src[lane][i] = (at >= 0 ? start + at : t) * xs;
+          found += at >= 0;
+          if (at >= 0) at = i + 1 < K ? tree_parent(parents[start + at], at, status) : -1;
         }
+        s_found[lane] = found;
       }
       s_slot[lane] = slot;
     }
@@ -399,33 +400,67 @@ __global__ void __launch_bounds__(kConvThreads) conv_tree_kernel(
     return;
   }
   if (c0 >= C) return;
-  for (int rr = 0; rr < rows; ++rr) {
-    const int64_t slot = s_slot[rr];
-    if (slot < 0) continue;
-    const bf16* taps = pool + slot * slot_stride + (int64_t)c0 * T;
-    float win[K][V];
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-      const int64_t src = s_src[rr][i];
-      if (src >= 0) {
-        if constexpr (VEC) unpack8(*reinterpret_cast<const uint4*>(x + src * xs + c0), win[T - i]);
-        else win[T - i][0] = bf2f(x[src * xs + c0]);
-      } else {
-        const int j = (int)(-1 - src);
-#pragma unroll
-        for (int ch = 0; ch < V; ++ch) win[T - i][ch] = bf2f(taps[ch * T + j]);
-      }
-    }
-    float out[V];
-#pragma unroll
-    for (int ch = 0; ch < V; ++ch) {
+  if constexpr (V == 1) {
+    for (int rr = 0; rr < rows; ++rr) {
+      if (s_slot[rr] < 0) continue;
+      const bf16* taps = pool + s_slot[rr] * slot_stride + (int64_t)c0 * T;
       float wn[K];
 #pragma unroll
-      for (int i = 0; i < K; ++i) wn[i] = win[i][ch];
-      out[ch] = conv_point<K>(wn, wv + ch * K);
+      for (int i = 0; i < K; ++i)
+        wn[T - i] = bf2f(i < s_found[rr] ? x[s_src[rr][i] + c0] : taps[T - 1 - (i - s_found[rr])]);
+      y[(t0 + rr) * ys + c0] = f2bf(conv_point<K>(wn, wv));
     }
-    if constexpr (VEC) *reinterpret_cast<uint4*>(y + (t0 + rr) * ys + c0) = pack8(out);
-    else y[(t0 + rr) * ys + c0] = f2bf(out[0]);
+  } else {
+    const bf16* xc = x + c0;
+    const auto load = [&](int rr, uint2(&raw)[K]) {
+      if (rr < rows && s_slot[rr] >= 0) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) raw[i] = *reinterpret_cast<const uint2*>(xc + s_src[rr][i]);
+      }
+    };
+    uint2 cur[K], nxt[K];
+    load(0, cur);
+    bf16* yp = y + t0 * ys + c0;
+    for (int rr = 0; rr < rows; ++rr, yp += ys) {
+      load(rr + 1, nxt);
+      if (s_slot[rr] >= 0) {
+        const int found = s_found[rr];
+        uint2 out;
+        if (found == K) {
+          // channels in pairs: fma.f32x2 rounds each as conv_point()'s fmaf
+          uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            float a0, a1;
+#pragma unroll
+            for (int i = K - 1; i >= 0; --i) {         // the oldest first
+              const uint32_t u = p == 0 ? cur[i].x : cur[i].y;
+              const float x0 = __uint_as_float(u << 16), x1 = __uint_as_float(u & 0xffff0000u);
+              const float w0 = wv[2 * p * K + T - i], w1 = wv[(2 * p + 1) * K + T - i];
+              if (i == K - 1) tc::fmul2(a0, a1, x0, x1, w0, w1);
+              else tc::ffma2(a0, a1, x0, x1, w0, w1, a0, a1);
+            }
+            const __nv_bfloat162 b2 = __floats2bfloat162_rn(conv_silu(a0), conv_silu(a1));
+            o[p] = *reinterpret_cast<const uint32_t*>(&b2);
+          }
+        } else {                                       // near the root: stored taps
+          const bf16* taps = pool + s_slot[rr] * slot_stride + (int64_t)c0 * T;
+          bf16* o = reinterpret_cast<bf16*>(&out);
+#pragma unroll
+          for (int ch = 0; ch < V; ++ch) {
+            float wn[K];
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+              wn[T - i] = bf2f(i < found ? reinterpret_cast<const bf16*>(&cur[i])[ch]
+                                         : taps[ch * T + T - 1 - (i - found)]);
+            o[ch] = f2bf(conv_point<K>(wn, wv + ch * K));
+          }
+        }
+        *reinterpret_cast<uint2*>(yp) = out;
+      }
+#pragma unroll
+      for (int i = 0; i < K; ++i) cur[i] = nxt[i];
+    }
   }
 }
 
@@ -587,20 +622,27 @@ extern "C" int gdn_conv_gate_tree(const void* x, int64_t x_row_stride, const voi
   GDN_REQUIRE(x && conv_pool && ids && cu_seqlens && parents && weight && y && b && a && a_log &&
                   dt_bias && g && beta,
               "%s: null pointer", fn);
-  const bool vec = channels % 8 == 0 && x_row_stride % 8 == 0 && y_row_stride % 8 == 0 &&
-                   aligned16(x) && aligned16(y) && aligned16(weight);
-  const int per_cta = vec ? kConvThreads * 8 : kConvThreads;
+  const bool vec = channels % 4 == 0 && x_row_stride % 4 == 0 && y_row_stride % 4 == 0 &&
+                   ((uintptr_t)x | (uintptr_t)y) % 8 == 0;
+  const int per_cta = vec ? kConvThreads * 4 : kConvThreads;
   const unsigned cy = (unsigned)((channels + per_cta - 1) / per_cta) + 1;   // + the gate's row
-  const int rows = kTreeConvRows;
+  // few rows are spread thin, so that a small call is not one CTA's loop
+  const int64_t thin = n_tokens * cy / (4 * sm_count());
+  const int rows = thin >= kTreeConvRows ? kTreeConvRows : thin < 2 ? 2 : (int)thin;
   const int64_t tiles = (n_tokens + rows - 1) / rows;
   GDN_UNSUPPORTED(tiles < (1ll << 31) && cy <= 65535, "%s: too many tokens or channels", fn);
   const GateArgs gate{(const bf16*)b, (const bf16*)a, ab_row_stride, num_v_heads, a_log, dt_bias,
                       param_dtype == GDN_DTYPE_BF16, g, (bf16*)beta};
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid((unsigned)tiles, cy);
-#define GDN_CT(KK, VV)                                                                            if (kernel == KK && vec == VV)                                                                    conv_tree_kernel<KK, VV><<<grid, kConvThreads, 0, s>>>(                                             (const bf16*)x, x_row_stride, (const bf16*)conv_pool, slot_stride, num_slots, ids,              cu_seqlens, n_seqs, parents, max_nodes, n_tokens, channels, (const bf16*)weight,                (bf16*)y, y_row_stride, rows, status, gate);
-  GDN_CT(2, true) GDN_CT(3, true) GDN_CT(4, true)
-  GDN_CT(2, false) GDN_CT(3, false) GDN_CT(4, false)
+#define GDN_CT(KK, VV)                                                                        \
+  if (kernel == KK && vec == (VV > 1))                                                        \
+    conv_tree_kernel<KK, VV><<<grid, kConvThreads, 0, s>>>(                                   \
+        (const bf16*)x, x_row_stride, (const bf16*)conv_pool, slot_stride, num_slots, ids,    \
+        cu_seqlens, n_seqs, parents, max_nodes, n_tokens, channels, (const bf16*)weight,      \
+        (bf16*)y, y_row_stride, rows, status, gate);
+  GDN_CT(2, 4) GDN_CT(3, 4) GDN_CT(4, 4)
+  GDN_CT(2, 1) GDN_CT(3, 1) GDN_CT(4, 1)
 #undef GDN_CT
   return check_launch(fn);
 }

@@ -9,99 +9,131 @@
 //
 // HBM-bound: every element is read once and written once (4 bytes), the table of
 // cosines and sines is R * 4 bytes per row, shared by the row's heads in L1 / L2.
-// D / 8 lanes own one head of one row, 16 bytes each; the norm is a shuffle sum
-// and the rotation's partner half comes from the lane R / 16 away, so nothing
-// goes through shared memory.  All arithmetic is fp32, rounded once at the end.
+// D / 8 lanes own NH heads of one row, eight elements of each per lane: their loads are
+// in flight together and they share the position, the slot and the table's row.  A lane's
+// elements are four of the first half of the rotation and their four partners of
+// the second, or eight behind it, so the rotation needs no exchange (with 16-byte
+// pieces and shuffles for the partners 27 us where this takes 24).  The norm is a
+// shuffle sum.  All arithmetic is fp32, rounded once at the end.
+//
+// NH: 6 where that many rows fill the GPU anyway (8.3k rows of 16 + 4 + 4 heads x 128:
+// 1 head 35 us, 2 28, 4 26, 6 24, 8 27; floor 16), else 2, which spread a small call
+// over more SMs (128 rows: 2.6 us where 6 take 4.2).
+#include "mma_util.cuh"
 #include "tree.cuh"
 
 namespace gdn {
 
 constexpr int kRopeThreads = 256;
 
-template <int D>
-__global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(
+template <int D, int NH>
+__global__ void __launch_bounds__(kRopeThreads, 4) qk_rope_kernel(
     const bf16* __restrict__ q, int64_t qs, const bf16* __restrict__ k, int64_t ks,
     const bf16* __restrict__ v, int64_t vs, const bf16* __restrict__ qw,
     const bf16* __restrict__ kw, float eps, float offset, const float* __restrict__ cos_sin,
     int64_t max_pos, int rot, const int64_t* __restrict__ positions, bf16* __restrict__ k_cache,
     bf16* __restrict__ v_cache, int64_t block_stride, int64_t token_stride, int64_t head_stride,
     int64_t num_blocks, int block_size, const int32_t* __restrict__ slots, bf16* __restrict__ out,
-    int64_t n_tokens, int HQ, int HKV, int32_t* status) {
+    int64_t n_tokens, int HQ, int HKV, int groups, int32_t* status) {
   constexpr int LPR = D / 8;                  // lanes per head
   const int heads = HQ + 2 * HKV;
-  const int64_t item = ((int64_t)blockIdx.x * kRopeThreads + threadIdx.x) / LPR;
-  const bool live = item < n_tokens * heads;
-  const int64_t t = live ? item / heads : 0;
-  const int h = live ? (int)(item - t * heads) : 0;
-  const int sub = threadIdx.x % LPR;
-  const int d0 = sub * 8;
+  const int64_t item = (int64_t)blockIdx.x * (kRopeThreads / LPR) + threadIdx.x / LPR;
+  const bool live = item < n_tokens * groups;
+  const int64_t t = live ? (item >> 31 ? item / groups : (int64_t)((unsigned)item / (unsigned)groups)) : 0;
+  const int h0 = live ? (int)(item - t * groups) * NH : heads;
+  // this lane's elements: da .. da + 3 and db .. db + 3
+  const int sub = threadIdx.x % LPR, half = rot / 2;
+  const bool turn = sub < rot / 8;
+  const int da = turn ? sub * 4 : sub * 8, db = turn ? half + sub * 4 : sub * 8 + 4;
 
-  const bool is_q = h < HQ, is_v = h >= HQ + HKV;
-  const int kvh = is_q ? 0 : is_v ? h - HQ - HKV : h - HQ;
-  const bf16* src = is_q ? q + t * qs + (int64_t)h * D
-                         : is_v ? v + t * vs + (int64_t)kvh * D : k + t * ks + (int64_t)kvh * D;
-  const uint4 raw = live ? *reinterpret_cast<const uint4*>(src + d0) : make_uint4(0, 0, 0, 0);
-  int64_t pos = 0;
-  bool ok = live;
-  if (live && !is_v) {
-    pos = positions[t];
-    if (pos < 0 || pos >= max_pos) {
-      if (status && sub == 0) atomicOr(status, GDN_STATUS_BAD_POSITION);
-      ok = false;
-      pos = 0;
+  uint2 ra[NH], rb[NH];
+#pragma unroll
+  for (int u = 0; u < NH; ++u) {
+    const int h = h0 + u;
+    ra[u] = rb[u] = make_uint2(0, 0);
+    if (h < heads) {
+      const bf16* src = h < HQ ? q + t * qs + (int64_t)h * D
+                               : h < HQ + HKV ? k + t * ks + (int64_t)(h - HQ) * D
+                                              : v + t * vs + (int64_t)(h - HQ - HKV) * D;
+      ra[u] = *reinterpret_cast<const uint2*>(src + da);
+      rb[u] = *reinterpret_cast<const uint2*>(src + db);
     }
   }
-  bf16* dst = nullptr;
-  if (live && is_q) {
-    dst = out + (t * HQ + h) * D;
-  } else if (live) {
-    const int64_t slot = slots[t];
-    if (slot >= 0 && slot < num_blocks * block_size) {
-      const int64_t page = slot / block_size;
-      dst = (is_v ? v_cache : k_cache) + page * block_stride +
-            (slot - page * block_size) * token_stride + (int64_t)kvh * head_stride;
-    } else if (slot != -1) {
-      if (status && sub == 0) atomicOr(status, GDN_STATUS_BAD_SLOT);
+  int64_t pos = live ? positions[t] : 0;
+  const int slot = live ? slots[t] : -1;
+  const bool placed = pos >= 0 && pos < max_pos;
+  if (!placed) {
+    if (status && sub == 0 && h0 < HQ + HKV) atomicOr(status, GDN_STATUS_BAD_POSITION);
+    pos = 0;
+  }
+  int64_t cache = -1;                         // the slot's place in the caches
+  if (slot >= 0 && slot < num_blocks * block_size) {
+    const int page = slot / block_size;
+    cache = page * block_stride + (int64_t)(slot - page * block_size) * token_stride;
+  } else if (slot != -1 && status && sub == 0 && h0 + NH > HQ) {
+    atomicOr(status, GDN_STATUS_BAD_SLOT);
+  }
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (turn && h0 < HQ + HKV) {
+    c = *reinterpret_cast<const float4*>(cos_sin + pos * rot + da);
+    s = *reinterpret_cast<const float4*>(cos_sin + pos * rot + db);
+  }
+  const auto unpack4 = [](const uint2& u, float(&f)[4]) {
+    f[0] = __uint_as_float(u.x << 16);
+    f[1] = __uint_as_float(u.x & 0xffff0000u);
+    f[2] = __uint_as_float(u.y << 16);
+    f[3] = __uint_as_float(u.y & 0xffff0000u);
+  };
+  float wa[4], wb[4];                         // weights of the heads' kind
+  const auto weights = [&](const bf16* w) {
+    unpack4(*reinterpret_cast<const uint2*>(w + da), wa);
+    unpack4(*reinterpret_cast<const uint2*>(w + db), wb);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      wa[e] += offset;
+      wb[e] += offset;
+    }
+  };
+  weights(h0 < HQ ? qw : kw);
+#pragma unroll
+  for (int u = 0; u < NH; ++u) {
+    const int h = h0 + u;
+    if (h == HQ && u > 0) weights(kw);
+    float a[4], b[4];
+    unpack4(ra[u], a);
+    unpack4(rb[u], b);
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(ss * (1.f / D) + eps);
+    bf16* dst = nullptr;
+    if (h < HQ) {
+      if (placed) dst = out + (t * HQ + h) * D;
+    } else if (h < heads && cache >= 0) {
+      if (h >= HQ + HKV) {
+        dst = v_cache + cache + (h - HQ - HKV) * head_stride;
+        *reinterpret_cast<uint2*>(dst + da) = ra[u];
+        *reinterpret_cast<uint2*>(dst + db) = rb[u];
+        dst = nullptr;
+      } else if (placed) {
+        dst = k_cache + cache + (h - HQ) * head_stride;
+      }
+    }
+    if (dst != nullptr) {
+      const float cc[4] = {c.x, c.y, c.z, c.w}, sc[4] = {s.x, s.y, s.z, s.w};
+      float y[4], z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x0 = a[e] * inv * wa[e], x1 = b[e] * inv * wb[e];
+        y[e] = x0 * cc[e] - x1 * sc[e];
+        z[e] = x1 * cc[e] + x0 * sc[e];
+      }
+      *reinterpret_cast<uint2*>(dst + da) = make_uint2(mm::pack2(y[0], y[1]), mm::pack2(y[2], y[3]));
+      *reinterpret_cast<uint2*>(dst + db) = make_uint2(mm::pack2(z[0], z[1]), mm::pack2(z[2], z[3]));
     }
   }
-  float x[8];
-  unpack8(raw, x);
-  float ss = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float inv = rsqrtf(ss * (1.f / D) + eps);
-  float wv[8];
-  unpack8(*reinterpret_cast<const uint4*>((is_q ? qw : kw) + d0), wv);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (wv[e] + offset);
-
-  // the rotation's other half: the lane rot / 16 away, within this head's lanes
-  const int half = rot / 2, far = rot / 16;
-  const bool lo = d0 < half, turn = d0 < rot;
-  const int lane = threadIdx.x & 31;
-  const int from = turn ? (lo ? lane + far : lane - far) : lane;
-  float other[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) other[e] = __shfl_sync(0xffffffffu, x[e], from);
-  if (dst == nullptr || !ok) return;
-  if (is_v) {
-    *reinterpret_cast<uint4*>(dst + d0) = raw;
-    return;
-  }
-  if (turn) {
-    const float* cs = cos_sin + pos * rot + (lo ? d0 : d0 - half);
-    float c[8], s[8];
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(cs + e);
-      *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(cs + half + e);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] * c[e] + (lo ? -other[e] : other[e]) * s[e];
-  }
-  *reinterpret_cast<uint4*>(dst + d0) = pack8(x);
 }
 
 }  // namespace gdn
@@ -144,21 +176,29 @@ extern "C" int gdn_qk_norm_rope_cache(
                       aligned16(k_weight) && aligned16(cos_sin) && aligned16(q_out) &&
                       aligned16(k_cache) && aligned16(v_cache),
                   "%s: operands and strides must be 16-byte aligned", fn);
-  const int64_t items = n_tokens * (num_q_heads + 2ll * num_kv_heads);
+  const int heads = num_q_heads + 2 * num_kv_heads;
+  // one full wave of threads with two heads each: enough rows for six
+  const bool many = n_tokens * heads * (head_dim / 8) / 2 >= (int64_t)sm_count() * 2048;
+  const int nh = many ? 6 : 2, groups = (heads + nh - 1) / nh;
+  const int64_t items = n_tokens * groups;
   const int64_t per_cta = kRopeThreads / (head_dim / 8);
   const int64_t ctas = (items + per_cta - 1) / per_cta;
   GDN_UNSUPPORTED(ctas < (1ll << 31), "%s: too many rows", fn);
   cudaStream_t s = (cudaStream_t)stream;
-#define GDN_ROPE(DD)                                                                             \
-  case DD:                                                                                       \
-    qk_rope_kernel<DD><<<(unsigned)ctas, kRopeThreads, 0, s>>>(                                  \
-        (const bf16*)q, q_row_stride, (const bf16*)k, k_row_stride, (const bf16*)v,              \
-        v_row_stride, (const bf16*)q_weight, (const bf16*)k_weight, eps, unit_offset ? 1.f : 0.f, \
-        cos_sin, max_position, rotary_dim, positions, (bf16*)k_cache, (bf16*)v_cache,            \
-        block_stride, token_stride, head_stride, num_blocks, block_size, slot_mapping,           \
-        (bf16*)q_out, n_tokens, num_q_heads, num_kv_heads, status);                              \
-    break;
-  switch (head_dim) { GDN_ROPE(64) GDN_ROPE(128) GDN_ROPE(256) }
+#define GDN_ROPE(DD, NH)                                                                          \
+  qk_rope_kernel<DD, NH><<<(unsigned)ctas, kRopeThreads, 0, s>>>(                                 \
+      (const bf16*)q, q_row_stride, (const bf16*)k, k_row_stride, (const bf16*)v, v_row_stride,   \
+      (const bf16*)q_weight, (const bf16*)k_weight, eps, unit_offset ? 1.f : 0.f, cos_sin,        \
+      max_position, rotary_dim, positions, (bf16*)k_cache, (bf16*)v_cache, block_stride,          \
+      token_stride, head_stride, num_blocks, block_size, slot_mapping, (bf16*)q_out, n_tokens,    \
+      num_q_heads, num_kv_heads, groups, status)
+#define GDN_ROPE2(DD)               \
+  if (head_dim == DD) {             \
+    if (many) GDN_ROPE(DD, 6);      \
+    else GDN_ROPE(DD, 2);           \
+  }
+  GDN_ROPE2(64) GDN_ROPE2(128) GDN_ROPE2(256)
+#undef GDN_ROPE2
 #undef GDN_ROPE
   return check_launch(fn);
 }

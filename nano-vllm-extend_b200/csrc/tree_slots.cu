@@ -32,39 +32,55 @@ __global__ void __launch_bounds__(kSlotThreads) tree_slot_kernel(
     s_par[i] = t >= 0 && t < n_rows ? parents[t] : -1;
   }
   int r = warp_seq_of(cu, n_seqs, t0 + (threadIdx.x & ~31));
-  __syncthreads();
   const int64_t t = t0 + threadIdx.x;
-  if (t >= n_rows) return;
   while (r < n_seqs && (int64_t)cu[r + 1] <= t) ++r;
-  int64_t pos = 0, slot = -1, start;
-  int n;
-  if (r < n_seqs && tree_rows(cu, r, n_rows, max_nodes, status, start, n) && t >= start &&
-      t < start + n) {
+  int64_t start = 0;
+  int n = 0, c = 0, last = -1;
+  const bool mine = t < n_rows && r < n_seqs &&
+                    tree_rows(cu, r, n_rows, max_nodes, status, start, n) && t >= start &&
+                    t < start + n;
+  if (mine) {
+    c = ctx[r];
+    if (accepted != nullptr) last = accepted[r];
+  }
+  __syncthreads();
+  if (t >= n_rows) return;
+  int64_t pos = 0, slot = -1;
+  if (mine) {
     const int i = (int)(t - start);
     const int* par = s_par + (start - (t0 - HALO));   // par[j]: node j of this sequence
-    int depth = 0;
-    for (int j = tree_parent(par[i], i, status); j >= 0; j = tree_parent(par[j], j, status)) ++depth;
-    const int64_t c = ctx[r];
-    if (c < 0) {
-      if (status) atomicOr(status, GDN_STATUS_BAD_SEQLEN);
-    } else {
-      pos = c + depth;
-      int64_t at = c + i;
-      bool kept = true;
-      if (accepted != nullptr) {
-        int j = accepted[r];
-        if (j < -1 || j >= n) {
-          if (status) atomicOr(status, GDN_STATUS_BAD_TREE);
-          j = -1;
-        }
-        while (j > i) j = tree_parent(par[j], j, status);
-        kept = j == i;
-        at = pos;
+    int depth = 0, p = par[i];
+    bool bad = c < 0, kept = true;
+    for (int j = i; p != -1; ++depth) {               // p < j: the walk ends
+      if (p < 0 || p >= j) {
+        bad = true;
+        break;
       }
+      j = p;
+      p = par[j];
+    }
+    if (accepted != nullptr) {
+      bad |= last < -1 || last >= n;
+      int j = bad ? -1 : last;
+      while (j > i) {
+        p = par[j];
+        if (p < -1 || p >= j) {
+          bad = true;
+          break;
+        }
+        j = p;
+      }
+      kept = j == i;
+    }
+    if (bad) {
+      if (status) atomicOr(status, c < 0 ? GDN_STATUS_BAD_SEQLEN : GDN_STATUS_BAD_TREE);
+    } else {
+      pos = (int64_t)c + depth;
+      const unsigned at = (unsigned)c + (accepted != nullptr ? depth : i);
       if (kept) {
-        const int64_t blk = at / block_size;
-        const int64_t page = blk < max_blocks ? tables[r * table_stride + blk] : -1;
-        slot = page * block_size + at % block_size;
+        const unsigned blk = at / (unsigned)block_size;
+        const int64_t page = blk < (unsigned)max_blocks ? tables[r * table_stride + blk] : -1;
+        slot = page * block_size + (at - blk * (unsigned)block_size);
         if (page < 0 || slot > INT32_MAX) {
           if (status) atomicOr(status, GDN_STATUS_BAD_SLOT);
           slot = -1;

@@ -492,6 +492,30 @@ def test_qk_norm_rope(ops, D, rot, offset):
     assert ops.check_status() == 0
 
 
+def test_qk_norm_rope_many_rows(ops):
+    """Enough rows for the form with more heads per thread; both kinds of heads in one group."""
+    r = np.random.default_rng(3)
+    n, HQ, HKV, D, rot = 5000, 9, 2, 64, 32
+    d = bf(rnd(r, n, HQ + 2 * HKV, D))
+    qw, kw = rnd(r, D), rnd(r, D)
+    ang = r.uniform(0, 6.3, (50, rot // 2))
+    cs = np.concatenate([np.cos(ang), np.sin(ang)], 1).astype(np.float32)
+    pos, slot = r.integers(0, 50, n), r.permutation(320 * 16)[:n]
+    slot[::7] = -1
+    kc, vc = (torch.zeros(320, 16, HKV, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    out = ops.qk_norm_rope_cache(d[:, :HQ], d[:, HQ:HQ + HKV], d[:, HQ + HKV:], bf(qw), bf(kw),
+                                 f32(cs), i64(pos), kc, vc, i32(slot))
+    c, s = cs[pos, :rot // 2].astype(np.float64), cs[pos, rot // 2:].astype(np.float64)
+    x = host(d)
+    close(out, R.norm_rope(x[:, :HQ], qw, c, s, 1e-6, 0), 2.0 ** -18, "q")
+    keep = slot >= 0
+    rk = R.norm_rope(x[:, HQ:HQ + HKV], kw, c, s, 1e-6, 0)
+    close(kc.view(-1, HKV, D)[slot[keep]], rk[keep], 2.0 ** -18, "k")
+    ref_v = torch.zeros_like(vc).view(-1, HKV, D)
+    ref_v[slot[keep]] = d[:, HQ + HKV:][torch.from_numpy(keep)]
+    assert torch.equal(vc.view(-1, HKV, D), ref_v) and ops.check_status() == 0
+
+
 def test_qk_norm_rope_unaligned_rows_and_one_row(ops):
     r = np.random.default_rng(0)
     for n in (1, 3):
