@@ -41,7 +41,9 @@ _STATUS: dict[int, torch.Tensor] = {}
 
 
 def _stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: a Stream object costs 2.5 us, as much as the launch
+    idx = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
 
 def status_word(device) -> torch.Tensor:
@@ -244,7 +246,7 @@ def _out_buffer(out, shape, device) -> torch.Tensor:
     """A bf16 output of `shape`: `out` itself when given (a contiguous tensor of
     that shape, e.g. a row slice of a larger buffer), else a new tensor."""
     if out is None:
-        return torch.empty(*shape, dtype=torch.bfloat16, device=device)
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
     assert tuple(out.shape) == tuple(shape) and out.dtype == torch.bfloat16 and \
         out.is_contiguous() and out.device == torch.device(device), \
         f"out must be a contiguous bf16 tensor of shape {tuple(shape)}"
@@ -332,9 +334,9 @@ def _slot_stride(pool: torch.Tensor) -> int:
 
 
 def _pool_view_check(pool: torch.Tensor, taps: int, channels: int):
-    assert pool.dim() == 3 and pool.shape[1] == channels and pool.shape[2] == taps, \
+    assert pool.dim() == 3 and pool.shape[1:] == (channels, taps), \
         f"conv pool view must be [slots, {channels}, {taps}]"
-    assert pool.stride(2) == 1 and pool.stride(1) == taps, "conv pool taps must be dense"
+    assert pool.stride()[1:] == (taps, 1), "conv pool taps must be dense"
     assert pool.dtype == torch.bfloat16
 
 
@@ -452,10 +454,10 @@ def _heads(t: torch.Tensor, name: str):
 
 
 def _state_view_check(s_pool: torch.Tensor, HV: int, DK: int, DV: int):
-    assert s_pool.dim() == 4 and tuple(s_pool.shape[1:]) == (HV, DK, DV), \
+    assert s_pool.dim() == 4 and s_pool.shape[1:] == (HV, DK, DV), \
         f"state pool view must be [slots, {HV}, {DK}, {DV}]"
     assert s_pool.dtype == torch.float32
-    assert s_pool.stride(1) == DK * DV and s_pool.stride(2) == DV and s_pool.stride(3) == 1
+    assert s_pool.stride()[1:] == (DK * DV, DV, 1)
 
 
 def _norm_args(z, norm_weight, rows, HV, DV):
@@ -715,21 +717,23 @@ def decode_fused(mixed: torch.Tensor, z: torch.Tensor, b: torch.Tensor, a: torch
 def _launch(name: str, device: torch.device, *args) -> None:
     """Call entry point ``name`` with its device's status word and current stream,
     on that device."""
-    lib = _lib.load()
+    fn = getattr(_lib.load(), name)
     if device.index == torch.cuda.current_device():
-        rc = getattr(lib, name)(*args, _p(status_word(device)), _stream_ptr(device))
+        rc = fn(*args, status_word(device).data_ptr(), _stream_ptr(device))
     else:
         with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args, _p(status_word(device)), _stream_ptr(device))
-    _lib.check(rc, name)
+            rc = fn(*args, status_word(device).data_ptr(), _stream_ptr(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _one_device(*ts) -> torch.device:
-    dev = ts[0].device
+    idx = ts[0].get_device()
     for t in ts:
-        assert t is None or (t.is_cuda and t.device == dev), \
-            "GDN operators take CUDA tensors of one device"
-    return dev
+        if t is not None and t.get_device() != idx:
+            idx = -1
+    assert idx >= 0, "GDN operators take CUDA tensors of one device"
+    return ts[0].device
 
 
 def _int32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
@@ -740,15 +744,30 @@ def _int32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     return t
 
 
+def _bf16_heads(t: torch.Tensor, name: str):
+    """[rows, H, D] bf16 view with dense heads -> (rows, H, D, row stride); the stride of a
+    single row means nothing and may be anything, so it becomes the row's width."""
+    assert t.dim() == 3 and t.dtype == torch.bfloat16, f"{name}: expected bf16 [rows, H, D]"
+    rows, H, D = t.shape
+    s = t.stride()
+    assert s[2] == 1 and (H == 1 or s[1] == D), f"{name}: heads must be dense within a row"
+    return rows, H, D, (s[0] if rows > 1 else H * D)
+
+
+def _bf16_rows(t: torch.Tensor, width: int, name: str) -> tuple[torch.Tensor, int, int]:
+    """(t as [rows, width], rows, row stride), the last dimension dense."""
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    assert t.dtype == torch.bfloat16, f"{name}: expected bf16"
+    rows = t.shape[0]
+    s = t.stride()
+    assert s[1] == 1 or width == 1, f"{name}: last dimension must be dense"
+    return t, rows, (s[0] if rows > 1 else width)
+
+
 def _tree(cu_seqlens, parents, max_nodes, n_seqs: int, n_rows: int):
     return (_int32(cu_seqlens, n_seqs + 1, "cu_seqlens"), _int32(parents, n_rows, "parents"),
             int(max_nodes))
-
-
-def _stride(row_stride: int, rows: int, width: int) -> int:
-    """The row stride to pass on; that of a single row means nothing and may be
-    anything, so it becomes the row's width."""
-    return row_stride if rows > 1 else width
 
 
 def _aligned_rows(t: torch.Tensor, row_stride: int, elements: int) -> bool:
@@ -765,54 +784,55 @@ def conv_gate_tree(x: torch.Tensor, state_pool: torch.Tensor, ids: torch.Tensor,
     of conv_gate_varlen.  Returns (y [N, C], g fp32 [N, Vh], beta bf16 [N, Vh])."""
     dev = _one_device(x, state_pool, ids, weight, cu_seqlens, parents, b, a, a_log, dt_bias)
     C = x.shape[-1]
-    w = weight.reshape(C, -1).contiguous()
-    K = w.shape[1]
+    x, N, xs = _bf16_rows(x, C, "x")
+    if weight.dim() != 2 or not weight.is_contiguous():
+        weight = weight.reshape(C, -1).contiguous()
+    K = weight.shape[1]
+    assert weight.dtype == torch.bfloat16 and weight.shape[0] == C
     _pool_view_check(state_pool, K - 1, C)
-    assert x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16
-    x2, xs = _rows2d(x, C)
-    N = x2.shape[0]
-    xs = _stride(xs, N, C)
     ids = _ids64(ids)
-    tree = _tree(cu_seqlens, parents, max_nodes, ids.numel(), N)
-    assert b.dtype == torch.bfloat16 and a.dtype == torch.bfloat16 and a.shape == b.shape
+    n_seqs = ids.numel()
+    tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, N)
     vh = a.shape[-1]
-    assert a.numel() == N * vh, "b / a need one row per token"
+    assert a.numel() == N * vh and b.shape == a.shape, "b / a need one row per token"
+    a, _, a_s = _bf16_rows(a, vh, "a")
+    b, _, b_s = _bf16_rows(b, vh, "b")
+    if a_s != b_s:
+        a, b, a_s = a.contiguous(), b.contiguous(), vh
     assert a_log.numel() == vh and dt_bias.numel() == vh and a_log.dtype == dt_bias.dtype
-    if a.dim() != 2 or b.dim() != 2 or a.stride(0) != b.stride(0) or a.stride(1) != 1 \
-            or b.stride(1) != 1:
-        a = a.reshape(-1, vh).contiguous()
-        b = b.reshape(-1, vh).contiguous()
-    if a_log.dtype == torch.bfloat16:
-        pdt, a_log, dt_bias = _lib.GDN_DTYPE_BF16, a_log.contiguous(), dt_bias.contiguous()
-    else:
-        pdt, a_log, dt_bias = (_lib.GDN_DTYPE_F32, a_log.float().contiguous(),
-                               dt_bias.float().contiguous())
-    _debug_checks(ids, state_pool.shape[0])
-    _debug_tree(tree, N)
-    y = torch.empty(N, C, dtype=x.dtype, device=dev)
+    pdt = _lib.GDN_DTYPE_BF16 if a_log.dtype == torch.bfloat16 else _lib.GDN_DTYPE_F32
+    if pdt == _lib.GDN_DTYPE_F32 and a_log.dtype != torch.float32:
+        a_log, dt_bias = a_log.float(), dt_bias.float()
+    if not (a_log.is_contiguous() and dt_bias.is_contiguous()):
+        a_log, dt_bias = a_log.contiguous(), dt_bias.contiguous()
+    if _DEBUG_CHECKS:
+        _debug_checks(ids, state_pool.shape[0])
+        _debug_tree(tree, N)
+    y = torch.empty(N, C, dtype=torch.bfloat16, device=dev)
     g = torch.empty(N, vh, dtype=torch.float32, device=dev)
     beta = torch.empty(N, vh, dtype=torch.bfloat16, device=dev)
-    _launch("gdn_conv_gate_tree", dev, _p(x2), xs, _p(state_pool), _slot_stride(state_pool),
-            state_pool.shape[0], _p(ids), _p(tree[0]), ids.numel(), _p(tree[1]), tree[2], N, C, K,
-            _p(w), _p(y), C, _p(b), _p(a), _stride(a.stride(0), N, vh), vh, _p(a_log), _p(dt_bias), pdt,
-            _p(g), _p(beta))
+    _launch("gdn_conv_gate_tree", dev, x.data_ptr(), xs, state_pool.data_ptr(),
+            _slot_stride(state_pool), state_pool.shape[0], ids.data_ptr(), tree[0].data_ptr(),
+            n_seqs, tree[1].data_ptr(), tree[2], N, C, K, weight.data_ptr(), y.data_ptr(), C,
+            b.data_ptr(), a.data_ptr(), a_s, vh, a_log.data_ptr(), dt_bias.data_ptr(), pdt,
+            g.data_ptr(), beta.data_ptr())
     return y, g, beta
 
 
 def _delta_args(k, v, g, beta, s_pool, ids):
     """The checks gated_delta_rule_tree and commit_tree share."""
-    N, HK, DK, ks = _heads(k, "k")
-    N_v, HV, DV, vs = _heads(v, "v")
+    N, HK, DK, ks = _bf16_heads(k, "k")
+    N_v, HV, DV, vs = _bf16_heads(v, "v")
     assert N_v == N and HV % HK == 0
-    assert k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16
-    g = g.reshape(N, HV)
-    beta = beta.reshape(N, HV)
+    assert g.numel() == N * HV and beta.numel() == N * HV and g.shape[-1] == HV and \
+        beta.shape[-1] == HV, "g / beta need one row per token"
     assert g.dtype == torch.float32 and beta.dtype == torch.bfloat16 and g.is_contiguous() and \
         beta.is_contiguous(), "g (fp32) / beta (bf16) must be contiguous"
     _state_view_check(s_pool, HV, DK, DV)
     ids = _ids64(ids)
-    _debug_checks(ids, s_pool.shape[0])
-    return (N, HK, HV, DK, DV, _stride(ks, N, HK * DK), _stride(vs, N, HV * DV), g, beta, ids)
+    if _DEBUG_CHECKS:
+        _debug_checks(ids, s_pool.shape[0])
+    return N, HK, HV, DK, DV, ks, vs, ids
 
 
 def gated_delta_rule_tree(q, k, v, g, beta, s_pool, ids, cu_seqlens, parents, max_nodes: int,
@@ -825,22 +845,33 @@ def gated_delta_rule_tree(q, k, v, g, beta, s_pool, ids, cu_seqlens, parents, ma
     RMSNorm of it, in fp32 up to the one rounding at the end (the single-step
     operators round three times on the way)."""
     dev = _one_device(q, k, v, g, beta, s_pool, ids, cu_seqlens, parents, z, norm_weight)
-    N, HK, HV, DK, DV, ks, vs, g, beta, ids = _delta_args(k, v, g, beta, s_pool, ids)
-    N_q, HK_q, DK_q, qs = _heads(q, "q")
-    assert (N_q, HK_q, DK_q) == (N, HK, DK) and q.dtype == torch.bfloat16
-    tree = _tree(cu_seqlens, parents, max_nodes, ids.numel(), N)
-    _debug_tree(tree, N)
+    N, HK, HV, DK, DV, ks, vs, ids = _delta_args(k, v, g, beta, s_pool, ids)
+    N_q, HK_q, DK_q, qs = _bf16_heads(q, "q")
+    assert N_q == N and HK_q == HK and DK_q == DK
+    n_seqs = ids.numel()
+    tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, N)
+    if _DEBUG_CHECKS:
+        _debug_tree(tree, N)
     if not _aligned_rows(v, vs, 4):
         v, vs = v.clone(memory_format=torch.contiguous_format), HV * DV
-    z3, zs, nw = _norm_args(z, norm_weight, N, HV, DV)
-    zs = _stride(zs, N, HV * DV)
-    if z3 is not None and not _aligned_rows(z3, zs, 4):
-        z3, zs = z3.clone(memory_format=torch.contiguous_format), HV * DV
+    zp, zs, wp = 0, 0, 0
+    if z is not None:
+        assert norm_weight is not None and norm_weight.dtype == torch.bfloat16 and \
+            norm_weight.numel() == DV
+        if z.dim() != 3:
+            z = z.reshape(N, HV, DV)
+        N_z, HV_z, DV_z, zs = _bf16_heads(z, "z")
+        assert N_z == N and HV_z == HV and DV_z == DV, "z must be [rows, HV, DV]"
+        if not _aligned_rows(z, zs, 4):
+            z, zs = z.clone(memory_format=torch.contiguous_format), HV * DV
+        if not norm_weight.is_contiguous():
+            norm_weight = norm_weight.contiguous()
+        zp, wp = z.data_ptr(), norm_weight.data_ptr()
     out = _out_buffer(out, (N, HV, DV), dev)
-    _launch("gdn_delta_rule_tree", dev, _p(q), _stride(qs, N, HK * DK), _p(k), ks, _p(v), vs, _p(g),
-            _p(beta), _p(s_pool), _slot_stride(s_pool), s_pool.shape[0], _p(ids), _p(tree[0]),
-            ids.numel(), _p(tree[1]), tree[2], N, _p(out), HK, HV, DK, DV, DK ** -0.5, _p(z3),
-            zs, _p(nw), float(eps))
+    _launch("gdn_delta_rule_tree", dev, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+            g.data_ptr(), beta.data_ptr(), s_pool.data_ptr(), _slot_stride(s_pool), s_pool.shape[0],
+            ids.data_ptr(), tree[0].data_ptr(), n_seqs, tree[1].data_ptr(), tree[2], N,
+            out.data_ptr(), HK, HV, DK, DV, DK ** -0.5, zp, zs, wp, float(eps))
     return out
 
 
@@ -854,22 +885,33 @@ def commit_tree(x, k, v, g, beta, conv_pool, s_pool, ids, cu_seqlens, parents, m
     its window and the path's rows of ``x`` [N, C], the input of
     :func:`conv_gate_tree`.  Both pools are updated in place."""
     dev = _one_device(x, k, v, g, beta, conv_pool, s_pool, ids, cu_seqlens, parents, accepted)
-    N, HK, HV, DK, DV, ks, vs, g, beta, ids = _delta_args(k, v, g, beta, s_pool, ids)
+    N, HK, HV, DK, DV, ks, vs, ids = _delta_args(k, v, g, beta, s_pool, ids)
     C = x.shape[-1]
-    assert x.dtype == torch.bfloat16
-    x2, xs = _rows2d(x, C)
-    assert x2.shape[0] == N
+    x, N_x, xs = _bf16_rows(x, C, "x")
+    assert N_x == N
     assert conv_pool.dim() == 3 and conv_pool.shape[0] == s_pool.shape[0], \
         "both pools index the same slots"
     K = conv_pool.shape[2] + 1
     _pool_view_check(conv_pool, K - 1, C)
-    tree = _tree(cu_seqlens, parents, max_nodes, ids.numel(), N)
-    accepted = _int32(accepted, ids.numel(), "accepted")
-    _debug_tree(tree, N, accepted)
-    _launch("gdn_commit_tree", dev, _p(x2), _stride(xs, N, C), _p(k), ks, _p(v), vs, _p(g), _p(beta),
-            _p(conv_pool), _slot_stride(conv_pool), C, K, _p(s_pool), _slot_stride(s_pool),
-            s_pool.shape[0], _p(ids), _p(tree[0]), ids.numel(), _p(tree[1]), _p(accepted), tree[2],
-            N, HK, HV, DK, DV)
+    n_seqs = ids.numel()
+    tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, N)
+    accepted = _int32(accepted, n_seqs, "accepted")
+    if _DEBUG_CHECKS:
+        _debug_tree(tree, N, accepted)
+    _launch("gdn_commit_tree", dev, x.data_ptr(), xs, k.data_ptr(), ks, v.data_ptr(), vs,
+            g.data_ptr(), beta.data_ptr(), conv_pool.data_ptr(), _slot_stride(conv_pool), C, K,
+            s_pool.data_ptr(), _slot_stride(s_pool), s_pool.shape[0], ids.data_ptr(),
+            tree[0].data_ptr(), n_seqs, tree[1].data_ptr(), accepted.data_ptr(), tree[2], N, HK, HV,
+            DK, DV)
+
+
+def _block_tables(t: torch.Tensor):
+    """(n_seqs, max_blocks, row stride) of int32 block tables."""
+    assert t.dim() == 2 and t.dtype == torch.int32, "block_tables must be int32 [n_seqs, max_blocks]"
+    n_seqs, n_blocks = t.shape
+    s = t.stride()
+    assert n_blocks <= 1 or s[1] == 1, "block_tables must have dense rows"
+    return n_seqs, n_blocks, (s[0] if n_seqs > 1 else n_blocks)
 
 
 def tree_slot_map(block_tables: torch.Tensor, context_lens: torch.Tensor,
@@ -882,33 +924,33 @@ def tree_slot_map(block_tables: torch.Tensor, context_lens: torch.Tensor,
     the accepted path's nodes get the slot of their position and all others -1.
     Rows behind the last sequence get position 0 and slot -1."""
     dev = _one_device(block_tables, context_lens, cu_seqlens, parents, accepted)
-    assert block_tables.dim() == 2 and block_tables.dtype == torch.int32 and \
-        (block_tables.shape[1] <= 1 or block_tables.stride(1) == 1), \
-        "block_tables must be int32 [n_seqs, max_blocks] with dense rows"
-    n_seqs, n_blocks = block_tables.shape
+    n_seqs, n_blocks, ts = _block_tables(block_tables)
     tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, n_rows)
     context_lens = _int32(context_lens, n_seqs, "context_lens")
+    acc = 0
     if accepted is not None:
         accepted = _int32(accepted, n_seqs, "accepted")
-    _debug_tree(tree, n_rows, accepted)
+        acc = accepted.data_ptr()
+    if _DEBUG_CHECKS:
+        _debug_tree(tree, n_rows, accepted)
     positions = torch.empty(n_rows, dtype=torch.int64, device=dev)
     slots = torch.empty(n_rows, dtype=torch.int32, device=dev)
-    _launch("gdn_tree_slot_map", dev, _p(block_tables), _stride(block_tables.stride(0), n_seqs, n_blocks),
-            n_blocks, _p(context_lens), _p(tree[0]), n_seqs, _p(tree[1]), _p(accepted), tree[2],
-            int(block_size), n_rows, _p(positions), _p(slots))
+    _launch("gdn_tree_slot_map", dev, block_tables.data_ptr(), ts, n_blocks,
+            context_lens.data_ptr(), tree[0].data_ptr(), n_seqs, tree[1].data_ptr(), acc, tree[2],
+            int(block_size), n_rows, positions.data_ptr(), slots.data_ptr())
     return positions, slots
 
 
 def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, HKV: int, D: int):
     """The strides (block, token, head) that both caches share."""
-    assert k_cache.dim() == 4 and tuple(k_cache.shape[2:]) == (HKV, D) and \
-        k_cache.shape == v_cache.shape, f"caches must be [blocks, block_size, {HKV}, {D}]"
+    shape, st = k_cache.shape, k_cache.stride()
+    assert len(shape) == 4 and shape[2] == HKV and shape[3] == D and v_cache.shape == shape, \
+        f"caches must be [blocks, block_size, {HKV}, {D}]"
     assert k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16
-    assert k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1, \
+    assert v_cache.stride() == st and st[3] == 1, \
         "caches must have the same strides and dense heads"
     # a dimension of one entry may have any stride: it is never stepped along
-    return tuple(k_cache.stride(i) if k_cache.shape[i] > 1 else max(k_cache.stride(i) // 8 * 8, D)
-                 for i in range(3))
+    return tuple(s if n > 1 else D for n, s in zip(shape[:3], st))
 
 
 def qk_norm_rope_cache(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache,
@@ -924,17 +966,15 @@ def qk_norm_rope_cache(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache,
     Returns the rotated queries [N, HQ, D]; fp32 up to the one rounding at the end."""
     dev = _one_device(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache,
                       slot_mapping)
-    N, HQ, D, qs = _heads(q, "q")
-    N_k, HKV, D_k, ks = _heads(k, "k")
-    assert (N_k, D_k) == (N, D) and v.shape == k.shape
-    vs = _stride(_heads(v, "v")[3], N, HKV * D)
-    qs, ks = _stride(qs, N, HQ * D), _stride(ks, N, HKV * D)
-    assert q.dtype == k.dtype == v.dtype == torch.bfloat16
-    assert q_weight.dtype == k_weight.dtype == torch.bfloat16
+    N, HQ, D, qs = _bf16_heads(q, "q")
+    N_k, HKV, D_k, ks = _bf16_heads(k, "k")
+    N_v, HKV_v, D_v, vs = _bf16_heads(v, "v")
+    assert N_k == N and N_v == N and D_k == D and D_v == D and HKV_v == HKV
+    assert q_weight.dtype == torch.bfloat16 and k_weight.dtype == torch.bfloat16
     assert q_weight.numel() == D and k_weight.numel() == D
     assert cos_sin.dim() == 2 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous(), \
         "cos_sin must be a contiguous fp32 [positions, rotary_dim]"
-    assert positions.dim() == 1 and positions.numel() == N and not positions.is_floating_point()
+    assert positions.numel() == N and not positions.is_floating_point()
     positions = _ids64(positions)
     slot_mapping = _int32(slot_mapping, N, "slot_mapping")
     bs, ts, hs = _paged_cache(k_cache, v_cache, HKV, D)
@@ -944,11 +984,18 @@ def qk_norm_rope_cache(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache,
         k, ks = k.clone(memory_format=torch.contiguous_format), HKV * D
     if not _aligned_rows(v, vs, 8):
         v, vs = v.clone(memory_format=torch.contiguous_format), HKV * D
+    if not q_weight.is_contiguous():
+        q_weight = q_weight.contiguous()
+    if not k_weight.is_contiguous():
+        k_weight = k_weight.contiguous()
     out = _out_buffer(out, (N, HQ, D), dev)
-    _launch("gdn_qk_norm_rope_cache", dev, _p(q), qs, _p(k), ks, _p(v), vs,
-            _p(q_weight.contiguous()), _p(k_weight.contiguous()), float(eps), int(unit_offset),
-            _p(cos_sin), cos_sin.shape[0], cos_sin.shape[1], _p(positions), _p(k_cache), _p(v_cache), bs, ts, hs, k_cache.shape[0], k_cache.shape[1],
-            _p(slot_mapping), _p(out), N, HQ, HKV, D)
+    blocks, block_size = k_cache.shape[:2]
+    max_pos, rot = cos_sin.shape
+    _launch("gdn_qk_norm_rope_cache", dev, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+            q_weight.data_ptr(), k_weight.data_ptr(), float(eps), int(unit_offset),
+            cos_sin.data_ptr(), max_pos, rot, positions.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), bs, ts, hs, blocks, block_size, slot_mapping.data_ptr(),
+            out.data_ptr(), N, HQ, HKV, D)
     return out
 
 
@@ -964,28 +1011,26 @@ def attention_tree(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, 
     context_lens[r] + the sequence's nodes (a longer sequence is skipped and
     flagged).  ``scale`` defaults to D ** -0.5.  Returns out [N, HQ, D]."""
     dev = _one_device(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, parents)
-    N, HQ, D, qs = _heads(q, "q")
-    qs = _stride(qs, N, HQ * D)
+    N, HQ, D, qs = _bf16_heads(q, "q")
     assert k_cache.dim() == 4
     HKV = k_cache.shape[2]
-    assert q.dtype == torch.bfloat16 and HQ % HKV == 0
+    assert HQ % HKV == 0
     bs, ts, hs = _paged_cache(k_cache, v_cache, HKV, D)
-    assert block_tables.dim() == 2 and block_tables.dtype == torch.int32 and \
-        (block_tables.shape[1] <= 1 or block_tables.stride(1) == 1), \
-        "block_tables must be int32 [n_seqs, max_blocks] with dense rows"
-    n_seqs, n_blocks = block_tables.shape
+    n_seqs, n_blocks, tstride = _block_tables(block_tables)
     tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, N)
     context_lens = _int32(context_lens, n_seqs, "context_lens")
-    _debug_tree(tree, N)
+    if _DEBUG_CHECKS:
+        _debug_tree(tree, N)
     if not _aligned_rows(q, qs, 8):
         q, qs = q.clone(memory_format=torch.contiguous_format), HQ * D
     out = _out_buffer(out, (N, HQ, D), dev)
     max_len = int(max_len)
     need = _lib.load().gdn_attention_tree_workspace_bytes(N, n_seqs, HQ, HKV, D, tree[2], max_len)
+    # made per call: calls on several streams, or graphs that hold one each, never share it
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _launch("gdn_attention_tree", dev, _p(q), qs, _p(k_cache), _p(v_cache), bs, ts,
-            hs, k_cache.shape[0], k_cache.shape[1], _p(block_tables),
-            _stride(block_tables.stride(0), n_seqs, n_blocks), n_blocks, _p(context_lens), _p(tree[0]), n_seqs,
-            _p(tree[1]), tree[2], N, max_len, _p(out), HQ, HKV, D,
-            D ** -0.5 if scale is None else float(scale), _p(ws), need)
+    _launch("gdn_attention_tree", dev, q.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(), bs,
+            ts, hs, k_cache.shape[0], k_cache.shape[1], block_tables.data_ptr(), tstride, n_blocks,
+            context_lens.data_ptr(), tree[0].data_ptr(), n_seqs, tree[1].data_ptr(), tree[2], N,
+            max_len, out.data_ptr(), HQ, HKV, D, D ** -0.5 if scale is None else float(scale),
+            _p(ws), need)
     return out
