@@ -58,7 +58,7 @@ SIGNATURES = {
                         i32, vp, vp, i32, i64, i32, i32, i32, i32, vp, vp],
     "gdn_qk_norm_rope_cache": [vp, i64, vp, i64, vp, i64, vp, vp, f32, i32, vp, i64, i32, vp, vp,
                                vp, i64, i64, i64, i64, i32, vp, vp, i64, i32, i32, i32, vp, vp],
-    "gdn_attention_tree_workspace_bytes": [i64, i32, i32, i32, i32, i32, i32],
+    "gdn_attention_tree_workspace_bytes": [i32, i32, i32, i32, i32],
     "gdn_attention_tree": [vp, i64, vp, vp, i64, i64, i64, i64, i32, vp, i64, i32, vp, vp, i32, vp,
                            i32, i64, i32, vp, i32, i32, i32, f32, vp, i64, vp, vp],
     "gdn_tree_slot_map": [vp, i64, i32, vp, vp, i32, vp, vp, i32, i32, i64, vp, vp, vp, vp],

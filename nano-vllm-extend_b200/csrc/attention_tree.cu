@@ -7,36 +7,42 @@
 //
 // HBM: every cached key and value of a sequence is read once (4 D bytes per
 // position and kv-head), so the G = HQ / HKV query heads of a kv-head and all
-// nodes form the rows of one tile: 16 WM rows per CTA.  Work is split along the
-// positions in chunks, so few sequences still fill the GPU and long ones do not
-// run behind the others; with more than one chunk each writes its rows' running
-// maximum, sum and weighted values in fp32 and a second launch joins them.
+// nodes form the rows of one tile of BM = 16 WM rows (more rows: further tiles).
 //
-// One pass over a chunk with the running maximum and sum of the softmax: tiles
-// of BN positions arrive by cp.async, three stages deep, rows swizzled for
-// ldmatrix; WM warps over rows x WN warps over positions, scores and
-// probabilities stay in registers (the score tile's accumulators are the next
-// product's A operand).  Sums and statistics are fp32; the probabilities are
+// Work is cut evenly, whatever the sequences' lengths: all tiles of BN positions of
+// all (sequence, kv-head, row tile) units in one line, of which each CTA takes an
+// equal run; every CTA finds its place by a scan over the lengths.  A unit that one CTA
+// holds whole is finished there; of one that is cut each CTA writes its rows' running
+// maximum, sum and weighted values in fp32, and a second launch joins them.  (Chunks of
+// a fixed length, one CTA each, left 128 sequences of 256 to 4352 positions at half the
+// copy rate: half of the CTAs had nothing to do, the others started up for 10 tiles.)
+//
+// A producer warp brings the tiles by TMA (boxes of as many positions as divide a
+// page, 128-byte swizzle) into a ring of stages, across unit borders; WM warps over
+// rows x WN warps over positions run one pass with the softmax's running maximum
+// and sum, scores and probabilities in registers (the score tile's accumulators are
+// the next product's A operand).  Sums and statistics are fp32; the probabilities are
 // rounded to bf16 as an operand of the second product, as the values are bf16.
 //
-// Positions behind the last node are filled with zeros, not read.  A node's
-// value row that is not finite must not reach nodes off its path (probability
-// zero times NaN): in tiles that hold nodes such rows are zeroed in shared
-// memory and the nodes that do see them get NaN outputs.
+// In the tiles that hold nodes or reach behind them, value rows behind the last node
+// are zeroed in shared memory, and so are nodes' rows that are not finite, which must
+// not reach nodes off their path (probability zero times NaN); the nodes that do see
+// one of those get NaN outputs.
 #include "mma_util.cuh"
 #include "tc_util.cuh"
+#include "tmap.cuh"
 #include "tree.cuh"
 
 namespace gdn {
 
-constexpr int kAttnStages = 3;
+constexpr uint32_t kAttnWait = 1u << 22;      // polls
+constexpr int kAttnSms = 148;
 
 struct AttnArgs {
   const bf16* q;
   int64_t qs;
-  const bf16 *k_cache, *v_cache;
-  int64_t block_stride, token_stride, head_stride, num_blocks;
-  int block_size;
+  int64_t num_blocks;
+  int block_size, box;            // positions of a page, and of one TMA box (divides it)
   const int32_t* tables;
   int64_t table_stride;
   int max_blocks;
@@ -48,416 +54,597 @@ struct AttnArgs {
   int64_t n_tokens;
   int max_len;
   bf16* out;
-  int HQ, HKV;
+  int HQ, HKV, G;
   float scale_log2;
-  int chunk, chunks, row_tiles;   // positions per chunk, chunks of the longest sequence
-  float* part_o;                  // [chunks][n_tokens * HQ][D]
-  float2* part_ml;                // [chunks][n_tokens * HQ]: maximum (base 2), sum
+  int64_t* prefix;                // [n_seqs + 1]: tiles before each sequence's
+  float* part_o;                  // [CTAs][2][BM][D]
+  float2* part_ml;                // [CTAs][2][BM]: maximum (base 2), sum
   int32_t* status;
 };
 
-// Context length of sequence r; false (and flagged) where it is negative or the
-// sequence is longer than the host's bound.
-__device__ __forceinline__ bool attn_len(const AttnArgs& a, int r, int n, int64_t& c) {
-  c = a.ctx[r];
-  if (c < 0 || c + n > a.max_len) {
-    if (a.status) atomicOr(a.status, GDN_STATUS_BAD_SEQLEN);
-    return false;
-  }
-  return true;
-}
-
-template <int D, int WM, int WN, int BN>
-struct AttnSmem {
-  bf16 q[16 * WM][D];
-  bf16 k[kAttnStages][BN][D];
-  bf16 v[kAttnStages][BN][D];
-  unsigned long long anc[kMaxTreeNodes];
-  unsigned long long bad;
-  int par[kMaxTreeNodes];
+// A sequence as attention sees it; n = 0: nothing to compute.
+struct AttnSeq {
+  int64_t start;
+  int n, ctx, tiles, row_tiles;
 };
 
-// Byte offset of 16-byte piece c of row r in a tile of D-wide bf16 rows: pieces
-// of 8 consecutive rows land in different banks.
-template <int D>
-__device__ __forceinline__ uint32_t tile_at(int r, int c) {
-  return (uint32_t)(r * D * 2 + ((c ^ (r & 7)) << 4));
+template <int BM, int BN>
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int r, int32_t* status) {
+  AttnSeq s{0, 0, 0, 0, 0};
+  int n;
+  if (!tree_rows(a.cu, r, a.n_tokens, a.max_nodes, status, s.start, n) || n == 0) return s;
+  const int c = a.ctx[r];
+  if (c < 0 || (int64_t)c + n > a.max_len) {
+    if (status) atomicOr(status, GDN_STATUS_BAD_SEQLEN);
+    return s;
+  }
+  s.n = n;
+  s.ctx = c;
+  s.tiles = (c + n + BN - 1) / BN;
+  s.row_tiles = (n * a.G + BM - 1) / BM;
+  return s;
 }
 
-template <int D, int WM, int WN, int BN>
-__global__ void __launch_bounds__(32 * WM * WN) attention_tree_kernel(const AttnArgs a) {
-  using S = AttnSmem<D, WM, WN, BN>;
-  constexpr int NT = 32 * WM * WN, BM = 16 * WM, PC = D / 8;
-  constexpr int WT = BN / WN;                 // positions of a tile per warp
+template <int D, int WM, int WN>
+struct Attn {
+  static constexpr int BM = 16 * WM, BN = 64, NC = WM * WN;      // NC: consumer warps
+  static constexpr int WT = BN / WN;                              // positions per warp
+  static constexpr int HALVES = D / 64;                           // 128-byte column blocks
+  static constexpr int CTAS = D <= 128 && WM <= 4 ? 2 : 1;        // per SM
+  static constexpr int STAGE = 2 * BN * D * 2;                    // bytes of keys and values
+  static constexpr int ST = CTAS == 2 ? (D == 64 ? 5 : 3) : (D == 256 ? 3 : 5);
+  struct Smem {
+    __align__(1024) unsigned char kv[ST][2][HALVES][BN * 128];
+    __align__(16) float join[WN > 1 ? WN * BM * 36 : 4];          // 32 columns at a time
+    float2 ml[WN > 1 ? WN * BM : 1];
+    unsigned long long anc[kMaxTreeNodes];
+    unsigned long long full[ST], empty[ST], bad;
+    int64_t scan_base, scan_total;
+    int scan_warp[NC + 1], scan_seq;
+    int par[kMaxTreeNodes];
+  };
+};
+
+// 2^x by the hardware's instruction (2 ulp; results below 2^-126 become zero).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Byte offset of 16-byte piece c of row r in a [HALVES][BN] tile of 128-byte swizzled rows.
+template <int BN>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  return (uint32_t)((c >> 3) * (BN * 128) + r * 128 + (((c ^ r) & 7) << 4));
+}
+
+template <int D, int WM, int WN>
+__global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
+    attention_tree_kernel(const __grid_constant__ CUtensorMap kmap,
+                          const __grid_constant__ CUtensorMap vmap, const AttnArgs a) {
+  using P = Attn<D, WM, WN>;
+  constexpr int NC = P::NC, NT = 32 * (NC + 1), BM = P::BM, BN = P::BN, WT = P::WT, ST = P::ST;
   static_assert(WT % 16 == 0, "a warp takes whole 16-position blocks");
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  S& sm = *reinterpret_cast<S*>(smem_raw);
-  int* pages = reinterpret_cast<int*>(smem_raw + sizeof(S));
+  extern __shared__ unsigned char smem_raw[];
+  auto& sm = *reinterpret_cast<typename P::Smem*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  const int rt = blockIdx.x % a.row_tiles;
-  const int kvh = (blockIdx.x / a.row_tiles) % a.HKV;
-  const int seq = blockIdx.x / (a.row_tiles * a.HKV);
-  const int chunk = blockIdx.y;
-  const int G = a.HQ / a.HKV;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tq = lane & 3;
-  const int wm = warp / WN, wn = warp - wm * WN;
-  int64_t start, ctx;
-  int n;
-  if (!tree_rows(a.cu, seq, a.n_tokens, a.max_nodes, a.status, start, n) ||
-      !attn_len(a, seq, n, ctx))
-    return;
-  const int row0 = rt * BM, rows = n * G;     // rows: node * G + head within the group
-  const int total = (int)ctx + n;
-  const int p_begin = chunk * a.chunk, p_end = min(total, p_begin + a.chunk);
-  if (row0 >= rows || p_begin >= p_end) return;
-
-  // the chunk's pages
-  const int page0 = p_begin / a.block_size, n_pages = (p_end - 1) / a.block_size - page0 + 1;
-  for (int i = tid; i < n_pages; i += NT) {
-    int p = page0 + i < a.max_blocks ? a.tables[seq * a.table_stride + page0 + i] : -1;
-    if (p < 0 || p >= a.num_blocks) {
-      if (a.status) atomicOr(a.status, GDN_STATUS_BAD_SLOT);
-      p = -1;
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      tc::mbar_init(tc::smem_u32(&sm.full[i]), 1);
+      tc::mbar_init(tc::smem_u32(&sm.empty[i]), NC);
     }
-    pages[i] = p;
+    tc::mbar_init_fence();
   }
-  if (tid < n) sm.par[tid] = tree_parent(a.parents[start + tid], tid, a.status);
-  if (tid == 0) sm.bad = 0;
-  // query rows
-  for (int i = tid; i < BM * PC; i += NT) {
-    const int r = i / PC, c = i - r * PC;
-    const int row = row0 + r;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (row < rows) {
-      const int node = row / G;
-      u = *reinterpret_cast<const uint4*>(a.q + (start + node) * a.qs +
-                                          (int64_t)(kvh * G + row - node * G) * D + c * 8);
+  // ---- this CTA's run of tiles: scan the sequences in strips of NT ----
+  const auto weight = [&](int r, int32_t* status) -> int64_t {
+    if (r >= a.n_seqs) return 0;
+    const AttnSeq s = attn_seq<BM, BN>(a, r, status);
+    return (int64_t)s.tiles * s.row_tiles * a.HKV;
+  };
+  const auto strip_sum = [&](int64_t v) {            // block-wide sum, and the sum before this thread
+    int64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
     }
-    *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(sm.q) + tile_at<D>(r, c)) = u;
+    // a strip's tiles fit 31 bits: NT sequences of at most 2^24 tiles (host check)
+    __syncthreads();
+    if (lane == 31) sm.scan_warp[warp] = (int)inc;
+    __syncthreads();
+    int64_t before = inc - v, total = 0;
+    for (int w = 0; w <= NC; ++w) {
+      if (w < warp) before += sm.scan_warp[w];
+      total += sm.scan_warp[w];
+    }
+    return make_longlong2(before, total);
+  };
+  int64_t total = 0;
+  const bool scribe = blockIdx.x == 0;
+  longlong2 first{0, 0};
+  for (int s0 = 0; s0 < a.n_seqs; s0 += NT) {
+    const longlong2 st = strip_sum(weight(s0 + tid, scribe ? a.status : nullptr));
+    if (s0 == 0) first = st;
+    if (scribe && s0 + tid < a.n_seqs) a.prefix[s0 + tid] = total + st.x;
+    total += st.y;
+  }
+  if (scribe && tid == 0) a.prefix[a.n_seqs] = total;
+  // no run is empty: fewer tiles than CTAs go to as many CTAs
+  const int64_t ctas = min((int64_t)gridDim.x, total);
+  if (blockIdx.x >= ctas) return;
+  const int64_t w0 = total * blockIdx.x / ctas, w1 = total * (blockIdx.x + 1) / ctas;
+  int64_t base = 0;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += NT) {
+    const int64_t v = weight(s0 + tid, nullptr);
+    const longlong2 st = a.n_seqs <= NT ? first : strip_sum(v);
+    const int64_t at = base + st.x;
+    if (w0 >= at && w0 < at + v) {
+      sm.scan_seq = s0 + tid;
+      sm.scan_base = at;
+    }
+    base += st.y;
+    if (base > w0) break;
   }
   __syncthreads();
-  if (tid < n) {
-    unsigned long long m = 0;
-    for (int j = tid; j >= 0; j = sm.par[j]) m |= 1ull << j;
-    sm.anc[tid] = m;
-  }
 
-  const int tiles = (p_end - p_begin + BN - 1) / BN;
-  auto load_tile = [&](int tile, int stage) {
-    const uint32_t k0 = tc::smem_u32(&sm.k[stage][0][0]), v0 = tc::smem_u32(&sm.v[stage][0][0]);
-    for (int i = tid; i < BN * PC; i += NT) {
-      const int r = i / PC, c = i - r * PC;
-      const int p = p_begin + tile * BN + r;
-      int64_t off = 0;
-      uint32_t bytes = 0;
-      if (p < p_end) {
-        const int blk = p / a.block_size;
-        const int page = pages[blk - page0];
-        if (page >= 0) {
-          off = page * a.block_stride + (p - blk * a.block_size) * a.token_stride +
-                kvh * a.head_stride + c * 8;
-          bytes = 16;
-        }
-      }
-      tc::cp_async16(k0 + tile_at<D>(r, c), a.k_cache + off, bytes);
-      tc::cp_async16(v0 + tile_at<D>(r, c), a.v_cache + off, bytes);
+  // ---- the run, a segment (part of a unit) at a time; every warp keeps the same place ----
+  int seq = sm.scan_seq;
+  int64_t seq_base = sm.scan_base;
+  int it = 0;                                        // tiles of this CTA so far
+  for (int64_t w = w0; w < w1;) {
+    const AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
+    const int64_t mine = (int64_t)s.tiles * s.row_tiles * a.HKV;
+    if (w >= seq_base + mine) {
+      seq_base += mine;
+      ++seq;
+      continue;
     }
-  };
-#pragma unroll
-  for (int s = 0; s < kAttnStages - 1; ++s) {
-    if (s < tiles) load_tile(s, s);
-    tc::cp_async_commit();
-  }
+    const int64_t local = w - seq_base;
+    const int unit = (int)(local / s.tiles), tile0 = (int)(local - (int64_t)unit * s.tiles);
+    const int kvh = unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
+    const int seg = (int)min((int64_t)(s.tiles - tile0), w1 - w);
+    const int len = s.ctx + s.n;
 
-  float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-  const int my_row[2] = {row0 + wm * 16 + gr, row0 + wm * 16 + gr + 8};
-  const uint32_t q_base = tc::smem_u32(&sm.q[0][0]);
-
-  for (int tile = 0; tile < tiles; ++tile) {
-    tc::cp_async_wait<kAttnStages - 2>();
-    __syncthreads();                          // tile has arrived; the stage loaded next is free
-    if (tile + kAttnStages - 1 < tiles)
-      load_tile(tile + kAttnStages - 1, (tile + kAttnStages - 1) % kAttnStages);
-    tc::cp_async_commit();
-    const int stage = tile % kAttnStages;
-    const int p_tile = p_begin + tile * BN;
-    const bool edge = p_tile + BN > (int)ctx;   // holds nodes or positions behind them
-    if (edge) {
-      // value rows of nodes: zero what is not finite and note whose it is
-      unsigned char* vt = reinterpret_cast<unsigned char*>(&sm.v[stage][0][0]);
-      for (int i = tid; i < BN * PC; i += NT) {
-        const int r = i / PC, c = i - r * PC;
-        const int j = p_tile + r - (int)ctx;
-        if (j < 0 || j >= n) continue;
-        uint4* p = reinterpret_cast<uint4*>(vt + tile_at<D>(r, c));
-        const uint4 u = *p;
-        float f[8];
-        unpack8(u, f);
-        bool finite = true;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) finite &= fabsf(f[e]) <= 3.4e38f;
-        if (!finite) {
-          *p = make_uint4(0, 0, 0, 0);
-          atomicOr(&sm.bad, 1ull << j);
-        }
-      }
-      __syncthreads();
-    }
-
-    // scores of this warp's 16 rows x WT positions
-    float s[WT / 8][4];
-#pragma unroll
-    for (int i = 0; i < WT / 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
-    const uint32_t k_base = tc::smem_u32(&sm.k[stage][0][0]);
-#pragma unroll
-    for (int kb = 0; kb < D / 16; ++kb) {
-      uint32_t qa[4];
-      mm::ldsm4(qa, q_base + tile_at<D>(wm * 16 + (lane & 15), kb * 2 + (lane >> 4)));
-#pragma unroll
-      for (int i = 0; i < WT / 8; i += 2) {
-        uint32_t b[4];
-        mm::ldsm4(b, k_base + tile_at<D>(wn * WT + i * 8 + (lane >> 4) * 8 + (lane & 7),
-                                         kb * 2 + ((lane >> 3) & 1)));
-        mm::mma16816(s[i], qa, b[0], b[1]);
-        mm::mma16816(s[i + 1], qa, b[2], b[3]);
-      }
-    }
-    // masks and scale
-    if (edge || p_tile + BN > p_end) {
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const unsigned long long m = my_row[hh] < rows ? sm.anc[my_row[hh] / G] : 0ull;
-#pragma unroll
-        for (int i = 0; i < WT / 8; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int p = p_tile + wn * WT + i * 8 + 2 * tq + e;
-            const int j = p - (int)ctx;
-            const bool seen = p < p_end && (j < 0 || (j < n && (m >> (j & 63) & 1)));
-            float& x = s[i][hh * 2 + e];
-            x = seen ? x * a.scale_log2 : -INFINITY;
+    if (warp == NC) {
+      // ---- producer: a lane per box looks its page up, 32 boxes ahead ----
+      const int per_tile = BN / a.box;               // boxes of a tile
+      for (int b0 = 0; b0 < seg * per_tile; b0 += 32) {
+        const int p_box = (tile0 * per_tile + b0 + lane) * a.box;
+        int page = -2, row = 0;                      // -2: behind the last node, nothing to load
+        if (b0 + lane < seg * per_tile && p_box < len) {
+          const int blk = p_box / a.block_size;
+          row = p_box - blk * a.block_size;
+          page = blk < a.max_blocks ? a.tables[seq * a.table_stride + blk] : -1;
+          if (page < 0 || page >= a.num_blocks) {
+            if (a.status) atomicOr(a.status, GDN_STATUS_BAD_SLOT);
+            page = -2;
           }
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+        const int boxes = min(32, seg * per_tile - b0);
+        for (int i = 0; i < boxes; ++i) {
+          const int in_tile = (b0 + i) % per_tile;
+          const int t = it + (b0 + i) / per_tile, stage = t % ST;
+          const int pg = __shfl_sync(0xffffffffu, page, i), rw = __shfl_sync(0xffffffffu, row, i);
+          if (lane == 0) {
+            const uint32_t full = tc::smem_u32(&sm.full[stage]);
+            if (in_tile == 0) {
+              if (!tc::mbar_wait(tc::smem_u32(&sm.empty[stage]), ((t / ST) & 1) ^ 1, kAttnWait) &&
+                  a.status)
+                atomicOr(a.status, GDN_STATUS_TIMEOUT);
+            }
+            if (in_tile == 0 || i == 0) {
+              // the boxes of this tile that this round of 32 issues; the tile's last
+              // round makes the arrival
+              const int m = min(per_tile - in_tile, boxes - i);
+              const int live = __popc(there >> i & (m == 32 ? 0xffffffffu : (1u << m) - 1));
+              const uint32_t bytes = (uint32_t)live * a.box * D * 4;
+              if (in_tile + m == per_tile) tc::mbar_expect_tx(full, bytes);
+              else asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full),
+                                "r"(bytes) : "memory");
+            }
+            if (pg >= 0) {
+#pragma unroll
+              for (int hf = 0; hf < P::HALVES; ++hf) {
+                const uint32_t off = in_tile * a.box * 128;
+                asm volatile(
+                    "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+                    "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(tc::smem_u32(&sm.kv[stage][0][hf][0]) + off),
+                    "l"(&kmap), "r"(hf * 64), "r"(kvh), "r"(rw), "r"(pg), "r"(full)
+                    : "memory");
+                asm volatile(
+                    "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+                    "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(tc::smem_u32(&sm.kv[stage][1][hf][0]) + off),
+                    "l"(&vmap), "r"(hf * 64), "r"(kvh), "r"(rw), "r"(pg), "r"(full)
+                    : "memory");
+              }
+            }
+          }
+          __syncwarp();
+        }
       }
     } else {
-#pragma unroll
-      for (int i = 0; i < WT / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][e] *= a.scale_log2;
-    }
-    // running maximum and sum (base 2)
-    uint32_t pa[WT / 16][4];
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      float m = mx[hh];
-#pragma unroll
-      for (int i = 0; i < WT / 8; ++i) m = fmaxf(m, fmaxf(s[i][hh * 2], s[i][hh * 2 + 1]));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const float base = m == -INFINITY ? 0.f : m;    // a row that has seen nothing yet
-      const float corr = exp2f(mx[hh] - base);
-      mx[hh] = m;
-      float add = 0.f;
-#pragma unroll
-      for (int i = 0; i < WT / 8; ++i) {
-        s[i][hh * 2] = exp2f(s[i][hh * 2] - base);
-        s[i][hh * 2 + 1] = exp2f(s[i][hh * 2 + 1] - base);
-        add += s[i][hh * 2] + s[i][hh * 2 + 1];
+      // ---- consumers ----
+      const auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(NC * 32) : "memory"); };
+      const int gr = lane >> 2, tq = lane & 3, wm = warp / WN, wn = warp - wm * WN;
+      const int row0 = rt * BM, rows = s.n * a.G;    // rows: node * G + head within the group
+      const int my_row[2] = {row0 + wm * 16 + gr, row0 + wm * 16 + gr + 8};
+      const bool idle = row0 + wm * 16 >= rows;      // no row of this warp exists
+      const bool masks = (tile0 + seg) * BN > s.ctx; // the segment reaches the nodes
+      if (masks) {
+        if (tid < s.n) sm.par[tid] = tree_parent(a.parents[s.start + tid], tid, a.status);
+        if (tid == 0) sm.bad = 0;
+        sync();
+        if (tid < s.n) {
+          unsigned long long m = 0;
+          for (int j = tid; j >= 0; j = sm.par[j]) m |= 1ull << j;
+          sm.anc[tid] = m;
+        }
       }
-      sum[hh] = sum[hh] * corr + add;
+      int node[2];
+      const bf16* qp[2];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][hh * 2] *= corr;
-        o[i][hh * 2 + 1] *= corr;
+      for (int hh = 0; hh < 2; ++hh) {
+        node[hh] = min(my_row[hh], rows - 1) / a.G;
+        qp[hh] = a.q + (s.start + node[hh]) * a.qs +
+                 (int64_t)(kvh * a.G + min(my_row[hh], rows - 1) - node[hh] * a.G) * D + 2 * tq;
       }
-    }
+      uint32_t qa[D / 16][4];
 #pragma unroll
-    for (int i = 0; i < WT / 16; ++i) {
-      pa[i][0] = mm::pack2(s[2 * i][0], s[2 * i][1]);
-      pa[i][1] = mm::pack2(s[2 * i][2], s[2 * i][3]);
-      pa[i][2] = mm::pack2(s[2 * i + 1][0], s[2 * i + 1][1]);
-      pa[i][3] = mm::pack2(s[2 * i + 1][2], s[2 * i + 1][3]);
-    }
-    const uint32_t v_base = tc::smem_u32(&sm.v[stage][0][0]);
-#pragma unroll
-    for (int i = 0; i < WT / 16; ++i)
-#pragma unroll
-      for (int c = 0; c < D / 8; c += 2) {
-        uint32_t b[4];
-        mm::ldsm4t(b, v_base + tile_at<D>(wn * WT + i * 16 + (lane & 15), c + (lane >> 4)));
-        mm::mma16816(o[c], pa[i], b[0], b[1]);
-        mm::mma16816(o[c + 1], pa[i], b[2], b[3]);
+      for (int kb = 0; kb < D / 16; ++kb) {
+        qa[kb][0] = *reinterpret_cast<const uint32_t*>(qp[0] + kb * 16);
+        qa[kb][1] = *reinterpret_cast<const uint32_t*>(qp[1] + kb * 16);
+        qa[kb][2] = *reinterpret_cast<const uint32_t*>(qp[0] + kb * 16 + 8);
+        qa[kb][3] = *reinterpret_cast<const uint32_t*>(qp[1] + kb * 16 + 8);
       }
-  }
-  tc::cp_async_wait<0>();
-#pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
-    sum[hh] += __shfl_xor_sync(0xffffffffu, sum[hh], 1);
-    sum[hh] += __shfl_xor_sync(0xffffffffu, sum[hh], 2);
-  }
+      if (masks) sync();
+      unsigned long long anc[2] = {0, 0};
+      if (masks) {
+        anc[0] = my_row[0] < rows ? sm.anc[node[0]] : 0ull;
+        anc[1] = my_row[1] < rows ? sm.anc[node[1]] : 0ull;
+      }
 
-  // join the WN warps of a row tile through shared memory (the stages are free)
-  if constexpr (WN > 1) {
-    __syncthreads();
-    float2* ml = reinterpret_cast<float2*>(&sm.k[0][0][0]);          // [WN][BM]
-    float* os = reinterpret_cast<float*>(ml + WN * BM);              // [WN][BM][D + 4]
-    static_assert(sizeof(float2) * WN * BM + sizeof(float) * WN * BM * (D + 4) <=
-                      sizeof(sm.k) + sizeof(sm.v),
-                  "the joined rows fit the stages");
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int r = wm * 16 + gr + hh * 8;
-      if (tq == 0) ml[wn * BM + r] = make_float2(mx[hh], sum[hh]);
+      float o[D / 8][4];
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
-        *reinterpret_cast<float2*>(&os[(wn * BM + r) * (D + 4) + i * 8 + 2 * tq]) =
-            make_float2(o[i][hh * 2], o[i][hh * 2 + 1]);
-    }
-    __syncthreads();
-    // every thread finishes pieces of 4 columns
-    for (int i = tid; i < BM * (D / 4); i += NT) {
-      const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
-      const int row = row0 + r;
-      if (row >= rows) continue;
-      float m = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < WN; ++w) m = fmaxf(m, ml[w * BM + r].x);
-      const float base = m == -INFINITY ? 0.f : m;
-      float l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+      float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+
+      for (int t = 0; t < seg; ++t) {
+        const int stage = (it + t) % ST;
+        if (!tc::mbar_wait(tc::smem_u32(&sm.full[stage]), ((it + t) / ST) & 1, kAttnWait)) {
+          if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
+          tc::mbar_wait(tc::smem_u32(&sm.full[stage]), ((it + t) / ST) & 1, kAttnWait);
+        }
+        const int p_tile = (tile0 + t) * BN;
+        const bool edge = p_tile + BN > s.ctx;       // holds nodes or positions behind them
+        if (edge) {
+          unsigned char* vt = &sm.kv[stage][1][0][0];
+          for (int i = tid; i < BN * (D / 8); i += NC * 32) {
+            const int r = i / (D / 8), c = i - r * (D / 8), j = p_tile + r - s.ctx;
+            if (j < 0) continue;
+            uint4* p = reinterpret_cast<uint4*>(vt + tile_at<BN>(r, c));
+            float f[8];
+            unpack8(*p, f);
+            bool finite = true;
 #pragma unroll
-      for (int w = 0; w < WN; ++w) {
-        const float2 p = ml[w * BM + r];
-        const float f = exp2f(p.x - base);
-        const float4 t = *reinterpret_cast<const float4*>(&os[(w * BM + r) * (D + 4) + c]);
-        l = fmaf(p.y, f, l);
-        acc.x = fmaf(t.x, f, acc.x);
-        acc.y = fmaf(t.y, f, acc.y);
-        acc.z = fmaf(t.z, f, acc.z);
-        acc.w = fmaf(t.w, f, acc.w);
+            for (int e = 0; e < 8; ++e) finite &= fabsf(f[e]) <= 3.4e38f;
+            if (j >= s.n || !finite) {
+              *p = make_uint4(0, 0, 0, 0);
+              if (j < s.n) atomicOr(&sm.bad, 1ull << j);
+            }
+          }
+          sync();
+        }
+        if (!idle) {
+          const uint32_t k_base = tc::smem_u32(&sm.kv[stage][0][0][0]);
+          const uint32_t v_base = tc::smem_u32(&sm.kv[stage][1][0][0]);
+          // XT positions at a time: their scores and probabilities stay in registers
+          constexpr int XT = WT > 32 ? 32 : WT;
+#pragma unroll
+          for (int x0 = 0; x0 < WT; x0 += XT) {
+            const int p0 = wn * WT + x0;               // first position within the tile
+            float x[XT / 8][4];
+#pragma unroll
+            for (int i = 0; i < XT / 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < D / 16; ++kb)
+#pragma unroll
+              for (int i = 0; i < XT / 8; i += 2) {
+                uint32_t b[4];
+                mm::ldsm4(b, k_base + tile_at<BN>(p0 + i * 8 + (lane >> 4) * 8 + (lane & 7),
+                                                  kb * 2 + ((lane >> 3) & 1)));
+                mm::mma16816(x[i], qa[kb], b[0], b[1]);
+                mm::mma16816(x[i + 1], qa[kb], b[2], b[3]);
+              }
+            if (edge) {
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int i = 0; i < XT / 8; ++i)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const int j = p_tile + p0 + i * 8 + 2 * tq + e - s.ctx;
+                    const bool seen = j < 0 || (j < s.n && (anc[hh] >> (j & 63) & 1));
+                    if (!seen) x[i][hh * 2 + e] = -INFINITY;
+                  }
+            }
+            // running maximum and sum; scaled to base 2 (scale > 0) within the exponent's argument
+            uint32_t pa[XT / 16][4];
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              float m = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < XT / 8; ++i) m = fmaxf(m, fmaxf(x[i][hh * 2], x[i][hh * 2 + 1]));
+              m *= a.scale_log2;
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+              m = fmaxf(m, mx[hh]);
+              const float off = m == -INFINITY ? 0.f : m;    // a row that has seen nothing yet
+              const float corr = ex2(mx[hh] - off);
+              float add = 0.f;
+#pragma unroll
+              for (int i = 0; i < XT / 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float& v = x[i][hh * 2 + e];
+                  v = ex2(fmaf(v, a.scale_log2, -off));
+                  add += v;
+                }
+              sum[hh] = sum[hh] * corr + add;
+              if (__any_sync(0xffffffffu, m != mx[hh])) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                  o[i][hh * 2] *= corr;
+                  o[i][hh * 2 + 1] *= corr;
+                }
+              }
+              mx[hh] = m;
+            }
+#pragma unroll
+            for (int i = 0; i < XT / 16; ++i) {
+              pa[i][0] = mm::pack2(x[2 * i][0], x[2 * i][1]);
+              pa[i][1] = mm::pack2(x[2 * i][2], x[2 * i][3]);
+              pa[i][2] = mm::pack2(x[2 * i + 1][0], x[2 * i + 1][1]);
+              pa[i][3] = mm::pack2(x[2 * i + 1][2], x[2 * i + 1][3]);
+            }
+#pragma unroll
+            for (int i = 0; i < XT / 16; ++i)
+#pragma unroll
+              for (int c = 0; c < D / 8; c += 2) {
+                uint32_t b[4];
+                mm::ldsm4t(b, v_base + tile_at<BN>(p0 + i * 16 + (lane & 15), c + (lane >> 4)));
+                mm::mma16816(o[c], pa[i], b[0], b[1]);
+                mm::mma16816(o[c + 1], pa[i], b[2], b[3]);
+              }
+          }
+        }
+        if (edge) tc::fence_async_smem();            // our writes before the next copy's
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.empty[stage]));
       }
-      const int node = row / G;
-      if (sm.anc[node] & sm.bad) acc.x = acc.y = acc.z = acc.w = __int_as_float(0x7fffffff);
-      const int64_t at = (start + node) * a.HQ + kvh * G + row - node * G;
-      if (a.chunks == 1) {
-        const float inv = 1.f / l;
-        uint2 u;
-        u.x = mm::pack2(acc.x * inv, acc.y * inv);
-        u.y = mm::pack2(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(a.out + at * D + c) = u;
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        sum[hh] += __shfl_xor_sync(0xffffffffu, sum[hh], 1);
+        sum[hh] += __shfl_xor_sync(0xffffffffu, sum[hh], 2);
+      }
+      const bool whole = tile0 == 0 && seg == s.tiles;
+      const int64_t part = ((int64_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * BM;
+      const unsigned long long bad = masks ? *reinterpret_cast<volatile unsigned long long*>(&sm.bad) : 0;
+
+      if constexpr (WN == 1) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          if (my_row[hh] >= rows) continue;
+          const bool nan = (anc[hh] & bad) != 0;
+          const float inv = whole ? 1.f / sum[hh] : 1.f;
+          const int r = wm * 16 + gr + hh * 8;
+          const int64_t at = (s.start + node[hh]) * a.HQ + kvh * a.G + my_row[hh] - node[hh] * a.G;
+          if (!whole && tq == 0) a.part_ml[part + r] = make_float2(mx[hh], sum[hh]);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            float u = o[i][hh * 2] * inv, v = o[i][hh * 2 + 1] * inv;
+            if (nan) u = v = __int_as_float(0x7fffffff);
+            if (whole)
+              *reinterpret_cast<uint32_t*>(a.out + at * D + i * 8 + 2 * tq) = mm::pack2(u, v);
+            else
+              *reinterpret_cast<float2*>(a.part_o + (part + r) * D + i * 8 + 2 * tq) = make_float2(u, v);
+          }
+        }
+        if (masks) sync();                           // the masks are used up
       } else {
-        const int64_t pr = chunk * (a.n_tokens * a.HQ) + at;
-        *reinterpret_cast<float4*>(a.part_o + pr * D + c) = acc;
-        if (c == 0) a.part_ml[pr] = make_float2(m, l);
+        // join the WN warps of a row tile: common maximum, then 32 columns at a time
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+          if (tq == 0) sm.ml[wn * BM + wm * 16 + gr + hh * 8] = make_float2(mx[hh], sum[hh]);
+        sync();
+        float inv[2];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int r = wm * 16 + gr + hh * 8;
+          float m = -INFINITY, l = 0.f;
+#pragma unroll
+          for (int v = 0; v < WN; ++v) m = fmaxf(m, sm.ml[v * BM + r].x);
+          const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int v = 0; v < WN; ++v) {
+            const float2 p = sm.ml[v * BM + r];
+            l = fmaf(p.y, ex2(p.x - off), l);
+          }
+          inv[hh] = ex2(mx[hh] - off) * (whole ? 1.f / l : 1.f);
+          if (anc[hh] & bad) inv[hh] = __int_as_float(0x7fffffff);
+          if (!whole && wn == 0 && tq == 0 && my_row[hh] < rows) a.part_ml[part + r] = make_float2(m, l);
+        }
+#pragma unroll
+        for (int cq = 0; cq < D / 32; ++cq) {
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<float2*>(
+                  &sm.join[(wn * BM + wm * 16 + gr + hh * 8) * 36 + i * 8 + 2 * tq]) =
+                  make_float2(o[cq * 4 + i][hh * 2] * inv[hh], o[cq * 4 + i][hh * 2 + 1] * inv[hh]);
+          sync();
+          for (int i = tid; i < BM * 8; i += NC * 32) {
+            const int r = i >> 3, c = (i & 7) * 4, row = row0 + r;
+            if (row < rows) {
+              float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int v = 0; v < WN; ++v) {
+                const float4 u = *reinterpret_cast<const float4*>(&sm.join[(v * BM + r) * 36 + c]);
+                acc.x += u.x;
+                acc.y += u.y;
+                acc.z += u.z;
+                acc.w += u.w;
+              }
+              if (whole) {
+                const int nd = row / a.G;
+                const int64_t at = (s.start + nd) * a.HQ + kvh * a.G + row - nd * a.G;
+                *reinterpret_cast<uint2*>(a.out + at * D + cq * 32 + c) =
+                    make_uint2(mm::pack2(acc.x, acc.y), mm::pack2(acc.z, acc.w));
+              } else {
+                *reinterpret_cast<float4*>(a.part_o + (part + r) * D + cq * 32 + c) = acc;
+              }
+            }
+          }
+          sync();
+        }
       }
     }
-  } else {
+    it += seg;
+    w += seg;
+  }
+}
+
+// Joins the parts of a unit that was cut: a CTA per (sequence, kv-head, row tile) and
+// four of its rows.  Few parts: a warp per row; many (a long sequence nearly alone): the
+// warps share a row's parts.
+template <int D, int WM, int WN>
+__global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, int max_row_tiles,
+                                                             int grid) {
+  using P = Attn<D, WM, WN>;
+  constexpr int BM = P::BM, BN = P::BN, CPL = D / 32;   // columns per lane
+  __shared__ float s_o[4][D];
+  __shared__ float2 s_ml[4];
+  const int per_seq = a.HKV * max_row_tiles;
+  const int seq = blockIdx.x / per_seq, u = blockIdx.x - seq * per_seq;
+  const int64_t base = a.prefix[seq], total = a.prefix[a.n_seqs];
+  const AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
+  if (s.n == 0 || u >= a.HKV * s.row_tiles) return;
+  const int64_t ctas = min((int64_t)grid, total);
+  const int64_t u0 = base + (int64_t)u * s.tiles, u1 = u0 + s.tiles;
+  // the CTA that holds tile w: the last b with total * b / ctas <= w
+  const int b0 = (int)(((u0 + 1) * ctas - 1) / total), b1 = (int)((u1 * ctas - 1) / total);
+  if (b0 == b1) return;
+  const int kvh = u / s.row_tiles, rt = u - kvh * s.row_tiles;
+  const int row0 = rt * BM, rows = min(BM, s.n * a.G - row0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the unit is the second part of the CTA it begins in the middle of, the first of all others
+  const int64_t part0 = (int64_t)b0 * 2 + (total * b0 / ctas >= u0 ? 0 : 1);
+  const int parts = b1 - b0 + 1;
+  const auto part = [&](int i) { return (i == 0 ? part0 : (int64_t)(b0 + i) * 2) * BM; };
+  const auto join = [&](int r, int from, int step, float& m, float& l, float(&acc)[CPL]) {
+    m = -INFINITY;
+    for (int i = from; i < parts; i += step) m = fmaxf(m, a.part_ml[part(i) + r].x);
+    const float off = m == -INFINITY ? 0.f : m;
+    l = 0.f;
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int row = my_row[hh];
-      if (row >= rows) continue;
-      const int node = row / G;
-      const int64_t at = (start + node) * a.HQ + kvh * G + row - node * G;
-      const bool nan = (sm.anc[node] & sm.bad) != 0;
-      const int64_t pr = chunk * (a.n_tokens * a.HQ) + at;
-      const float inv = a.chunks == 1 ? 1.f / sum[hh] : 1.f;
-      if (a.chunks > 1 && tq == 0) a.part_ml[pr] = make_float2(mx[hh], sum[hh]);
+    for (int e = 0; e < CPL; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int i = from; i < parts; i += step) {
+      const float2 p = a.part_ml[part(i) + r];
+      const float* src = a.part_o + (part(i) + r) * D + lane;
+      const float f = ex2(p.x - off);
+      l = fmaf(p.y, f, l);
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        float x = o[i][hh * 2] * inv, y = o[i][hh * 2 + 1] * inv;
-        if (nan) x = y = __int_as_float(0x7fffffff);
-        if (a.chunks == 1)
-          *reinterpret_cast<uint32_t*>(a.out + at * D + i * 8 + 2 * tq) = mm::pack2(x, y);
-        else
-          *reinterpret_cast<float2*>(a.part_o + pr * D + i * 8 + 2 * tq) = make_float2(x, y);
+      for (int e = 0; e < CPL; ++e) acc[e] = fmaf(src[32 * e], f, acc[e]);
+    }
+  };
+  const auto store = [&](int r, float l, const float(&acc)[CPL]) {
+    const float inv = 1.f / l;
+    const int nd = (row0 + r) / a.G;
+    bf16* dst = a.out + ((s.start + nd) * a.HQ + kvh * a.G + row0 + r - nd * a.G) * D + lane;
+#pragma unroll
+    for (int e = 0; e < CPL; ++e) dst[32 * e] = f2bf(acc[e] * inv);
+  };
+  float m, l, acc[CPL];
+  const int r0 = blockIdx.y * 4;
+  if (parts < 16) {
+    if (r0 + warp < rows) {
+      join(r0 + warp, 0, 1, m, l, acc);
+      store(r0 + warp, l, acc);
+    }
+    return;
+  }
+  for (int r = r0; r < min(r0 + 4, rows); ++r) {
+    join(r, warp, 4, m, l, acc);
+    __syncthreads();                                   // the last row's sums are used up
+#pragma unroll
+    for (int e = 0; e < CPL; ++e) s_o[warp][lane + 32 * e] = acc[e];
+    if (lane == 0) s_ml[warp] = make_float2(m, l);
+    __syncthreads();
+    if (warp == 0) {
+      m = fmaxf(fmaxf(s_ml[0].x, s_ml[1].x), fmaxf(s_ml[2].x, s_ml[3].x));
+      const float off = m == -INFINITY ? 0.f : m;
+      l = 0.f;
+#pragma unroll
+      for (int e = 0; e < CPL; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float f = ex2(s_ml[v].x - off);
+        l = fmaf(s_ml[v].y, f, l);
+#pragma unroll
+        for (int e = 0; e < CPL; ++e) acc[e] = fmaf(s_o[v][lane + 32 * e], f, acc[e]);
       }
+      store(r, l, acc);
     }
   }
 }
 
-// Joins a row's chunks: D / 4 lanes per (node, query head).
-template <int D>
-__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a) {
-  constexpr int LPR = D / 4;
-  const int seq = blockIdx.y;
-  int64_t start, ctx;
-  int n;
-  if (!tree_rows(a.cu, seq, a.n_tokens, a.max_nodes, nullptr, start, n)) return;
-  const int item = (int)(blockIdx.x * 256 + threadIdx.x);
-  const int r = item / LPR, c = (item - r * LPR) * 4;
-  if (r >= n * a.HQ) return;
-  ctx = a.ctx[seq];
-  if (ctx < 0 || ctx + n > a.max_len) return;
-  const int chunks = (int)((ctx + n + a.chunk - 1) / a.chunk);
-  const int64_t at = start * a.HQ + r, step = a.n_tokens * a.HQ;
-  float m = -INFINITY;
-  for (int i = 0; i < chunks; ++i) m = fmaxf(m, a.part_ml[i * step + at].x);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < chunks; ++i) {
-    const float2 p = a.part_ml[i * step + at];
-    const float f = exp2f(p.x - base);
-    const float4 t = *reinterpret_cast<const float4*>(a.part_o + (i * step + at) * D + c);
-    l = fmaf(p.y, f, l);
-    acc.x = fmaf(t.x, f, acc.x);
-    acc.y = fmaf(t.y, f, acc.y);
-    acc.z = fmaf(t.z, f, acc.z);
-    acc.w = fmaf(t.w, f, acc.w);
-  }
-  const float inv = 1.f / l;
-  uint2 u;
-  u.x = mm::pack2(acc.x * inv, acc.y * inv);
-  u.y = mm::pack2(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(a.out + at * D + c) = u;
+// Rows per CTA tile (16 wm) by the rows of the largest tree, and how many CTAs run.
+// (128 rows of head dim 256 would not fit the registers.)
+static int attn_wm(int max_nodes, int G, int D) {
+  const int rows = max_nodes * G;
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 || D == 256 ? 4 : 8;
 }
+static int attn_ctas(int wm, int D) { return kAttnSms * (D <= 128 && wm <= 4 ? 2 : 1); }
 
-// How a call is cut: rows per CTA, and positions per chunk.
-struct AttnPlan {
-  int wm, row_tiles, chunk, chunks;
+struct AttnSpace {
+  int64_t prefix, part_o, part_ml, bytes;
 };
-
-static AttnPlan attn_plan(int n_seqs, int HQ, int HKV, int D, int max_nodes, int max_len) {
-  AttnPlan p;
-  const int rows = max_nodes * (HQ / HKV);
-  p.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  p.row_tiles = (rows + 16 * p.wm - 1) / (16 * p.wm);
-  const int64_t units = (int64_t)n_seqs * HKV * p.row_tiles;
-  const int64_t want = 148 * 24;                      // CTAs, for an even finish
-  int64_t chunk = (units * max_len + want - 1) / want;
-  chunk = (chunk + 63) / 64 * 64;
-  if (chunk < 256) chunk = 256;
-  if (chunk > 4096) chunk = 4096;
-  p.chunk = (int)chunk;
-  p.chunks = (max_len + p.chunk - 1) / p.chunk;
-  if (p.chunks < 1) p.chunks = 1;
-  return p;
+static AttnSpace attn_space(int wm, int n_seqs, int D) {
+  const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+  const int64_t rows = (int64_t)attn_ctas(wm, D) * 2 * 16 * wm;
+  AttnSpace s;
+  s.prefix = 0;
+  s.part_o = up((n_seqs + 1ll) * 8);
+  s.part_ml = s.part_o + rows * D * 4;
+  s.bytes = s.part_ml + rows * 8;
+  return s;
 }
 
-static int64_t attn_workspace(const AttnPlan& p, int64_t n_tokens, int HQ, int D) {
-  return p.chunks == 1 ? 0 : p.chunks * n_tokens * HQ * (4ll * D + 8);
-}
-
-template <int D, int WM, int WN, int BN>
-static int launch_attention(const AttnArgs& a, cudaStream_t s) {
-  const int pages = a.chunk / a.block_size + 2;
-  const size_t bytes = sizeof(AttnSmem<D, WM, WN, BN>) + pages * sizeof(int);
-  auto fn = attention_tree_kernel<D, WM, WN, BN>;
+template <int D, int WM, int WN>
+static int launch_attention(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttnArgs& a,
+                            cudaStream_t s) {
+  using P = Attn<D, WM, WN>;
+  constexpr size_t bytes = sizeof(typename P::Smem) + 1024;
+  static_assert(bytes * P::CTAS + 1024 * P::CTAS <= 228 * 1024, "shared memory of one SM");
+  auto fn = attention_tree_kernel<D, WM, WN>;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
       cudaSuccess)
     return check_launch("gdn_attention_tree");
-  const dim3 grid((unsigned)(a.n_seqs * a.HKV * a.row_tiles), (unsigned)a.chunks);
-  fn<<<grid, 32 * WM * WN, bytes, s>>>(a);
-  if (a.chunks > 1) {
-    const int items = a.max_nodes * a.HQ * (D / 4);
-    attention_join_kernel<D><<<dim3((items + 255) / 256, a.n_seqs), 256, 0, s>>>(a);
-  }
+  const int ctas = attn_ctas(WM, D);
+  fn<<<ctas, 32 * (P::NC + 1), bytes, s>>>(kmap, vmap, a);
+  const int row_tiles = (a.max_nodes * a.G + P::BM - 1) / P::BM;
+  const int rows = row_tiles > 1 ? P::BM : a.max_nodes * a.G;
+  attention_join_kernel<D, WM, WN>
+      <<<dim3((unsigned)(a.n_seqs * a.HKV * row_tiles), (unsigned)((rows + 3) / 4)), 128, 0, s>>>(
+          a, row_tiles, ctas);
   return check_launch("gdn_attention_tree");
 }
 
@@ -465,15 +652,13 @@ static int launch_attention(const AttnArgs& a, cudaStream_t s) {
 
 using namespace gdn;
 
-extern "C" int64_t gdn_attention_tree_workspace_bytes(int64_t n_tokens, int32_t n_seqs,
-                                                      int32_t num_q_heads, int32_t num_kv_heads,
-                                                      int32_t head_dim, int32_t max_nodes,
-                                                      int32_t max_len) {
-  if (n_tokens <= 0 || n_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
-      max_nodes <= 0 || max_len <= 0)
+extern "C" int64_t gdn_attention_tree_workspace_bytes(int32_t n_seqs, int32_t num_q_heads,
+                                                      int32_t num_kv_heads, int32_t head_dim,
+                                                      int32_t max_nodes) {
+  if (n_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_nodes <= 0)
     return 0;
-  return attn_workspace(attn_plan(n_seqs, num_q_heads, num_kv_heads, head_dim, max_nodes, max_len),
-                        n_tokens, num_q_heads, head_dim);
+  return attn_space(attn_wm(max_nodes, num_q_heads / num_kv_heads, head_dim), n_seqs,
+                    head_dim).bytes;
 }
 
 extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const void* k_cache,
@@ -507,34 +692,60 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
               "%s: cache strides smaller than a head", fn);
   if (n_seqs == 0 || n_tokens == 0 || max_nodes == 0) return GDN_OK;
   GDN_REQUIRE(max_len >= 1, "%s: max_len %d leaves no room for a node", fn, max_len);
+  GDN_REQUIRE(scale > 0.f && scale < 1e30f, "%s: the scale must be positive", fn);
   GDN_REQUIRE(q && k_cache && v_cache && block_tables && context_lens && cu_seqlens && parents && out,
               "%s: null pointer", fn);
+  GDN_REQUIRE(num_blocks > 0 && max_blocks > 0, "%s: no pages", fn);
   GDN_UNSUPPORTED(((q_row_stride | block_stride | token_stride | head_stride) & 7) == 0 &&
                       aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
                   "%s: operands and strides must be 16-byte aligned", fn);
-  GDN_UNSUPPORTED(max_len <= (1 << 30), "%s: max_len %d too large", fn, max_len);
-  const AttnPlan p = attn_plan(n_seqs, num_q_heads, num_kv_heads, head_dim, max_nodes, max_len);
-  const int64_t need = attn_workspace(p, n_tokens, num_q_heads, head_dim);
-  GDN_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned16(workspace)),
-              "%s: workspace of %lld bytes needed (16-byte aligned), got %lld", fn, (long long)need,
-              (long long)workspace_bytes);
-  GDN_UNSUPPORTED((int64_t)n_seqs * num_kv_heads * p.row_tiles < (1ll << 31) && p.chunks <= 65535 &&
-                      n_seqs <= 65535,
-                  "%s: too many sequences, heads or chunks", fn);
-  AttnArgs a{(const bf16*)q, q_row_stride, (const bf16*)k_cache, (const bf16*)v_cache,
-             block_stride, token_stride, head_stride, num_blocks, block_size, block_tables,
-             table_stride, max_blocks, context_lens, cu_seqlens, n_seqs, parents, max_nodes,
-             n_tokens, max_len, (bf16*)out, num_q_heads, num_kv_heads,
-             scale * 1.4426950408889634f, p.chunk, p.chunks, p.row_tiles, (float*)workspace,
-             nullptr, status};
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + p.chunks * n_tokens * num_q_heads * head_dim);
+  const int G = num_q_heads / num_kv_heads, wm = attn_wm(max_nodes, G, head_dim);
+  // the scan adds up 32-bit tile counts of up to 288 sequences; TMA coordinates are 32 bits
+  const int row_tiles = (max_nodes * G + 16 * wm - 1) / (16 * wm);
+  GDN_UNSUPPORTED((max_len / 64 + 1ll) * num_kv_heads * row_tiles <= (1ll << 22) &&
+                      num_blocks < (1ll << 31) && max_len <= (1 << 30),
+                  "%s: max_len %d with %d kv heads too large", fn, max_len, num_kv_heads);
+  GDN_UNSUPPORTED((int64_t)n_seqs * num_kv_heads * row_tiles < (1ll << 31),
+                  "%s: too many sequences or heads", fn);
+  const AttnSpace sp = attn_space(wm, n_seqs, head_dim);
+  GDN_REQUIRE(workspace != nullptr && workspace_bytes >= sp.bytes && aligned16(workspace),
+              "%s: workspace of %lld bytes needed (16-byte aligned), got %lld", fn,
+              (long long)sp.bytes, (long long)workspace_bytes);
+  int box = 64;                                    // positions per TMA box: divides a page
+  while (block_size % box) box /= 2;
+  const EncodeTiledFn encode = encode_tiled();
+  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)num_kv_heads, (cuuint64_t)block_size,
+                              (cuuint64_t)num_blocks};
+  const cuuint64_t strides[3] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2,
+                                 (cuuint64_t)block_stride * 2};
+  const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, step[4] = {1, 1, 1, 1};
+  CUtensorMap kmap, vmap;
+  const auto make = [&](CUtensorMap* m, const void* p) {
+    return encode != nullptr &&
+           encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, boxes,
+                  step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (!make(&kmap, k_cache) || !make(&vmap, v_cache)) {
+    set_error("%s: the caches' tensor maps could not be encoded", fn);
+    return GDN_ERR_CUDA;
+  }
+  char* ws = static_cast<char*>(workspace);
+  const AttnArgs a{(const bf16*)q, q_row_stride, num_blocks, block_size, box, block_tables,
+                   table_stride, max_blocks, context_lens, cu_seqlens, n_seqs, parents, max_nodes,
+                   n_tokens, max_len, (bf16*)out, num_q_heads, num_kv_heads, G,
+                   scale * 1.4426950408889634f, reinterpret_cast<int64_t*>(ws + sp.prefix),
+                   reinterpret_cast<float*>(ws + sp.part_o),
+                   reinterpret_cast<float2*>(ws + sp.part_ml), status};
   cudaStream_t s = (cudaStream_t)stream;
-#define GDN_AT(D, BN)                                                   \
-  if (p.wm == 1) return launch_attention<D, 1, 4, BN < 64 ? 64 : BN>(a, s); \
-  if (p.wm == 2) return launch_attention<D, 2, 2, BN>(a, s);            \
-  return launch_attention<D, 4, 1, BN>(a, s)
-  if (head_dim == 64) { GDN_AT(64, 64); }
-  if (head_dim == 128) { GDN_AT(128, 64); }
-  GDN_AT(256, 32);
+#define GDN_AT(D)                                                   \
+  if (wm == 1) return launch_attention<D, 1, 4>(kmap, vmap, a, s);  \
+  if (wm == 2) return launch_attention<D, 2, 2>(kmap, vmap, a, s);  \
+  if (wm == 4) return launch_attention<D, 4, 1>(kmap, vmap, a, s);
+  if (head_dim == 64) { GDN_AT(64) }
+  if (head_dim == 128) { GDN_AT(128) }
+  if (head_dim == 256) { GDN_AT(256) }
 #undef GDN_AT
+  return head_dim == 64 ? launch_attention<64, 8, 1>(kmap, vmap, a, s)
+                        : launch_attention<128, 8, 1>(kmap, vmap, a, s);
 }

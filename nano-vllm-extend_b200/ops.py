@@ -1025,7 +1025,7 @@ def attention_tree(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, 
         q, qs = q.clone(memory_format=torch.contiguous_format), HQ * D
     out = _out_buffer(out, (N, HQ, D), dev)
     max_len = int(max_len)
-    need = _lib.load().gdn_attention_tree_workspace_bytes(N, n_seqs, HQ, HKV, D, tree[2], max_len)
+    need = _lib.load().gdn_attention_tree_workspace_bytes(n_seqs, HQ, HKV, D, tree[2])
     # made per call: calls on several streams, or graphs that hold one each, never share it
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _launch("gdn_attention_tree", dev, q.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(), bs,

@@ -96,7 +96,11 @@ REFUSED = [
     ("gdn_attention_tree", attn_args, dict(D=80), UNSUPPORTED, "head dim"),
     ("gdn_attention_tree", attn_args, dict(HKV=3), INVALID, "multiple"),
     ("gdn_attention_tree", attn_args, dict(max_len=0), INVALID, "max_len"),
-    ("gdn_attention_tree", attn_args, dict(max_len=100000), INVALID, "workspace"),
+    ("gdn_attention_tree", attn_args, dict(), INVALID, "workspace"),
+    ("gdn_attention_tree", attn_args, dict(scale=0.0), INVALID, "scale"),
+    ("gdn_attention_tree", attn_args, dict(scale=float("nan")), INVALID, "scale"),
+    ("gdn_attention_tree", attn_args, dict(max_len=1 << 29), UNSUPPORTED, "max_len"),
+    ("gdn_attention_tree", attn_args, dict(blocks=0), INVALID, "pages"),
     ("gdn_attention_tree", attn_args, dict(hs=60), INVALID, "strides"),
     ("gdn_attention_tree", attn_args, dict(kc=FAKE + 2), UNSUPPORTED, "aligned"),
     ("gdn_attention_tree", attn_args, dict(table=None), INVALID, "null"),
@@ -124,11 +128,13 @@ def test_empty_calls_are_noops(pkg, name, make, change):
 
 
 def test_attention_workspace(pkg):
+    """Two parts per CTA (148 SMs x 2, or x 1 for wide trees and head dim 256) of a row tile's fp32
+    rows with maximum and sum, after the padded int64 tile counts."""
     f = pkg._lib.load().gdn_attention_tree_workspace_bytes
-    assert f(128, 128, 16, 4, 128, 1, 200) == 0           # short: one chunk
-    assert f(0, 4, 16, 4, 128, 1, 5000) == 0
-    need = f(8, 8, 16, 4, 128, 1, 131073)
-    assert need > 0 and need % (8 * 16 * (4 * 128 + 8)) == 0
+    assert f(0, 16, 4, 128, 1) == 0 and f(4, 16, 4, 128, 0) == 0
+    assert f(8, 16, 4, 128, 1) == 256 + 296 * 2 * 16 * (4 * 128 + 8)
+    assert f(31, 16, 4, 128, 17) == 256 + 148 * 2 * 128 * (4 * 128 + 8)
+    assert f(32, 8, 4, 256, 16) == 512 + 148 * 2 * 32 * (4 * 256 + 8)
 
 
 def test_cpu_tensors_are_refused(pkg):
