@@ -229,7 +229,7 @@ class DecodeStack:
 
 C3 = dict(layers=24, attn_every=4, hidden=2048, HK=16, DK=128, HV=32, DV=128, K=4, q_heads=16,
           kv_heads=4, head_dim=128, inter=6144, vocab=151936, bs=128, ctx_lo=256, ctx_hi=4096,
-          gen=256, slots=256, eps=1e-6)
+          gen=256, slots=256, eps=1e-6, block=256)
 
 
 def _add_rms(h, r, w, eps):
@@ -249,11 +249,11 @@ class HybridStage:
     fused residual chain (hidden, residual) between layers; the first stage
     embeds the tokens (vocab 151,936), the last applies the final norm and the
     LM head and takes the greedy token.  Attention is GQA 16 q / 4 kv heads x
-    128 through torch SDPA over a contiguous KV cache whose length is the mean
-    config-3 context (prompts U[256, 4096] plus half of 256 generated tokens:
-    2304): the attention layers' weights and KV bytes are config 3's, but the
-    KV cache is not paged.  Weights random (seeded); the whole stage step is
-    one CUDA graph."""
+    128 with per-head query / key norms and a quarter of each head rotated
+    (ops.qk_norm_rope_cache), over a paged KV cache with blocks of 256 positions
+    (ops.attention_tree) whose length is the mean config-3 context (prompts
+    U[256, 4096] plus half of 256 generated tokens: 2304, the step's own token
+    included).  Weights random (seeded); the whole stage step is one CUDA graph."""
 
     def __init__(self, pkg, dev, seed, lo, hi, first, last):
         c = C3
@@ -269,6 +269,16 @@ class HybridStage:
                                    linear_value_head_dim=c["DV"], linear_conv_kernel_dim=c["K"],
                                    rms_norm_eps=c["eps"]))
         self.ctx_len = (c["ctx_lo"] + c["ctx_hi"]) // 2 + c["gen"] // 2
+        # every sequence's pages, in a seeded order; all but the step's token are filled
+        pages = -(-self.ctx_len // c["block"])
+        order = torch.randperm(bs * pages, generator=torch.Generator().manual_seed(seed + 1))
+        self.tables = order.view(bs, pages).to(dev, torch.int32)
+        self.ctx_lens = torch.full((bs,), self.ctx_len - 1, dtype=torch.int32, device=dev)
+        self.roots = torch.full((bs,), -1, dtype=torch.int32, device=dev)
+        rot = c["head_dim"] // 4
+        freq = 1e6 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+        angle = torch.arange(self.ctx_len, dtype=torch.float64)[:, None] * freq
+        self.cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float().to(dev)
         self.layers = []
         gdn = []
         prev = torch.get_default_dtype()
@@ -283,8 +293,10 @@ class HybridStage:
                     qd, kd = c["q_heads"] * c["head_dim"], c["kv_heads"] * c["head_dim"]
                     L["qkv"] = nrm(qd + 2 * kd, H, std=H ** -0.5)
                     L["o"] = nrm(H, qd, std=qd ** -0.5)
-                    L["k_cache"] = nrm(bs, c["kv_heads"], self.ctx_len, c["head_dim"], std=1.0)
-                    L["v_cache"] = nrm(bs, c["kv_heads"], self.ctx_len, c["head_dim"], std=1.0)
+                    shape = (bs * pages, c["block"], c["kv_heads"], c["head_dim"])
+                    L["k_cache"], L["v_cache"] = nrm(*shape, std=1.0), nrm(*shape, std=1.0)
+                    L["q_norm"] = torch.zeros(c["head_dim"], dtype=torch.bfloat16, device=dev)
+                    L["k_norm"] = torch.zeros(c["head_dim"], dtype=torch.bfloat16, device=dev)
                 else:
                     with torch.device(dev), torch.no_grad():
                         # unsharded: a pipeline stage's layers hold no collective
@@ -317,14 +329,19 @@ class HybridStage:
     def _attn(self, L, h):
         c = C3
         bs, qh, kh, hd = h.shape[0], c["q_heads"], c["kv_heads"], c["head_dim"]
-        qkv = torch.nn.functional.linear(h, L["qkv"])
-        q = qkv[:, :qh * hd].view(bs, qh, 1, hd)
-        o = torch.nn.functional.scaled_dot_product_attention(q, L["k_cache"], L["v_cache"],
-                                                             enable_gqa=True)
-        return torch.nn.functional.linear(o.reshape(bs, qh * hd), L["o"])
+        ops = self.pkg.ops
+        qkv = torch.nn.functional.linear(h, L["qkv"]).view(bs, qh + 2 * kh, hd)
+        q = ops.qk_norm_rope_cache(qkv[:, :qh], qkv[:, qh:qh + kh], qkv[:, qh + kh:], L["q_norm"],
+                                   L["k_norm"], self.cos_sin, self.pos, L["k_cache"], L["v_cache"],
+                                   self.kv_slots, eps=c["eps"], unit_offset=True)
+        o = ops.attention_tree(q, L["k_cache"], L["v_cache"], self.tables, self.ctx_lens, self.cu,
+                               self.roots, 1, self.ctx_len)
+        return torch.nn.functional.linear(o.view(bs, qh * hd), L["o"])
 
     def _step(self):
         eps = C3["eps"]
+        self.pos, self.kv_slots = self.pkg.ops.tree_slot_map(
+            self.tables, self.ctx_lens, self.cu, self.roots, 1, C3["block"], C3["bs"])
         if self.first:
             h, r = self.embed[self.tokens], None
         else:
@@ -436,7 +453,7 @@ def pp_bench(pkg, dev, world, rank, steps, warmup):
     exposed = (t_pp - fill - t_local) / t_pp
     per_stage = [b - a for a, b in (P.split_layers(c["layers"], world, r) for r in range(world))]
     out = {"workload": "config3-shaped hybrid decoder, decode steps of 128 sequences: 24 layers "
-                       "(every 4th full attention GQA 16q/4kv x 128 over a 2304-token KV cache, "
+                       "(every 4th full attention GQA 16q/4kv x 128 over 2304 paged tokens, "
                        "the rest GDN), SwiGLU 6144, vocab 151936, bf16; embedding on the first "
                        "stage, final norm + LM head + greedy token on the last",
            "stages": world, "layers_per_stage": per_stage,

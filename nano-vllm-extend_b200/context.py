@@ -34,6 +34,16 @@ class Context:
     vision_embeds: tuple = ()
 
 
+@dataclass(slots=True)
+class DraftContext(Context):
+    """A step whose rows are drafted trees (not in the reference): sequence r owns the
+    rows of cu_seqlens_q, at most max_seqlen_q of them, ``draft_parents`` (int32 [rows]
+    on the device) holds each row's parent within its sequence, -1 for a row that
+    follows the stored context.  The layers leave their slots' state as it is until the
+    accepted paths are committed (layer.commit_drafts)."""
+    draft_parents: torch.Tensor | None = None
+
+
 _CONTEXT = Context()
 
 
@@ -52,6 +62,13 @@ def set_context(cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0, max_seqlen
                        flashinfer_decode, flashinfer_prefill,
                        draft_slot_mapping, draft_block_tables,
                        linear_state_ids, lens_q, vision_embeds)
+
+
+def set_draft_context(cu_seqlens, draft_parents, max_nodes, linear_state_ids):
+    """Make the step one of drafted trees (:class:`DraftContext`)."""
+    global _CONTEXT
+    _CONTEXT = DraftContext(cu_seqlens, cu_seqlens, max_nodes, max_nodes,
+                            linear_state_ids=linear_state_ids, draft_parents=draft_parents)
 
 
 def reset_context():

@@ -19,6 +19,10 @@ What differs is the execution, B200-first:
   rows to the varlen conv + chunked-prefill kernels driven by cu_seqlens;
 * no gather / scatter of pool rows: every kernel reads and writes the state
   in its slot;
+* drafted tokens (``context.DraftContext``) are computed as trees from the slots'
+  states, which stay as they are; :meth:`Qwen3_5GatedDeltaNet.commit_drafts` takes the
+  accepted path over (the reference excludes this model from speculative
+  decoding: a rejected token cannot be taken out of a recurrent state);
 * no host synchronisation on the decode path, so the engine's CUDA-graph
   capture of decode steps works as before (pad rows use the dummy slot).
 """
@@ -127,6 +131,7 @@ class Qwen3_5GatedDeltaNet(nn.Module):
                                           self.hidden_size, tp_rank, tp_size, P.get_tp_group())
         self.s_cache: torch.Tensor | None = None      # [slots, HV, DK, DV] fp32 view
         self.conv_cache: torch.Tensor | None = None   # [slots, conv_dim, K-1] view
+        self._drafted = None                          # what commit_drafts() needs of the last forward
 
     # -- weight loading -----------------------------------------------------
 
@@ -182,6 +187,14 @@ class Qwen3_5GatedDeltaNet(nn.Module):
         a = proj[:, r[2]:r[3]]
 
         T = int(ctx.max_seqlen_q)
+        self._drafted = None
+        parents = getattr(ctx, "draft_parents", None)
+        if parents is not None:
+            core = torch.empty(N, hv, self.head_v_dim, dtype=torch.bfloat16,
+                               device=hidden_states.device)
+            with self._range("gdn.draft_core"):
+                self._draft_core(mixed, z, b, a, ids, (ctx.cu_seqlens_q, parents, T), out=core)
+            return self._finish(core)
         if T == 1:
             n1 = N
             lens_q = None
@@ -203,10 +216,13 @@ class Qwen3_5GatedDeltaNet(nn.Module):
             cu_p = cu_q[n1:] - cu_q[n1] if n1 else cu_q
             self._prefill_core(mixed[n1:], b[n1:], a[n1:], ids[n1:], cu_p, max(lens_q[n1:]),
                                z[n1:], out=core[n1:])
-        if self.report_status and ops.is_status_publisher(self, hidden_states.device):
-            ops.publish_status(hidden_states.device)
+        return self._finish(core)
+
+    def _finish(self, core: torch.Tensor) -> torch.Tensor:
+        if self.report_status and ops.is_status_publisher(self, core.device):
+            ops.publish_status(core.device)
         with self._range("gdn.out_proj"):
-            return self.out_proj(core.view(N, vd))
+            return self.out_proj(core.view(core.shape[0], self.value_dim))
 
     def _split(self, y: torch.Tensor):
         kd = self.key_dim
@@ -252,6 +268,35 @@ class Qwen3_5GatedDeltaNet(nn.Module):
             return ops.chunk_gated_delta_rule_varlen(
                 q, k, v, g, beta, self.s_cache, ids, cu_seqlens, max_seqlen, z=z,
                 norm_weight=self.norm.weight, eps=self.norm.eps, out=out)
+
+    def _draft_core(self, mixed, z, b, a, ids, tree, out):
+        """Rows of drafted trees: conv and gate along each row's ancestors, then the
+        delta rule with the gated norm; the slots are only read."""
+        y, g, beta = ops.conv_gate_tree(
+            mixed, self.conv_cache, ids, self.conv1d.weight.view(self.conv_dim, self.conv_kernel),
+            *tree, b, a, self.A_log[self._v_head_slice], self.dt_bias[self._v_head_slice])
+        q, k, v = self._split(y)
+        ops.gated_delta_rule_tree(q, k, v, g, beta, self.s_cache, ids, *tree, z=z,
+                                  norm_weight=self.norm.weight, eps=self.norm.eps, out=out)
+        self._drafted = (mixed, k, v, g, beta, ids, tree)
+
+    def commit_drafts(self, accepted: torch.Tensor) -> None:
+        """Take the accepted paths of the last forward's trees into this layer's slots:
+        ``accepted[r]`` (integers [n_seqs] on the device) is sequence r's last accepted
+        node, -1 for none.  Once per forward: the rows it needs are let go."""
+        if self._drafted is None:
+            raise RuntimeError("no drafted rows: commit_drafts() follows a forward with "
+                               "draft_parents in the context, once")
+        mixed, k, v, g, beta, ids, tree = self._drafted
+        self._drafted = None
+        ops.commit_tree(mixed, k, v, g, beta, self.conv_cache, self.s_cache, ids, *tree, accepted)
+
+
+def commit_drafts(model: torch.nn.Module, accepted: torch.Tensor) -> None:
+    """:meth:`Qwen3_5GatedDeltaNet.commit_drafts` of every such layer of a model."""
+    for m in model.modules():
+        if isinstance(m, Qwen3_5GatedDeltaNet):
+            m.commit_drafts(accepted)
 
 
 def install(qwen3_5_module=None, parallel_module=None, context_module=None):
