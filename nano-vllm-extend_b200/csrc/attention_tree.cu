@@ -522,14 +522,15 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
 }
 
 // Joins the parts of a unit that was cut: a CTA per (sequence, kv-head, row tile) and
-// four of its rows.  Few parts: a warp per row; many (a long sequence nearly alone): the
-// warps share a row's parts.
-template <int D, int WM, int WN>
+// four of its rows, a warp each; or, SHARE, where there are fewer units than CTAs and
+// hence many parts to each, a CTA per row whose warps share its parts.  (Launched early,
+// to wait on the device for the first kernel's end, the two took 2 us longer.)
+template <int D, int WM, int WN, bool SHARE>
 __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, int max_row_tiles,
                                                              int grid) {
   using P = Attn<D, WM, WN>;
   constexpr int BM = P::BM, BN = P::BN, CPL = D / 32;   // columns per lane
-  __shared__ float s_o[4][D];
+  __shared__ float s_o[SHARE ? 4 : 1][SHARE ? D : 1];
   __shared__ float2 s_ml[4];
   const int per_seq = a.HKV * max_row_tiles;
   const int seq = blockIdx.x / per_seq, u = blockIdx.x - seq * per_seq;
@@ -549,20 +550,31 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
   const int parts = b1 - b0 + 1;
   const auto part = [&](int i) { return (i == 0 ? part0 : (int64_t)(b0 + i) * 2) * BM; };
   const auto join = [&](int r, int from, int step, float& m, float& l, float(&acc)[CPL]) {
+    // 32 parts' statistics at a time, a lane each
     m = -INFINITY;
-    for (int i = from; i < parts; i += step) m = fmaxf(m, a.part_ml[part(i) + r].x);
-    const float off = m == -INFINITY ? 0.f : m;
     l = 0.f;
 #pragma unroll
     for (int e = 0; e < CPL; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int i = from; i < parts; i += step) {
-      const float2 p = a.part_ml[part(i) + r];
-      const float* src = a.part_o + (part(i) + r) * D + lane;
-      const float f = ex2(p.x - off);
-      l = fmaf(p.y, f, l);
+    for (int i0 = from; i0 < parts; i0 += 32 * step) {
+      const int mine = i0 + lane * step;
+      const float2 p = mine < parts ? a.part_ml[part(mine) + r] : make_float2(-INFINITY, 0.f);
+      float top = p.x;
 #pragma unroll
-      for (int e = 0; e < CPL; ++e) acc[e] = fmaf(src[32 * e], f, acc[e]);
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = fmaxf(top, m);
+      const float off = top == -INFINITY ? 0.f : top, old = ex2(m - off), f = ex2(p.x - off);
+      m = top;
+      l = l * old + warp_sum(p.y * f);
+#pragma unroll
+      for (int e = 0; e < CPL; ++e) acc[e] *= old;
+      const int count = min(32, (parts - i0 + step - 1) / step);
+#pragma unroll 8
+      for (int j = 0; j < count; ++j) {
+        const float* src = a.part_o + (part(i0 + j * step) + r) * D + lane;
+        const float fj = __shfl_sync(0xffffffffu, f, j);
+#pragma unroll
+        for (int e = 0; e < CPL; ++e) acc[e] = fmaf(src[32 * e], fj, acc[e]);
+      }
     }
   };
   const auto store = [&](int r, float l, const float(&acc)[CPL]) {
@@ -573,17 +585,16 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
     for (int e = 0; e < CPL; ++e) dst[32 * e] = f2bf(acc[e] * inv);
   };
   float m, l, acc[CPL];
-  const int r0 = blockIdx.y * 4;
-  if (parts < 16) {
-    if (r0 + warp < rows) {
-      join(r0 + warp, 0, 1, m, l, acc);
-      store(r0 + warp, l, acc);
+  if constexpr (!SHARE) {
+    const int r = blockIdx.y * 4 + warp;
+    if (r < rows) {
+      join(r, 0, 1, m, l, acc);
+      store(r, l, acc);
     }
-    return;
-  }
-  for (int r = r0; r < min(r0 + 4, rows); ++r) {
+  } else {
+    const int r = blockIdx.y;
+    if (r >= rows) return;
     join(r, warp, 4, m, l, acc);
-    __syncthreads();                                   // the last row's sums are used up
 #pragma unroll
     for (int e = 0; e < CPL; ++e) s_o[warp][lane + 32 * e] = acc[e];
     if (lane == 0) s_ml[warp] = make_float2(m, l);
@@ -642,9 +653,10 @@ static int launch_attention(const CUtensorMap& kmap, const CUtensorMap& vmap, co
   fn<<<ctas, 32 * (P::NC + 1), bytes, s>>>(kmap, vmap, a);
   const int row_tiles = (a.max_nodes * a.G + P::BM - 1) / P::BM;
   const int rows = row_tiles > 1 ? P::BM : a.max_nodes * a.G;
-  attention_join_kernel<D, WM, WN>
-      <<<dim3((unsigned)(a.n_seqs * a.HKV * row_tiles), (unsigned)((rows + 3) / 4)), 128, 0, s>>>(
-          a, row_tiles, ctas);
+  const bool share = (int64_t)a.n_seqs * a.HKV * row_tiles * 4 < ctas;
+  const dim3 grid((unsigned)(a.n_seqs * a.HKV * row_tiles), (unsigned)(share ? rows : (rows + 3) / 4));
+  if (share) attention_join_kernel<D, WM, WN, true><<<grid, 128, 0, s>>>(a, row_tiles, ctas);
+  else attention_join_kernel<D, WM, WN, false><<<grid, 128, 0, s>>>(a, row_tiles, ctas);
   return check_launch("gdn_attention_tree");
 }
 
