@@ -85,22 +85,154 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int r, int32_t* s
   return s;
 }
 
+// Shared memory of the scan that finds a CTA's run of tiles.
+struct AttnScan {
+  int64_t base;
+  int warp[9], seq;
+};
+
+// The CTA's run [w0, w1) of all units' tiles, the sequence it begins in and that one's
+// first tile; false: none.  All threads (NW warps) take part; the sequences are scanned
+// in strips of a thread each.  CTA 0 also leaves every sequence's first tile for the
+// joining kernel, and flags malformed sequences.
+template <int BM, int BN, int NW>
+__device__ __forceinline__ bool attn_run(const AttnArgs& a, AttnScan& sc, int64_t& w0, int64_t& w1,
+                                         int& seq, int64_t& seq_base) {
+  constexpr int NT = 32 * NW;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const auto weight = [&](int r, int32_t* status) -> int64_t {
+    if (r >= a.n_seqs) return 0;
+    const AttnSeq s = attn_seq<BM, BN>(a, r, status);
+    return (int64_t)s.tiles * s.row_tiles * a.HKV;
+  };
+  const auto strip_sum = [&](int64_t v) {            // the sum before this thread, and of all
+    int64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    // a strip's tiles fit 31 bits: at most 288 sequences of 2^22 tiles (host check)
+    __syncthreads();
+    if (lane == 31) sc.warp[warp] = (int)inc;
+    __syncthreads();
+    int64_t before = inc - v, all = 0;
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) before += sc.warp[w];
+      all += sc.warp[w];
+    }
+    return make_longlong2(before, all);
+  };
+  int64_t total = 0;
+  const bool scribe = blockIdx.x == 0;
+  longlong2 first{0, 0};
+  for (int s0 = 0; s0 < a.n_seqs; s0 += NT) {
+    const longlong2 st = strip_sum(weight(s0 + tid, scribe ? a.status : nullptr));
+    if (s0 == 0) first = st;
+    if (scribe && s0 + tid < a.n_seqs) a.prefix[s0 + tid] = total + st.x;
+    total += st.y;
+  }
+  if (scribe && tid == 0) a.prefix[a.n_seqs] = total;
+  // no run is empty: fewer tiles than CTAs go to as many CTAs
+  const int64_t ctas = min((int64_t)gridDim.x, total);
+  if (blockIdx.x >= ctas) return false;
+  w0 = total * blockIdx.x / ctas;
+  w1 = total * (blockIdx.x + 1) / ctas;
+  int64_t base = 0;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += NT) {
+    const int64_t v = weight(s0 + tid, nullptr);
+    const longlong2 st = a.n_seqs <= NT ? first : strip_sum(v);
+    const int64_t at = base + st.x;
+    if (w0 >= at && w0 < at + v) {
+      sc.seq = s0 + tid;
+      sc.base = at;
+    }
+    base += st.y;
+    if (base > w0) break;
+  }
+  __syncthreads();
+  seq = sc.seq;
+  seq_base = sc.base;
+  return true;
+}
+
+// The producer warp's part of a segment: `seg` tiles from tile0 on into the ring of
+// stages (tile number `it` of this CTA comes first).  A lane per box looks its page up,
+// 32 boxes ahead; a missing page is flagged and its positions are left as they are.
+template <int D, int BN, int ST>
+__device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMap& kmap,
+                                             const CUtensorMap& vmap, uint32_t kv0,
+                                             unsigned long long* fulls, unsigned long long* empties,
+                                             int seq, int kvh, int len, int tile0, int seg, int it) {
+  constexpr int HALVES = D / 64;
+  const int lane = threadIdx.x & 31;
+  const int per_tile = BN / a.box;                   // boxes of a tile
+  for (int b0 = 0; b0 < seg * per_tile; b0 += 32) {
+    const int p_box = (tile0 * per_tile + b0 + lane) * a.box;
+    int page = -2, row = 0;                          // -2: nothing to load
+    if (b0 + lane < seg * per_tile && p_box < len) {
+      const int blk = p_box / a.block_size;
+      row = p_box - blk * a.block_size;
+      page = blk < a.max_blocks ? a.tables[seq * a.table_stride + blk] : -1;
+      if (page < 0 || page >= a.num_blocks) {
+        if (a.status) atomicOr(a.status, GDN_STATUS_BAD_SLOT);
+        page = -2;
+      }
+    }
+    const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+    const int boxes = min(32, seg * per_tile - b0);
+    for (int i = 0; i < boxes; ++i) {
+      const int in_tile = (b0 + i) % per_tile;
+      const int t = it + (b0 + i) / per_tile, stage = t % ST;
+      const int pg = __shfl_sync(0xffffffffu, page, i), rw = __shfl_sync(0xffffffffu, row, i);
+      if (lane == 0) {
+        const uint32_t full = tc::smem_u32(&fulls[stage]);
+        if (in_tile == 0 &&
+            !tc::mbar_wait(tc::smem_u32(&empties[stage]), ((t / ST) & 1) ^ 1, kAttnWait) && a.status)
+          atomicOr(a.status, GDN_STATUS_TIMEOUT);
+        if (in_tile == 0 || i == 0) {
+          // the boxes of this tile that this round of 32 issues; the tile's last
+          // round makes the arrival
+          const int m = min(per_tile - in_tile, boxes - i);
+          const int live = __popc(there >> i & (m == 32 ? 0xffffffffu : (1u << m) - 1));
+          const uint32_t bytes = (uint32_t)live * a.box * D * 4;
+          if (in_tile + m == per_tile) tc::mbar_expect_tx(full, bytes);
+          else asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full),
+                            "r"(bytes) : "memory");
+        }
+        if (pg >= 0) {
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int hf = 0; hf < HALVES; ++hf)
+              asm volatile(
+                  "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+                  "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                      kv0 + ((stage * 2 + kv) * HALVES + hf) * (BN * 128) + in_tile * a.box * 128),
+                  "l"(kv == 0 ? &kmap : &vmap), "r"(hf * 64), "r"(kvh), "r"(rw), "r"(pg), "r"(full)
+                  : "memory");
+        }
+      }
+      __syncwarp();
+    }
+  }
+}
+
 template <int D, int WM, int WN>
 struct Attn {
   static constexpr int BM = 16 * WM, BN = 64, NC = WM * WN;      // NC: consumer warps
   static constexpr int WT = BN / WN;                              // positions per warp
   static constexpr int HALVES = D / 64;                           // 128-byte column blocks
-  static constexpr int CTAS = D <= 128 && WM <= 4 ? 2 : 1;        // per SM
+  static constexpr int CTAS = D <= 128 ? 2 : 1;                   // per SM
   static constexpr int STAGE = 2 * BN * D * 2;                    // bytes of keys and values
-  static constexpr int ST = CTAS == 2 ? (D == 64 ? 5 : 3) : (D == 256 ? 3 : 5);
+  static constexpr int ST = D == 64 ? 5 : 3;
   struct Smem {
     __align__(1024) unsigned char kv[ST][2][HALVES][BN * 128];
     __align__(16) float join[WN > 1 ? WN * BM * 36 : 4];          // 32 columns at a time
     float2 ml[WN > 1 ? WN * BM : 1];
     unsigned long long anc[kMaxTreeNodes];
     unsigned long long full[ST], empty[ST], bad;
-    int64_t scan_base, scan_total;
-    int scan_warp[NC + 1], scan_seq;
+    AttnScan scan;
     int par[kMaxTreeNodes];
   };
 };
@@ -123,7 +255,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
     attention_tree_kernel(const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const AttnArgs a) {
   using P = Attn<D, WM, WN>;
-  constexpr int NC = P::NC, NT = 32 * (NC + 1), BM = P::BM, BN = P::BN, WT = P::WT, ST = P::ST;
+  constexpr int NC = P::NC, BM = P::BM, BN = P::BN, WT = P::WT, ST = P::ST;
   static_assert(WT % 16 == 0, "a warp takes whole 16-position blocks");
   extern __shared__ unsigned char smem_raw[];
   auto& sm = *reinterpret_cast<typename P::Smem*>(
@@ -137,61 +269,11 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
     }
     tc::mbar_init_fence();
   }
-  // ---- this CTA's run of tiles: scan the sequences in strips of NT ----
-  const auto weight = [&](int r, int32_t* status) -> int64_t {
-    if (r >= a.n_seqs) return 0;
-    const AttnSeq s = attn_seq<BM, BN>(a, r, status);
-    return (int64_t)s.tiles * s.row_tiles * a.HKV;
-  };
-  const auto strip_sum = [&](int64_t v) {            // block-wide sum, and the sum before this thread
-    int64_t inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += t;
-    }
-    // a strip's tiles fit 31 bits: NT sequences of at most 2^24 tiles (host check)
-    __syncthreads();
-    if (lane == 31) sm.scan_warp[warp] = (int)inc;
-    __syncthreads();
-    int64_t before = inc - v, total = 0;
-    for (int w = 0; w <= NC; ++w) {
-      if (w < warp) before += sm.scan_warp[w];
-      total += sm.scan_warp[w];
-    }
-    return make_longlong2(before, total);
-  };
-  int64_t total = 0;
-  const bool scribe = blockIdx.x == 0;
-  longlong2 first{0, 0};
-  for (int s0 = 0; s0 < a.n_seqs; s0 += NT) {
-    const longlong2 st = strip_sum(weight(s0 + tid, scribe ? a.status : nullptr));
-    if (s0 == 0) first = st;
-    if (scribe && s0 + tid < a.n_seqs) a.prefix[s0 + tid] = total + st.x;
-    total += st.y;
-  }
-  if (scribe && tid == 0) a.prefix[a.n_seqs] = total;
-  // no run is empty: fewer tiles than CTAs go to as many CTAs
-  const int64_t ctas = min((int64_t)gridDim.x, total);
-  if (blockIdx.x >= ctas) return;
-  const int64_t w0 = total * blockIdx.x / ctas, w1 = total * (blockIdx.x + 1) / ctas;
-  int64_t base = 0;
-  for (int s0 = 0; s0 < a.n_seqs; s0 += NT) {
-    const int64_t v = weight(s0 + tid, nullptr);
-    const longlong2 st = a.n_seqs <= NT ? first : strip_sum(v);
-    const int64_t at = base + st.x;
-    if (w0 >= at && w0 < at + v) {
-      sm.scan_seq = s0 + tid;
-      sm.scan_base = at;
-    }
-    base += st.y;
-    if (base > w0) break;
-  }
-  __syncthreads();
+  int64_t w0, w1, seq_base;
+  int seq;
+  if (!attn_run<BM, BN, NC + 1>(a, sm.scan, w0, w1, seq, seq_base)) return;
 
   // ---- the run, a segment (part of a unit) at a time; every warp keeps the same place ----
-  int seq = sm.scan_seq;
-  int64_t seq_base = sm.scan_base;
   int it = 0;                                        // tiles of this CTA so far
   for (int64_t w = w0; w < w1;) {
     const AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
@@ -208,63 +290,8 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
     const int len = s.ctx + s.n;
 
     if (warp == NC) {
-      // ---- producer: a lane per box looks its page up, 32 boxes ahead ----
-      const int per_tile = BN / a.box;               // boxes of a tile
-      for (int b0 = 0; b0 < seg * per_tile; b0 += 32) {
-        const int p_box = (tile0 * per_tile + b0 + lane) * a.box;
-        int page = -2, row = 0;                      // -2: behind the last node, nothing to load
-        if (b0 + lane < seg * per_tile && p_box < len) {
-          const int blk = p_box / a.block_size;
-          row = p_box - blk * a.block_size;
-          page = blk < a.max_blocks ? a.tables[seq * a.table_stride + blk] : -1;
-          if (page < 0 || page >= a.num_blocks) {
-            if (a.status) atomicOr(a.status, GDN_STATUS_BAD_SLOT);
-            page = -2;
-          }
-        }
-        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
-        const int boxes = min(32, seg * per_tile - b0);
-        for (int i = 0; i < boxes; ++i) {
-          const int in_tile = (b0 + i) % per_tile;
-          const int t = it + (b0 + i) / per_tile, stage = t % ST;
-          const int pg = __shfl_sync(0xffffffffu, page, i), rw = __shfl_sync(0xffffffffu, row, i);
-          if (lane == 0) {
-            const uint32_t full = tc::smem_u32(&sm.full[stage]);
-            if (in_tile == 0) {
-              if (!tc::mbar_wait(tc::smem_u32(&sm.empty[stage]), ((t / ST) & 1) ^ 1, kAttnWait) &&
-                  a.status)
-                atomicOr(a.status, GDN_STATUS_TIMEOUT);
-            }
-            if (in_tile == 0 || i == 0) {
-              // the boxes of this tile that this round of 32 issues; the tile's last
-              // round makes the arrival
-              const int m = min(per_tile - in_tile, boxes - i);
-              const int live = __popc(there >> i & (m == 32 ? 0xffffffffu : (1u << m) - 1));
-              const uint32_t bytes = (uint32_t)live * a.box * D * 4;
-              if (in_tile + m == per_tile) tc::mbar_expect_tx(full, bytes);
-              else asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full),
-                                "r"(bytes) : "memory");
-            }
-            if (pg >= 0) {
-#pragma unroll
-              for (int hf = 0; hf < P::HALVES; ++hf) {
-                const uint32_t off = in_tile * a.box * 128;
-                asm volatile(
-                    "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
-                    "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(tc::smem_u32(&sm.kv[stage][0][hf][0]) + off),
-                    "l"(&kmap), "r"(hf * 64), "r"(kvh), "r"(rw), "r"(pg), "r"(full)
-                    : "memory");
-                asm volatile(
-                    "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
-                    "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(tc::smem_u32(&sm.kv[stage][1][hf][0]) + off),
-                    "l"(&vmap), "r"(hf * 64), "r"(kvh), "r"(rw), "r"(pg), "r"(full)
-                    : "memory");
-              }
-            }
-          }
-          __syncwarp();
-        }
-      }
+      attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, seq,
+                              kvh, len, tile0, seg, it);
     } else {
       // ---- consumers ----
       const auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(NC * 32) : "memory"); };
@@ -521,15 +548,290 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows (more than 32 of a unit): the same on tcgen05, 128 rows to a tile.
+//
+// mma.sync reaches a quarter of the tensor cores' rate, and 128 rows need 64 products
+// per byte: with it, 32 trees of 16 to 32 nodes over 4 to 8 thousand positions took
+// 214 us against 62 of memory traffic.  Here one thread issues S = Q K^T (128 x 64) and
+// O += P V (128 x D) from shared memory into TMEM; four warps, a thread per row, read S
+// (no exchange between lanes), write P as bf16 into shared memory and correct O; S and P
+// are double, so the products of a tile run under the softmax of the one before, and
+// the TMA producer keeps ST - 1 further tiles under way.  O is corrected only
+// when a row's maximum has grown by more than 2^8 since its last correction: until then
+// its probabilities are measured against the older maximum, which the final division
+// cancels.
+// ---------------------------------------------------------------------------
+template <int D>
+struct AttnTc {
+  static constexpr int BM = 128, BN = 64, HALVES = D / 64, ST = D == 64 ? 8 : 4;
+  static constexpr uint32_t kColS = 0, kColO = 128, kCols = 256;   // S: two of 64 columns
+  struct Smem {
+    __align__(1024) unsigned char kv[ST][2][HALVES][BN * 128];
+    __align__(1024) unsigned char q[HALVES][BM * 128];
+    __align__(1024) unsigned char p[2][BM * 128];
+    unsigned long long anc[kMaxTreeNodes], bad;
+    unsigned long long full[ST], empty[ST], s_full[2], s_free[2], p_full[2], pv_done[2], q_full;
+    AttnScan scan;
+    uint32_t tmem;
+    int par[kMaxTreeNodes];
+  };
+};
+
+template <int D>
+__global__ void __launch_bounds__(192, 1)
+    attention_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+                             const __grid_constant__ CUtensorMap vmap, const AttnArgs a) {
+  using P = AttnTc<D>;
+  constexpr int BM = P::BM, BN = P::BN, ST = P::ST, HALVES = P::HALVES;
+  extern __shared__ unsigned char smem_raw[];
+  auto& sm = *reinterpret_cast<typename P::Smem*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const auto bar = [](unsigned long long& b) { return tc::smem_u32(&b); };
+
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      tc::mbar_init(bar(sm.full[i]), 1);
+      tc::mbar_init(bar(sm.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(bar(sm.s_full[i]), 1);
+      tc::mbar_init(bar(sm.s_free[i]), 4);
+      tc::mbar_init(bar(sm.p_full[i]), 4);
+      tc::mbar_init(bar(sm.pv_done[i]), 1);
+    }
+    tc::mbar_init(bar(sm.q_full), 4);
+    tc::mbar_init_fence();
+  }
+  int64_t w0, w1, seq_base;
+  int seq;
+  if (!attn_run<BM, BN, 6>(a, sm.scan, w0, w1, seq, seq_base)) return;
+  if (warp == 5) tc::tmem_alloc(tc::smem_u32(&sm.tmem), P::kCols);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sm.tmem;
+
+  // a bounded wait; one that gives up is flagged and waits once more
+  const auto wait = [&](unsigned long long& b, uint32_t parity) {
+    if (tc::mbar_wait(bar(b), parity, kAttnWait)) return;
+    if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
+    tc::mbar_wait(bar(b), parity, kAttnWait);
+  };
+
+  int it = 0, segs = 0;                              // tiles and segments of this CTA so far
+  for (int64_t w = w0; w < w1;) {
+    const AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
+    const int64_t mine = (int64_t)s.tiles * s.row_tiles * a.HKV;
+    if (w >= seq_base + mine) {
+      seq_base += mine;
+      ++seq;
+      continue;
+    }
+    const int64_t local = w - seq_base;
+    const int unit = (int)(local / s.tiles), tile0 = (int)(local - (int64_t)unit * s.tiles);
+    const int kvh = unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
+    const int seg = (int)min((int64_t)(s.tiles - tile0), w1 - w);
+
+    if (warp == 4) {
+      attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, seq,
+                              kvh, s.ctx + s.n, tile0, seg, it);
+    } else if (warp == 5) {
+      // ---- products ----
+      if (lane == 0) {
+        const uint32_t q0 = tc::smem_u32(&sm.q[0][0]);
+        const auto scores = [&](int T) {
+          wait(sm.full[T % ST], (T / ST) & 1);
+          wait(sm.s_free[T & 1], ((T >> 1) & 1) ^ 1);
+          tc::fence_after();
+          const uint32_t k0 = tc::smem_u32(&sm.kv[T % ST][0][0][0]);
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)
+            tc::mma_bf16(tmem + P::kColS + (T & 1) * 64,
+                         tc::smem_desc(q0 + (x >> 2) * (BM * 128) + (x & 3) * 32, 16, 1024),
+                         tc::smem_desc(k0 + (x >> 2) * (BN * 128) + (x & 3) * 32, 16, 1024),
+                         tc::idesc_bf16(BM, BN, false, false), x > 0);
+          tc::mma_commit(bar(sm.s_full[T & 1]));
+        };
+        wait(sm.q_full, segs & 1);
+        scores(it);
+        for (int t = 0; t < seg; ++t) {
+          const int T = it + t;
+          if (t + 1 < seg) scores(T + 1);
+          wait(sm.p_full[T & 1], (T >> 1) & 1);
+          tc::fence_after();
+          const uint32_t p0 = tc::smem_u32(&sm.p[T & 1][0]);
+          const uint32_t v0 = tc::smem_u32(&sm.kv[T % ST][1][0][0]);
+#pragma unroll
+          for (int x = 0; x < BN / 16; ++x)
+            tc::mma_bf16(tmem + P::kColO, tc::smem_desc(p0 + x * 32, 16, 1024),
+                         tc::smem_desc(v0 + x * 2048, BN * 128, 1024),
+                         tc::idesc_bf16(BM, D, false, true), (t > 0 || x > 0) ? 1u : 0u);
+          tc::mma_commit(bar(sm.empty[T % ST]));
+          tc::mma_commit(bar(sm.pv_done[T & 1]));
+        }
+      }
+      __syncwarp();
+    } else {
+      // ---- softmax: a thread per row ----
+      const auto sync = [&]() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+      const int row = rt * BM + tid, rows = s.n * a.G;
+      const bool masks = (tile0 + seg) * BN > s.ctx;  // the segment reaches the nodes
+      if (masks) {
+        if (tid < s.n) sm.par[tid] = tree_parent(a.parents[s.start + tid], tid, a.status);
+        if (tid == 0) sm.bad = 0;
+        sync();
+        if (tid < s.n) {
+          unsigned long long m = 0;
+          for (int j = tid; j >= 0; j = sm.par[j]) m |= 1ull << j;
+          sm.anc[tid] = m;
+        }
+      }
+      const int node = min(row, rows - 1) / a.G;
+      const int64_t at = (s.start + node) * a.HQ + kvh * a.G + row - node * a.G;
+      {
+        const bf16* src = a.q + (s.start + node) * a.qs + (int64_t)(kvh * a.G + row - node * a.G) * D;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 u = row < rows ? *reinterpret_cast<const uint4*>(src + c * 8)
+                                     : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(&sm.q[c >> 3][tc::sw128(tid, (c & 7) * 8)]) = u;
+        }
+      }
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(bar(sm.q_full));
+      if (masks) sync();
+      const unsigned long long anc = masks && row < rows ? sm.anc[node] : 0ull;
+      const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);
+
+      float ref = -INFINITY, sum = 0.f;              // base 2: what the probabilities are measured against
+      for (int t = 0; t < seg; ++t) {
+        const int T = it + t, p_tile = (tile0 + t) * BN;
+        const bool edge = p_tile + BN > s.ctx;       // holds nodes or positions behind them
+        if (edge) {
+          wait(sm.full[T % ST], (T / ST) & 1);
+          unsigned char* vt = &sm.kv[T % ST][1][0][0];
+          for (int i = tid; i < BN * (D / 8); i += 128) {
+            const int r = i / (D / 8), c = i - r * (D / 8), j = p_tile + r - s.ctx;
+            if (j < 0) continue;
+            uint4* p = reinterpret_cast<uint4*>(vt + tile_at<BN>(r, c));
+            float f[8];
+            unpack8(*p, f);
+            bool finite = true;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) finite &= fabsf(f[e]) <= 3.4e38f;
+            if (j >= s.n || !finite) {
+              *p = make_uint4(0, 0, 0, 0);
+              if (j < s.n) atomicOr(&sm.bad, 1ull << j);
+            }
+          }
+        }
+        wait(sm.s_full[T & 1], (T >> 1) & 1);
+        tc::fence_after();
+        float x[2][32];
+        tc::tmem_ld32x2(tl + P::kColS + (T & 1) * 64, tl + P::kColS + (T & 1) * 64 + 32, x[0], x[1]);
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(bar(sm.s_free[T & 1]));
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            const int j = p_tile + i - s.ctx;
+            if (!(j < 0 || (j < s.n && (anc >> (j & 63) & 1)))) x[i >> 5][i & 31] = -INFINITY;
+          }
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], x[i >> 5][i & 31]);
+        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+        const bool grown = m > ref + 8.f;            // (from -inf: the row's first positions)
+        const float was = ref;
+        if (grown) ref = m;
+        const float off = ref == -INFINITY ? 0.f : ref;
+        const float corr = grown ? ex2(was - off) : 1.f;
+        float a4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          float& v = x[i >> 5][i & 31];
+          v = ex2(fmaf(v, a.scale_log2, -off));
+          a4[i & 3] += v;
+        }
+        sum = sum * corr + ((a4[0] + a4[1]) + (a4[2] + a4[3]));
+        // P's buffer was read by the product of two tiles ago
+        wait(sm.pv_done[T & 1], ((T >> 1) & 1) ^ 1);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(&sm.p[T & 1][tc::sw128(tid, c * 8)]) =
+              pack8(&x[c >> 2][(c & 3) * 8]);
+        if (t > 0 && __any_sync(0xffffffffu, grown)) {
+          wait(sm.pv_done[(T - 1) & 1], ((T - 1) >> 1) & 1);
+          tc::fence_after();
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            tc::tmem_ld32(tl + P::kColO + c, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= corr;
+            tc::tmem_st32(tl + P::kColO + c, o);
+          }
+          tc::tmem_wait_st();
+        }
+        tc::fence_async_smem();                      // P and the zeroed values, before the product reads them
+        tc::fence_before();
+        if (edge) sync();                            // every value row is clean
+        else __syncwarp();
+        if (lane == 0) tc::mbar_arrive(bar(sm.p_full[T & 1]));
+      }
+      // the last product is done: O is whole
+      wait(sm.pv_done[(it + seg - 1) & 1], ((it + seg - 1) >> 1) & 1);
+      tc::fence_after();
+      const bool whole = tile0 == 0 && seg == s.tiles;
+      const int64_t part = ((int64_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * BM + tid;
+      const bool nan = masks && (anc & *reinterpret_cast<volatile unsigned long long*>(&sm.bad)) != 0;
+      const float inv = nan ? __int_as_float(0x7fffffff) : whole ? 1.f / sum : 1.f;
+      if (!whole && row < rows) a.part_ml[part] = make_float2(ref, sum);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        tc::tmem_ld32(tl + P::kColO + c, o);
+        if (row < rows) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= inv;
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              *reinterpret_cast<uint4*>(a.out + at * D + c + e) = pack8(o + e);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(a.part_o + part * D + c + e) =
+                  make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+      }
+      tc::fence_before();
+      sync();                                        // masks, Q and O are used up
+    }
+    it += seg;
+    ++segs;
+    w += seg;
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 5) tc::tmem_dealloc(tmem, P::kCols);
+}
+
 // Joins the parts of a unit that was cut: a CTA per (sequence, kv-head, row tile) and
 // four of its rows, a warp each; or, SHARE, where there are fewer units than CTAs and
 // hence many parts to each, a CTA per row whose warps share its parts.  (Launched early,
 // to wait on the device for the first kernel's end, the two took 2 us longer.)
-template <int D, int WM, int WN, bool SHARE>
+template <int D, int BM, int BN, bool SHARE>
 __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, int max_row_tiles,
                                                              int grid) {
-  using P = Attn<D, WM, WN>;
-  constexpr int BM = P::BM, BN = P::BN, CPL = D / 32;   // columns per lane
+  constexpr int CPL = D / 32;                          // columns per lane
   __shared__ float s_o[SHARE ? 4 : 1][SHARE ? D : 1];
   __shared__ float2 s_ml[4];
   const int per_seq = a.HKV * max_row_tiles;
@@ -617,20 +919,22 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
   }
 }
 
-// Rows per CTA tile (16 wm) by the rows of the largest tree, and how many CTAs run.
-// (128 rows of head dim 256 would not fit the registers.)
-static int attn_wm(int max_nodes, int G, int D) {
+// Rows per CTA tile, by the rows of the largest tree: 16 or 32 (mma.sync; the traffic
+// bounds them), 128 on tcgen05 from 33 on (17 nodes of 4 heads: 116 us with mma.sync at 64
+// rows, TC64 here).  Head dim 256: 64 at most, with mma.sync (128 rows would not fit
+// TMEM and shared memory).  And how many CTAs run.
+static int attn_rows(int max_nodes, int G, int D) {
   const int rows = max_nodes * G;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 || D == 256 ? 4 : 8;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : D == 256 ? 64 : 128;
 }
-static int attn_ctas(int wm, int D) { return kAttnSms * (D <= 128 && wm <= 4 ? 2 : 1); }
+static int attn_ctas(int bm, int D) { return kAttnSms * (D <= 128 && bm <= 32 ? 2 : 1); }
 
 struct AttnSpace {
   int64_t prefix, part_o, part_ml, bytes;
 };
-static AttnSpace attn_space(int wm, int n_seqs, int D) {
+static AttnSpace attn_space(int bm, int n_seqs, int D) {
   const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-  const int64_t rows = (int64_t)attn_ctas(wm, D) * 2 * 16 * wm;
+  const int64_t rows = (int64_t)attn_ctas(bm, D) * 2 * bm;
   AttnSpace s;
   s.prefix = 0;
   s.part_o = up((n_seqs + 1ll) * 8);
@@ -639,24 +943,45 @@ static AttnSpace attn_space(int wm, int n_seqs, int D) {
   return s;
 }
 
+template <int D, int BM, int BN>
+static void launch_join(const AttnArgs& a, int ctas, cudaStream_t s) {
+  const int row_tiles = (a.max_nodes * a.G + BM - 1) / BM;
+  const int rows = row_tiles > 1 ? BM : a.max_nodes * a.G;
+  const bool share = (int64_t)a.n_seqs * a.HKV * row_tiles * 4 < ctas;
+  const dim3 grid((unsigned)(a.n_seqs * a.HKV * row_tiles), (unsigned)(share ? rows : (rows + 3) / 4));
+  if (share) attention_join_kernel<D, BM, BN, true><<<grid, 128, 0, s>>>(a, row_tiles, ctas);
+  else attention_join_kernel<D, BM, BN, false><<<grid, 128, 0, s>>>(a, row_tiles, ctas);
+}
+
 template <int D, int WM, int WN>
 static int launch_attention(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttnArgs& a,
                             cudaStream_t s) {
   using P = Attn<D, WM, WN>;
   constexpr size_t bytes = sizeof(typename P::Smem) + 1024;
-  static_assert(bytes * P::CTAS + 1024 * P::CTAS <= 228 * 1024, "shared memory of one SM");
+  static_assert((bytes + 1024) * P::CTAS <= 228 * 1024, "shared memory of one SM");
   auto fn = attention_tree_kernel<D, WM, WN>;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
       cudaSuccess)
     return check_launch("gdn_attention_tree");
-  const int ctas = attn_ctas(WM, D);
+  const int ctas = attn_ctas(P::BM, D);
   fn<<<ctas, 32 * (P::NC + 1), bytes, s>>>(kmap, vmap, a);
-  const int row_tiles = (a.max_nodes * a.G + P::BM - 1) / P::BM;
-  const int rows = row_tiles > 1 ? P::BM : a.max_nodes * a.G;
-  const bool share = (int64_t)a.n_seqs * a.HKV * row_tiles * 4 < ctas;
-  const dim3 grid((unsigned)(a.n_seqs * a.HKV * row_tiles), (unsigned)(share ? rows : (rows + 3) / 4));
-  if (share) attention_join_kernel<D, WM, WN, true><<<grid, 128, 0, s>>>(a, row_tiles, ctas);
-  else attention_join_kernel<D, WM, WN, false><<<grid, 128, 0, s>>>(a, row_tiles, ctas);
+  launch_join<D, P::BM, P::BN>(a, ctas, s);
+  return check_launch("gdn_attention_tree");
+}
+
+template <int D>
+static int launch_attention_tc(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttnArgs& a,
+                               cudaStream_t s) {
+  using P = AttnTc<D>;
+  constexpr size_t bytes = sizeof(typename P::Smem) + 1024;
+  static_assert(bytes + 1024 <= 228 * 1024, "shared memory of one SM");
+  auto fn = attention_tree_tc_kernel<D>;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
+      cudaSuccess)
+    return check_launch("gdn_attention_tree");
+  const int ctas = attn_ctas(P::BM, D);
+  fn<<<ctas, 192, bytes, s>>>(kmap, vmap, a);
+  launch_join<D, P::BM, P::BN>(a, ctas, s);
   return check_launch("gdn_attention_tree");
 }
 
@@ -669,7 +994,7 @@ extern "C" int64_t gdn_attention_tree_workspace_bytes(int32_t n_seqs, int32_t nu
                                                       int32_t max_nodes) {
   if (n_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_nodes <= 0)
     return 0;
-  return attn_space(attn_wm(max_nodes, num_q_heads / num_kv_heads, head_dim), n_seqs,
+  return attn_space(attn_rows(max_nodes, num_q_heads / num_kv_heads, head_dim), n_seqs,
                     head_dim).bytes;
 }
 
@@ -711,15 +1036,15 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
   GDN_UNSUPPORTED(((q_row_stride | block_stride | token_stride | head_stride) & 7) == 0 &&
                       aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
                   "%s: operands and strides must be 16-byte aligned", fn);
-  const int G = num_q_heads / num_kv_heads, wm = attn_wm(max_nodes, G, head_dim);
+  const int G = num_q_heads / num_kv_heads, bm = attn_rows(max_nodes, G, head_dim);
   // the scan adds up 32-bit tile counts of up to 288 sequences; TMA coordinates are 32 bits
-  const int row_tiles = (max_nodes * G + 16 * wm - 1) / (16 * wm);
+  const int row_tiles = (max_nodes * G + bm - 1) / bm;
   GDN_UNSUPPORTED((max_len / 64 + 1ll) * num_kv_heads * row_tiles <= (1ll << 22) &&
                       num_blocks < (1ll << 31) && max_len <= (1 << 30),
                   "%s: max_len %d with %d kv heads too large", fn, max_len, num_kv_heads);
   GDN_UNSUPPORTED((int64_t)n_seqs * num_kv_heads * row_tiles < (1ll << 31),
                   "%s: too many sequences or heads", fn);
-  const AttnSpace sp = attn_space(wm, n_seqs, head_dim);
+  const AttnSpace sp = attn_space(bm, n_seqs, head_dim);
   GDN_REQUIRE(workspace != nullptr && workspace_bytes >= sp.bytes && aligned16(workspace),
               "%s: workspace of %lld bytes needed (16-byte aligned), got %lld", fn,
               (long long)sp.bytes, (long long)workspace_bytes);
@@ -750,14 +1075,18 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
                    reinterpret_cast<float*>(ws + sp.part_o),
                    reinterpret_cast<float2*>(ws + sp.part_ml), status};
   cudaStream_t s = (cudaStream_t)stream;
-#define GDN_AT(D)                                                   \
-  if (wm == 1) return launch_attention<D, 1, 4>(kmap, vmap, a, s);  \
-  if (wm == 2) return launch_attention<D, 2, 2>(kmap, vmap, a, s);  \
-  if (wm == 4) return launch_attention<D, 4, 1>(kmap, vmap, a, s);
-  if (head_dim == 64) { GDN_AT(64) }
-  if (head_dim == 128) { GDN_AT(128) }
-  if (head_dim == 256) { GDN_AT(256) }
+#define GDN_AT(D)                                                    \
+  if (bm == 16) return launch_attention<D, 1, 4>(kmap, vmap, a, s);  \
+  if (bm == 32) return launch_attention<D, 2, 2>(kmap, vmap, a, s);
+  if (head_dim == 64) {
+    GDN_AT(64)
+    return launch_attention_tc<64>(kmap, vmap, a, s);
+  }
+  if (head_dim == 128) {
+    GDN_AT(128)
+    return launch_attention_tc<128>(kmap, vmap, a, s);
+  }
+  GDN_AT(256)
 #undef GDN_AT
-  return head_dim == 64 ? launch_attention<64, 8, 1>(kmap, vmap, a, s)
-                        : launch_attention<128, 8, 1>(kmap, vmap, a, s);
+  return launch_attention<256, 4, 1>(kmap, vmap, a, s);
 }
