@@ -88,7 +88,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int r, int32_t* s
 // Shared memory of the scan that finds a CTA's run of tiles.
 struct AttnScan {
   int64_t base;
-  int warp[9], seq;
+  int warp[11], seq;
 };
 
 // The CTA's run [w0, w1) of all units' tiles, the sequence it begins in and that one's
@@ -112,7 +112,7 @@ __device__ __forceinline__ bool attn_run(const AttnArgs& a, AttnScan& sc, int64_
       const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    // a strip's tiles fit 31 bits: at most 288 sequences of 2^22 tiles (host check)
+    // a strip's tiles fit 31 bits: at most 352 sequences of 2^22 tiles (host check)
     __syncthreads();
     if (lane == 31) sc.warp[warp] = (int)inc;
     __syncthreads();
@@ -553,19 +553,21 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
 //
 // mma.sync reaches a quarter of the tensor cores' rate, and 128 rows need 64 products
 // per byte: with it, 32 trees of 16 to 32 nodes over 4 to 8 thousand positions took
-// 214 us against 62 of memory traffic.  Here one thread issues S = Q K^T (128 x 64) and
-// O += P V (128 x D) from shared memory into TMEM; four warps, a thread per row, read S
-// (no exchange between lanes), write P as bf16 into shared memory and correct O; S and P
-// are double, so the products of a tile run under the softmax of the one before, and
-// the TMA producer keeps ST - 1 further tiles under way.  O is corrected only
-// when a row's maximum has grown by more than 2^8 since its last correction: until then
-// its probabilities are measured against the older maximum, which the final division
-// cancels.
+// 214 us against 62 of memory traffic.  Here S = Q K^T (128 x 64) and O += P V (128 x D)
+// are issued by a thread each, from shared memory into TMEM; two groups of four warps, a thread
+// per row, take the tiles in turn: read S (no exchange between lanes), write P as bf16
+// into shared memory and correct O.  Each group has its own S, P, running maximum, sum
+// and O, joined at the end of a segment, so that the two chains of a tile (product,
+// softmax, product) never wait for one another (one group and one issuing thread: 144
+// us; this: 108, the tensor cores busy for some 1100 of a tile's 1350 cycles).  The TMA producer
+// keeps ST - 1 further tiles under way.  O is corrected only when a row's maximum has
+// grown by more than 2^8 since its last correction: until then its probabilities are
+// measured against the older maximum, which the final division cancels.
 // ---------------------------------------------------------------------------
 template <int D>
 struct AttnTc {
   static constexpr int BM = 128, BN = 64, HALVES = D / 64, ST = D == 64 ? 8 : 4;
-  static constexpr uint32_t kColS = 0, kColO = 128, kCols = 256;   // S: two of 64 columns
+  static constexpr uint32_t kColS = 0, kColO = 128, kCols = D == 64 ? 256 : 512;   // two of each
   struct Smem {
     __align__(1024) unsigned char kv[ST][2][HALVES][BN * 128];
     __align__(1024) unsigned char q[HALVES][BM * 128];
@@ -573,13 +575,14 @@ struct AttnTc {
     unsigned long long anc[kMaxTreeNodes], bad;
     unsigned long long full[ST], empty[ST], s_full[2], s_free[2], p_full[2], pv_done[2], q_full;
     AttnScan scan;
+    float2 ml[2][BM];
     uint32_t tmem;
     int par[kMaxTreeNodes];
   };
 };
 
 template <int D>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(352, 1)
     attention_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
                              const __grid_constant__ CUtensorMap vmap, const AttnArgs a) {
   using P = AttnTc<D>;
@@ -601,13 +604,13 @@ __global__ void __launch_bounds__(192, 1)
       tc::mbar_init(bar(sm.p_full[i]), 4);
       tc::mbar_init(bar(sm.pv_done[i]), 1);
     }
-    tc::mbar_init(bar(sm.q_full), 4);
+    tc::mbar_init(bar(sm.q_full), 8);
     tc::mbar_init_fence();
   }
   int64_t w0, w1, seq_base;
   int seq;
-  if (!attn_run<BM, BN, 6>(a, sm.scan, w0, w1, seq, seq_base)) return;
-  if (warp == 5) tc::tmem_alloc(tc::smem_u32(&sm.tmem), P::kCols);
+  if (!attn_run<BM, BN, 11>(a, sm.scan, w0, w1, seq, seq_base)) return;
+  if (warp == 9) tc::tmem_alloc(tc::smem_u32(&sm.tmem), P::kCols);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -634,54 +637,56 @@ __global__ void __launch_bounds__(192, 1)
     const int kvh = unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
     const int seg = (int)min((int64_t)(s.tiles - tile0), w1 - w);
 
-    if (warp == 4) {
+    if (warp == 8) {
       attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, seq,
                               kvh, s.ctx + s.n, tile0, seg, it);
-    } else if (warp == 5) {
-      // ---- products ----
-      if (lane == 0) {
-        const uint32_t q0 = tc::smem_u32(&sm.q[0][0]);
-        const auto scores = [&](int T) {
+    } else if (warp >= 9) {
+      // ---- products: a thread for S, one for O.  (One thread for both took 2200 cycles
+      // a tile, most of them instructions; hence also descriptors made once, of which a
+      // step advances the address field.) ----
+      if (lane == 0 && warp == 9) {
+        wait(sm.q_full, segs & 1);
+        const uint64_t qd = tc::smem_desc(tc::smem_u32(&sm.q[0][0]), 16, 1024);
+        for (int T = it; T < it + seg; ++T) {
           wait(sm.full[T % ST], (T / ST) & 1);
           wait(sm.s_free[T & 1], ((T >> 1) & 1) ^ 1);
           tc::fence_after();
-          const uint32_t k0 = tc::smem_u32(&sm.kv[T % ST][0][0][0]);
+          const uint64_t kd = tc::smem_desc(tc::smem_u32(&sm.kv[T % ST][0][0][0]), 16, 1024);
 #pragma unroll
           for (int x = 0; x < D / 16; ++x)
             tc::mma_bf16(tmem + P::kColS + (T & 1) * 64,
-                         tc::smem_desc(q0 + (x >> 2) * (BM * 128) + (x & 3) * 32, 16, 1024),
-                         tc::smem_desc(k0 + (x >> 2) * (BN * 128) + (x & 3) * 32, 16, 1024),
+                         qd + ((x >> 2) * (BM * 128) + (x & 3) * 32) / 16,
+                         kd + ((x >> 2) * (BN * 128) + (x & 3) * 32) / 16,
                          tc::idesc_bf16(BM, BN, false, false), x > 0);
           tc::mma_commit(bar(sm.s_full[T & 1]));
-        };
-        wait(sm.q_full, segs & 1);
-        scores(it);
+        }
+      } else if (lane == 0) {
         for (int t = 0; t < seg; ++t) {
           const int T = it + t;
-          if (t + 1 < seg) scores(T + 1);
+          wait(sm.full[T % ST], (T / ST) & 1);
           wait(sm.p_full[T & 1], (T >> 1) & 1);
           tc::fence_after();
-          const uint32_t p0 = tc::smem_u32(&sm.p[T & 1][0]);
-          const uint32_t v0 = tc::smem_u32(&sm.kv[T % ST][1][0][0]);
+          const uint64_t pd = tc::smem_desc(tc::smem_u32(&sm.p[T & 1][0]), 16, 1024);
+          const uint64_t vd = tc::smem_desc(tc::smem_u32(&sm.kv[T % ST][1][0][0]), BN * 128, 1024);
 #pragma unroll
           for (int x = 0; x < BN / 16; ++x)
-            tc::mma_bf16(tmem + P::kColO, tc::smem_desc(p0 + x * 32, 16, 1024),
-                         tc::smem_desc(v0 + x * 2048, BN * 128, 1024),
-                         tc::idesc_bf16(BM, D, false, true), (t > 0 || x > 0) ? 1u : 0u);
+            tc::mma_bf16(tmem + P::kColO + (T & 1) * D, pd + x * 32 / 16, vd + x * 2048 / 16,
+                         tc::idesc_bf16(BM, D, false, true), (t > 1 || x > 0) ? 1u : 0u);
           tc::mma_commit(bar(sm.empty[T % ST]));
           tc::mma_commit(bar(sm.pv_done[T & 1]));
         }
       }
       __syncwarp();
     } else {
-      // ---- softmax: a thread per row ----
-      const auto sync = [&]() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-      const int row = rt * BM + tid, rows = s.n * a.G;
+      // ---- softmax: a thread per row and group; group g takes the tiles of parity g ----
+      const auto sync_all = [&]() { asm volatile("bar.sync 3, 256;" ::: "memory"); };
+      const int grp = warp >> 2, r = tid & 127;
+      const int row = rt * BM + r, rows = s.n * a.G;
       const bool masks = (tile0 + seg) * BN > s.ctx;  // the segment reaches the nodes
       if (masks) {
         if (tid < s.n) sm.par[tid] = tree_parent(a.parents[s.start + tid], tid, a.status);
         if (tid == 0) sm.bad = 0;
-        sync();
+        sync_all();
         if (tid < s.n) {
           unsigned long long m = 0;
           for (int j = tid; j >= 0; j = sm.par[j]) m |= 1ull << j;
@@ -693,30 +698,31 @@ __global__ void __launch_bounds__(192, 1)
       {
         const bf16* src = a.q + (s.start + node) * a.qs + (int64_t)(kvh * a.G + row - node * a.G) * D;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
+        for (int i = 0; i < D / 16; ++i) {
+          const int c = grp * (D / 16) + i;
           const uint4 u = row < rows ? *reinterpret_cast<const uint4*>(src + c * 8)
                                      : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(&sm.q[c >> 3][tc::sw128(tid, (c & 7) * 8)]) = u;
+          *reinterpret_cast<uint4*>(&sm.q[c >> 3][tc::sw128(r, (c & 7) * 8)]) = u;
         }
       }
       tc::fence_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(bar(sm.q_full));
-      if (masks) sync();
+      if (masks) sync_all();
       const unsigned long long anc = masks && row < rows ? sm.anc[node] : 0ull;
-      const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);
+      const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 
       float ref = -INFINITY, sum = 0.f;              // base 2: what the probabilities are measured against
-      for (int t = 0; t < seg; ++t) {
+      for (int t = (grp ^ it) & 1; t < seg; t += 2) {
         const int T = it + t, p_tile = (tile0 + t) * BN;
         const bool edge = p_tile + BN > s.ctx;       // holds nodes or positions behind them
         if (edge) {
           wait(sm.full[T % ST], (T / ST) & 1);
           unsigned char* vt = &sm.kv[T % ST][1][0][0];
-          for (int i = tid; i < BN * (D / 8); i += 128) {
-            const int r = i / (D / 8), c = i - r * (D / 8), j = p_tile + r - s.ctx;
+          for (int i = r; i < BN * (D / 8); i += 128) {
+            const int vrow = i / (D / 8), c = i - vrow * (D / 8), j = p_tile + vrow - s.ctx;
             if (j < 0) continue;
-            uint4* p = reinterpret_cast<uint4*>(vt + tile_at<BN>(r, c));
+            uint4* p = reinterpret_cast<uint4*>(vt + tile_at<BN>(vrow, c));
             float f[8];
             unpack8(*p, f);
             bool finite = true;
@@ -728,13 +734,13 @@ __global__ void __launch_bounds__(192, 1)
             }
           }
         }
-        wait(sm.s_full[T & 1], (T >> 1) & 1);
+        wait(sm.s_full[grp], (T >> 1) & 1);
         tc::fence_after();
         float x[2][32];
-        tc::tmem_ld32x2(tl + P::kColS + (T & 1) * 64, tl + P::kColS + (T & 1) * 64 + 32, x[0], x[1]);
+        tc::tmem_ld32x2(tl + P::kColS + grp * 64, tl + P::kColS + grp * 64 + 32, x[0], x[1]);
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(bar(sm.s_free[T & 1]));
+        if (lane == 0) tc::mbar_arrive(bar(sm.s_free[grp]));
         if (edge) {
 #pragma unroll
           for (int i = 0; i < 64; ++i) {
@@ -759,46 +765,66 @@ __global__ void __launch_bounds__(192, 1)
           a4[i & 3] += v;
         }
         sum = sum * corr + ((a4[0] + a4[1]) + (a4[2] + a4[3]));
-        // P's buffer was read by the product of two tiles ago
-        wait(sm.pv_done[T & 1], ((T >> 1) & 1) ^ 1);
+        // the group's last product has read P and left O alone
+        wait(sm.pv_done[grp], ((T >> 1) & 1) ^ 1);
 #pragma unroll
         for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(&sm.p[T & 1][tc::sw128(tid, c * 8)]) =
-              pack8(&x[c >> 2][(c & 3) * 8]);
-        if (t > 0 && __any_sync(0xffffffffu, grown)) {
-          wait(sm.pv_done[(T - 1) & 1], ((T - 1) >> 1) & 1);
+          *reinterpret_cast<uint4*>(&sm.p[grp][tc::sw128(r, c * 8)]) = pack8(&x[c >> 2][(c & 3) * 8]);
+        if (t > 1 && __any_sync(0xffffffffu, grown)) {
           tc::fence_after();
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
             float o[32];
-            tc::tmem_ld32(tl + P::kColO + c, o);
+            tc::tmem_ld32(tl + P::kColO + grp * D + c, o);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] *= corr;
-            tc::tmem_st32(tl + P::kColO + c, o);
+            tc::tmem_st32(tl + P::kColO + grp * D + c, o);
           }
           tc::tmem_wait_st();
         }
         tc::fence_async_smem();                      // P and the zeroed values, before the product reads them
         tc::fence_before();
-        if (edge) sync();                            // every value row is clean
+        if (edge) asm volatile("bar.sync %0, 128;" ::"r"(grp + 1) : "memory");   // every value row is clean
         else __syncwarp();
-        if (lane == 0) tc::mbar_arrive(bar(sm.p_full[T & 1]));
+        if (lane == 0) tc::mbar_arrive(bar(sm.p_full[grp]));
       }
-      // the last product is done: O is whole
-      wait(sm.pv_done[(it + seg - 1) & 1], ((it + seg - 1) >> 1) & 1);
+      // join the groups: both last products are done
+      sm.ml[grp][r] = make_float2(ref, sum);
+      bool has[2];
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int T = it + seg - 1 - ((it + seg - 1 - v) & 1);   // the last tile of parity v
+        has[v] = T >= it;
+        if (has[v]) wait(sm.pv_done[v], (T >> 1) & 1);
+      }
       tc::fence_after();
+      sync_all();
+      const float2 ml0 = sm.ml[0][r], ml1 = sm.ml[1][r];
+      const float top = fmaxf(ml0.x, ml1.x), off = top == -INFINITY ? 0.f : top;
+      float f0 = ex2(ml0.x - off), f1 = ex2(ml1.x - off);
+      const float l = ml0.y * f0 + ml1.y * f1;
       const bool whole = tile0 == 0 && seg == s.tiles;
-      const int64_t part = ((int64_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * BM + tid;
+      const int64_t part = ((int64_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * BM + r;
       const bool nan = masks && (anc & *reinterpret_cast<volatile unsigned long long*>(&sm.bad)) != 0;
-      const float inv = nan ? __int_as_float(0x7fffffff) : whole ? 1.f / sum : 1.f;
-      if (!whole && row < rows) a.part_ml[part] = make_float2(ref, sum);
+      const float inv = nan ? __int_as_float(0x7fffffff) : whole ? 1.f / l : 1.f;
+      f0 *= inv;
+      f1 *= inv;
+      if (!whole && grp == 0 && row < rows) a.part_ml[part] = make_float2(top, l);
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int i = 0; i < D / 64; ++i) {
+        const int c = grp * (D / 2) + i * 32;        // a half of the columns each
         float o[32];
-        tc::tmem_ld32(tl + P::kColO + c, o);
-        if (row < rows) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= inv;
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+          if (has[v]) {
+            float y[32];
+            tc::tmem_ld32(tl + P::kColO + v * D + c, y);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(y[e], v == 0 ? f0 : f1, o[e]);
+          }
+        if (row < rows) {
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8)
@@ -812,7 +838,7 @@ __global__ void __launch_bounds__(192, 1)
         }
       }
       tc::fence_before();
-      sync();                                        // masks, Q and O are used up
+      sync_all();                                    // masks, Q and O are used up
     }
     it += seg;
     ++segs;
@@ -821,7 +847,7 @@ __global__ void __launch_bounds__(192, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 5) tc::tmem_dealloc(tmem, P::kCols);
+  if (warp == 9) tc::tmem_dealloc(tmem, P::kCols);
 }
 
 // Joins the parts of a unit that was cut: a CTA per (sequence, kv-head, row tile) and
@@ -920,8 +946,8 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
 }
 
 // Rows per CTA tile, by the rows of the largest tree: 16 or 32 (mma.sync; the traffic
-// bounds them), 128 on tcgen05 from 33 on (17 nodes of 4 heads: 116 us with mma.sync at 64
-// rows, TC64 here).  Head dim 256: 64 at most, with mma.sync (128 rows would not fit
+// bounds them), 128 on tcgen05 from 33 on (32 sequences of 6144 positions and 16 nodes
+// of 4 heads: 116 us with mma.sync at 64 rows, 95 here).  Head dim 256: 64 at most, with mma.sync (128 rows would not fit
 // TMEM and shared memory).  And how many CTAs run.
 static int attn_rows(int max_nodes, int G, int D) {
   const int rows = max_nodes * G;
@@ -980,7 +1006,7 @@ static int launch_attention_tc(const CUtensorMap& kmap, const CUtensorMap& vmap,
       cudaSuccess)
     return check_launch("gdn_attention_tree");
   const int ctas = attn_ctas(P::BM, D);
-  fn<<<ctas, 192, bytes, s>>>(kmap, vmap, a);
+  fn<<<ctas, 352, bytes, s>>>(kmap, vmap, a);
   launch_join<D, P::BM, P::BN>(a, ctas, s);
   return check_launch("gdn_attention_tree");
 }
@@ -1037,7 +1063,7 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
                       aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
                   "%s: operands and strides must be 16-byte aligned", fn);
   const int G = num_q_heads / num_kv_heads, bm = attn_rows(max_nodes, G, head_dim);
-  // the scan adds up 32-bit tile counts of up to 288 sequences; TMA coordinates are 32 bits
+  // the scan adds up 32-bit tile counts of up to 352 sequences; TMA coordinates are 32 bits
   const int row_tiles = (max_nodes * G + bm - 1) / bm;
   GDN_UNSUPPORTED((max_len / 64 + 1ll) * num_kv_heads * row_tiles <= (1ll << 22) &&
                       num_blocks < (1ll << 31) && max_len <= (1 << 30),
