@@ -55,9 +55,10 @@ struct AttnArgs {
   int max_len;
   bf16* out;
   int HQ, HKV, G;
+  int tile_rows;                  // rows of a row tile: BM, or on tcgen05 the whole nodes in it
   float scale_log2;
   int64_t* prefix;                // [n_seqs + 1]: tiles before each sequence's
-  float* part_o;                  // [CTAs][2][BM][D]
+  float* part_o;                  // [CTAs][2][D / 4][BM][4]: rows side by side
   float2* part_ml;                // [CTAs][2][BM]: maximum (base 2), sum
   int32_t* status;
 };
@@ -81,14 +82,15 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int r, int32_t* s
   s.n = n;
   s.ctx = c;
   s.tiles = (c + n + BN - 1) / BN;
-  s.row_tiles = (n * a.G + BM - 1) / BM;
+  const int rows = BM == 128 ? a.tile_rows : BM;     // (a constant divides faster)
+  s.row_tiles = (n * a.G + rows - 1) / rows;
   return s;
 }
 
 // Shared memory of the scan that finds a CTA's run of tiles.
 struct AttnScan {
   int64_t base;
-  int warp[11], seq;
+  int warp[12], seq;
 };
 
 // The CTA's run [w0, w1) of all units' tiles, the sequence it begins in and that one's
@@ -112,7 +114,7 @@ __device__ __forceinline__ bool attn_run(const AttnArgs& a, AttnScan& sc, int64_
       const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    // a strip's tiles fit 31 bits: at most 352 sequences of 2^22 tiles (host check)
+    // a strip's tiles fit 31 bits: at most 384 sequences of 2^22 tiles (host check)
     __syncthreads();
     if (lane == 31) sc.warp[warp] = (int)inc;
     __syncthreads();
@@ -220,12 +222,13 @@ __device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMa
 
 template <int D, int WM, int WN>
 struct Attn {
-  static constexpr int BM = 16 * WM, BN = 64, NC = WM * WN;      // NC: consumer warps
+  static constexpr int BM = 16 * WM, NC = WM * WN;               // NC: consumer warps
+  static constexpr int BN = D == 64 ? 128 : 64;                   // positions of a tile: 32 KB and more
   static constexpr int WT = BN / WN;                              // positions per warp
   static constexpr int HALVES = D / 64;                           // 128-byte column blocks
   static constexpr int CTAS = D <= 128 ? 2 : 1;                   // per SM
   static constexpr int STAGE = 2 * BN * D * 2;                    // bytes of keys and values
-  static constexpr int ST = D == 64 ? 5 : 3;
+  static constexpr int ST = 3;
   struct Smem {
     __align__(1024) unsigned char kv[ST][2][HALVES][BN * 128];
     __align__(16) float join[WN > 1 ? WN * BM * 36 : 4];          // 32 columns at a time
@@ -275,16 +278,15 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
 
   // ---- the run, a segment (part of a unit) at a time; every warp keeps the same place ----
   int it = 0;                                        // tiles of this CTA so far
+  AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
   for (int64_t w = w0; w < w1;) {
-    const AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
-    const int64_t mine = (int64_t)s.tiles * s.row_tiles * a.HKV;
+    const int mine = s.tiles * s.row_tiles * a.HKV;  // at most 2^22 (host check)
     if (w >= seq_base + mine) {
       seq_base += mine;
-      ++seq;
+      s = attn_seq<BM, BN>(a, ++seq, nullptr);
       continue;
     }
-    const int64_t local = w - seq_base;
-    const int unit = (int)(local / s.tiles), tile0 = (int)(local - (int64_t)unit * s.tiles);
+    const int local = (int)(w - seq_base), unit = local / s.tiles, tile0 = local - unit * s.tiles;
     const int kvh = unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
     const int seg = (int)min((int64_t)(s.tiles - tile0), w1 - w);
     const int len = s.ctx + s.n;
@@ -480,7 +482,9 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
             if (whole)
               *reinterpret_cast<uint32_t*>(a.out + at * D + i * 8 + 2 * tq) = mm::pack2(u, v);
             else
-              *reinterpret_cast<float2*>(a.part_o + (part + r) * D + i * 8 + 2 * tq) = make_float2(u, v);
+              *reinterpret_cast<float2*>(a.part_o + part * D +
+                                         ((i * 2 + (tq >> 1)) * BM + r) * 4 + (tq & 1) * 2) =
+                  make_float2(u, v);
           }
         }
         if (masks) sync();                           // the masks are used up
@@ -518,7 +522,8 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
                   make_float2(o[cq * 4 + i][hh * 2] * inv[hh], o[cq * 4 + i][hh * 2 + 1] * inv[hh]);
           sync();
           for (int i = tid; i < BM * 8; i += NC * 32) {
-            const int r = i >> 3, c = (i & 7) * 4, row = row0 + r;
+            // a whole unit's rows are written along their columns, parts along the rows
+            const int r = whole ? i >> 3 : i % BM, c = (whole ? i & 7 : i / BM) * 4, row = row0 + r;
             if (row < rows) {
               float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
                 *reinterpret_cast<uint2*>(a.out + at * D + cq * 32 + c) =
                     make_uint2(mm::pack2(acc.x, acc.y), mm::pack2(acc.z, acc.w));
               } else {
-                *reinterpret_cast<float4*>(a.part_o + (part + r) * D + cq * 32 + c) = acc;
+                *reinterpret_cast<float4*>(a.part_o + part * D + ((cq * 32 + c) / 4 * BM + r) * 4) = acc;
               }
             }
           }
@@ -559,8 +564,10 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
 // into shared memory and correct O.  Each group has its own S, P, running maximum, sum
 // and O, joined at the end of a segment, so that the two chains of a tile (product,
 // softmax, product) never wait for one another (one group and one issuing thread: 144
-// us; this: 108, the tensor cores busy for some 1100 of a tile's 1350 cycles).  The TMA producer
-// keeps ST - 1 further tiles under way.  O is corrected only when a row's maximum has
+// us).  The TMA producer keeps ST - 1 further tiles under way, and one more warp brings the
+// next segment's queries (a box of whole nodes' heads) and its nodes' ancestors: what a
+// segment does once is what is left above the memory traffic (queries through registers
+// when the segment began: 105 us, now 90; a longer context costs 6.3 TB/s).  O is corrected only when a row's maximum has
 // grown by more than 2^8 since its last correction: until then its probabilities are
 // measured against the older maximum, which the final division cancels.
 // ---------------------------------------------------------------------------
@@ -570,23 +577,24 @@ struct AttnTc {
   static constexpr uint32_t kColS = 0, kColO = 128, kCols = D == 64 ? 256 : 512;   // two of each
   struct Smem {
     __align__(1024) unsigned char kv[ST][2][HALVES][BN * 128];
-    __align__(1024) unsigned char q[HALVES][BM * 128];
+    __align__(1024) unsigned char q[2][HALVES][BM * 128];           // of two segments, as anc and bad
     __align__(1024) unsigned char p[2][BM * 128];
-    unsigned long long anc[kMaxTreeNodes], bad;
-    unsigned long long full[ST], empty[ST], s_full[2], s_free[2], p_full[2], pv_done[2], q_full;
+    unsigned long long anc[2][kMaxTreeNodes], bad[2];
+    unsigned long long full[ST], empty[ST], s_full[2], s_free[2], p_full[2], pv_done[2], q_full[2],
+        q_empty[2], anc_full[2];
     AttnScan scan;
-    float2 ml[2][BM];
     uint32_t tmem;
     int par[kMaxTreeNodes];
   };
 };
 
 template <int D>
-__global__ void __launch_bounds__(352, 1)
+__global__ void __launch_bounds__(384, 1)
     attention_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
-                             const __grid_constant__ CUtensorMap vmap, const AttnArgs a) {
+                             const __grid_constant__ CUtensorMap vmap,
+                             const __grid_constant__ CUtensorMap qmap, const AttnArgs a) {
   using P = AttnTc<D>;
-  constexpr int BM = P::BM, BN = P::BN, ST = P::ST, HALVES = P::HALVES;
+  constexpr int BM = P::BM, BN = P::BN, ST = P::ST;
   extern __shared__ unsigned char smem_raw[];
   auto& sm = *reinterpret_cast<typename P::Smem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -603,13 +611,15 @@ __global__ void __launch_bounds__(352, 1)
       tc::mbar_init(bar(sm.s_free[i]), 4);
       tc::mbar_init(bar(sm.p_full[i]), 4);
       tc::mbar_init(bar(sm.pv_done[i]), 1);
+      tc::mbar_init(bar(sm.q_full[i]), 1);
+      tc::mbar_init(bar(sm.anc_full[i]), 1);
+      tc::mbar_init(bar(sm.q_empty[i]), 9);           // the last S, and the softmax warps
     }
-    tc::mbar_init(bar(sm.q_full), 8);
     tc::mbar_init_fence();
   }
   int64_t w0, w1, seq_base;
   int seq;
-  if (!attn_run<BM, BN, 11>(a, sm.scan, w0, w1, seq, seq_base)) return;
+  if (!attn_run<BM, BN, 12>(a, sm.scan, w0, w1, seq, seq_base)) return;
   if (warp == 9) tc::tmem_alloc(tc::smem_u32(&sm.tmem), P::kCols);
   tc::fence_before();
   __syncthreads();
@@ -624,29 +634,52 @@ __global__ void __launch_bounds__(352, 1)
   };
 
   int it = 0, segs = 0;                              // tiles and segments of this CTA so far
+  AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
   for (int64_t w = w0; w < w1;) {
-    const AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
-    const int64_t mine = (int64_t)s.tiles * s.row_tiles * a.HKV;
+    const int mine = s.tiles * s.row_tiles * a.HKV;  // at most 2^22 (host check)
     if (w >= seq_base + mine) {
       seq_base += mine;
-      ++seq;
+      s = attn_seq<BM, BN>(a, ++seq, nullptr);
       continue;
     }
-    const int64_t local = w - seq_base;
-    const int unit = (int)(local / s.tiles), tile0 = (int)(local - (int64_t)unit * s.tiles);
+    const int local = (int)(w - seq_base), unit = local / s.tiles, tile0 = local - unit * s.tiles;
     const int kvh = unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
     const int seg = (int)min((int64_t)(s.tiles - tile0), w1 - w);
 
     if (warp == 8) {
       attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, seq,
                               kvh, s.ctx + s.n, tile0, seg, it);
+    } else if (warp == 11) {
+      // ---- the segment's queries and ancestors, while the one before is worked on ----
+      const int b = segs & 1;
+      wait(sm.q_empty[b], ((segs >> 1) & 1) ^ 1);
+      if (lane == 0) {
+        tc::mbar_expect_tx(bar(sm.q_full[b]), (uint32_t)a.tile_rows * D * 2);
+#pragma unroll
+        for (int hf = 0; hf < P::HALVES; ++hf)
+          tc::tma_load_3d(tc::smem_u32(&sm.q[b][hf][0]), &qmap, hf * 64, kvh * a.G,
+                          (int)s.start + rt * (a.tile_rows / a.G), bar(sm.q_full[b]));
+      }
+      if ((tile0 + seg) * BN > s.ctx) {              // the segment reaches the nodes
+        for (int j = lane; j < s.n; j += 32) sm.par[j] = tree_parent(a.parents[s.start + j], j, a.status);
+        __syncwarp();
+        for (int j = lane; j < s.n; j += 32) {
+          unsigned long long m = 0;
+          for (int x = j; x >= 0; x = sm.par[x]) m |= 1ull << x;
+          sm.anc[b][j] = m;
+        }
+        if (lane == 0) sm.bad[b] = 0;
+        __syncwarp();
+      }
+      if (lane == 0) tc::mbar_arrive(bar(sm.anc_full[b]));
+      __syncwarp();
     } else if (warp >= 9) {
       // ---- products: a thread for S, one for O.  (One thread for both took 2200 cycles
       // a tile, most of them instructions; hence also descriptors made once, of which a
       // step advances the address field.) ----
       if (lane == 0 && warp == 9) {
-        wait(sm.q_full, segs & 1);
-        const uint64_t qd = tc::smem_desc(tc::smem_u32(&sm.q[0][0]), 16, 1024);
+        wait(sm.q_full[segs & 1], (segs >> 1) & 1);
+        const uint64_t qd = tc::smem_desc(tc::smem_u32(&sm.q[segs & 1][0][0]), 16, 1024);
         for (int T = it; T < it + seg; ++T) {
           wait(sm.full[T % ST], (T / ST) & 1);
           wait(sm.s_free[T & 1], ((T >> 1) & 1) ^ 1);
@@ -660,6 +693,7 @@ __global__ void __launch_bounds__(352, 1)
                          tc::idesc_bf16(BM, BN, false, false), x > 0);
           tc::mma_commit(bar(sm.s_full[T & 1]));
         }
+        tc::mma_commit(bar(sm.q_empty[segs & 1]));
       } else if (lane == 0) {
         for (int t = 0; t < seg; ++t) {
           const int T = it + t;
@@ -681,44 +715,23 @@ __global__ void __launch_bounds__(352, 1)
       // ---- softmax: a thread per row and group; group g takes the tiles of parity g ----
       const auto sync_all = [&]() { asm volatile("bar.sync 3, 256;" ::: "memory"); };
       const int grp = warp >> 2, r = tid & 127;
-      const int row = rt * BM + r, rows = s.n * a.G;
-      const bool masks = (tile0 + seg) * BN > s.ctx;  // the segment reaches the nodes
-      if (masks) {
-        if (tid < s.n) sm.par[tid] = tree_parent(a.parents[s.start + tid], tid, a.status);
-        if (tid == 0) sm.bad = 0;
-        sync_all();
-        if (tid < s.n) {
-          unsigned long long m = 0;
-          for (int j = tid; j >= 0; j = sm.par[j]) m |= 1ull << j;
-          sm.anc[tid] = m;
-        }
-      }
-      const int node = min(row, rows - 1) / a.G;
+      const int row = rt * a.tile_rows + r;
+      const int rows = r < a.tile_rows ? s.n * a.G : 0;      // 0: no row of this thread's
+      const int node = row < rows ? row / a.G : 0;
       const int64_t at = (s.start + node) * a.HQ + kvh * a.G + row - node * a.G;
-      {
-        const bf16* src = a.q + (s.start + node) * a.qs + (int64_t)(kvh * a.G + row - node * a.G) * D;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const int c = grp * (D / 16) + i;
-          const uint4 u = row < rows ? *reinterpret_cast<const uint4*>(src + c * 8)
-                                     : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(&sm.q[c >> 3][tc::sw128(r, (c & 7) * 8)]) = u;
-        }
-      }
-      tc::fence_async_smem();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(bar(sm.q_full));
-      if (masks) sync_all();
-      const unsigned long long anc = masks && row < rows ? sm.anc[node] : 0ull;
       const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 
       float ref = -INFINITY, sum = 0.f;              // base 2: what the probabilities are measured against
       for (int t = (grp ^ it) & 1; t < seg; t += 2) {
         const int T = it + t, p_tile = (tile0 + t) * BN;
         const bool edge = p_tile + BN > s.ctx;       // holds nodes or positions behind them
+        unsigned long long anc = 0;
         if (edge) {
+          wait(sm.anc_full[segs & 1], (segs >> 1) & 1);
+          if (row < rows) anc = sm.anc[segs & 1][node];
           wait(sm.full[T % ST], (T / ST) & 1);
           unsigned char* vt = &sm.kv[T % ST][1][0][0];
+#pragma unroll 1
           for (int i = r; i < BN * (D / 8); i += 128) {
             const int vrow = i / (D / 8), c = i - vrow * (D / 8), j = p_tile + vrow - s.ctx;
             if (j < 0) continue;
@@ -730,7 +743,7 @@ __global__ void __launch_bounds__(352, 1)
             for (int e = 0; e < 8; ++e) finite &= fabsf(f[e]) <= 3.4e38f;
             if (j >= s.n || !finite) {
               *p = make_uint4(0, 0, 0, 0);
-              if (j < s.n) atomicOr(&sm.bad, 1ull << j);
+              if (j < s.n) atomicOr(&sm.bad[segs & 1], 1ull << j);
             }
           }
         }
@@ -741,11 +754,15 @@ __global__ void __launch_bounds__(352, 1)
         tc::fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(sm.s_free[grp]));
-        if (edge) {
+        if (edge) {                                  // a bit per position that the row sees
+          const int nodes_at = s.ctx - p_tile;       // > -64, as the tile holds a node
+          const unsigned long long see =
+              nodes_at >= 0 ? ((1ull << nodes_at) - 1) | anc << nodes_at : anc >> -nodes_at;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const int j = p_tile + i - s.ctx;
-            if (!(j < 0 || (j < s.n && (anc >> (j & 63) & 1)))) x[i >> 5][i & 31] = -INFINITY;
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t bits = (uint32_t)(see >> 32 * h);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[h][i] = bits >> i & 1 ? x[h][i] : -INFINITY;
           }
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -788,28 +805,35 @@ __global__ void __launch_bounds__(352, 1)
         else __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(sm.p_full[grp]));
       }
-      // join the groups: both last products are done
-      sm.ml[grp][r] = make_float2(ref, sum);
+      // join the groups: each waits for its own last product, which leaves its P free
       bool has[2];
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
         const int T = it + seg - 1 - ((it + seg - 1 - v) & 1);   // the last tile of parity v
         has[v] = T >= it;
-        if (has[v]) wait(sm.pv_done[v], (T >> 1) & 1);
+        if (has[v] && v == grp) wait(sm.pv_done[v], (T >> 1) & 1);
       }
-      tc::fence_after();
+      const auto ml = [&](int g) -> float2& { return reinterpret_cast<float2*>(&sm.p[g][0])[r]; };
+      ml(grp) = make_float2(ref, sum);
+      tc::fence_before();
       sync_all();
-      const float2 ml0 = sm.ml[0][r], ml1 = sm.ml[1][r];
+      tc::fence_after();
+      const float2 ml0 = ml(0), ml1 = ml(1);
       const float top = fmaxf(ml0.x, ml1.x), off = top == -INFINITY ? 0.f : top;
       float f0 = ex2(ml0.x - off), f1 = ex2(ml1.x - off);
       const float l = ml0.y * f0 + ml1.y * f1;
       const bool whole = tile0 == 0 && seg == s.tiles;
-      const int64_t part = ((int64_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * BM + r;
-      const bool nan = masks && (anc & *reinterpret_cast<volatile unsigned long long*>(&sm.bad)) != 0;
+      const int64_t part = ((int64_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * BM;
+      bool nan = false;                              // the row sees a value row that is not finite
+      if ((tile0 + seg) * BN > s.ctx) {
+        wait(sm.anc_full[segs & 1], (segs >> 1) & 1);
+        nan = row < rows && (sm.anc[segs & 1][node] &
+                             *reinterpret_cast<volatile unsigned long long*>(&sm.bad[segs & 1])) != 0;
+      }
       const float inv = nan ? __int_as_float(0x7fffffff) : whole ? 1.f / l : 1.f;
       f0 *= inv;
       f1 *= inv;
-      if (!whole && grp == 0 && row < rows) a.part_ml[part] = make_float2(top, l);
+      if (!whole && grp == 0 && row < rows) a.part_ml[part + r] = make_float2(top, l);
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
         const int c = grp * (D / 2) + i * 32;        // a half of the columns each
@@ -832,13 +856,14 @@ __global__ void __launch_bounds__(352, 1)
           } else {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(a.part_o + part * D + c + e) =
+              *reinterpret_cast<float4*>(a.part_o + part * D + ((c + e) / 4 * BM + r) * 4) =
                   make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
       }
       tc::fence_before();
-      sync_all();                                    // masks, Q and O are used up
+      sync_all();                                    // masks and O are used up
+      if (lane == 0) tc::mbar_arrive(bar(sm.q_empty[segs & 1]));
     }
     it += seg;
     ++segs;
@@ -850,16 +875,26 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 9) tc::tmem_dealloc(tmem, P::kCols);
 }
 
-// Joins the parts of a unit that was cut: a CTA per (sequence, kv-head, row tile) and
-// four of its rows, a warp each; or, SHARE, where there are fewer units than CTAs and
-// hence many parts to each, a CTA per row whose warps share its parts.  (Launched early,
-// to wait on the device for the first kernel's end, the two took 2 us longer.)
-template <int D, int BM, int BN, bool SHARE>
+// Joins the parts of a unit that was cut: a thread per row and 16 columns, threads side
+// by side on rows.  SHARES of them split a row's parts, 8 where there are far fewer units
+// than CTAs and hence many parts to each.  (A warp per row took 11 us instead of 7 for
+// 32 sequences of 6144 positions and 32 nodes; launched early, to wait on the device for
+// the first kernel's end, the two took 2 us longer.)
+template <int D, int BM, int SHARES>
+struct AttnJoin {
+  static constexpr int RT = BM < 128 / SHARES ? BM : 128 / SHARES;   // rows per CTA
+  static constexpr int CG = 128 / SHARES / RT < D / 16 ? 128 / SHARES / RT : D / 16;   // column groups
+  static constexpr int kThreads = SHARES * RT * CG;
+  static constexpr int kBlocksY = BM / RT * (D / 16 / CG);
+  static_assert(D / 16 % CG == 0 && BM % RT == 0, "whole blocks");
+};
+
+template <int D, int BM, int BN, int SHARES>
 __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, int max_row_tiles,
                                                              int grid) {
-  constexpr int CPL = D / 32;                          // columns per lane
-  __shared__ float s_o[SHARE ? 4 : 1][SHARE ? D : 1];
-  __shared__ float2 s_ml[4];
+  using J = AttnJoin<D, BM, SHARES>;
+  __shared__ float s_o[SHARES > 1 ? SHARES : 1][SHARES > 1 ? 17 * J::RT : 1];
+  __shared__ float2 s_ml[SHARES][J::RT];
   const int per_seq = a.HKV * max_row_tiles;
   const int seq = blockIdx.x / per_seq, u = blockIdx.x - seq * per_seq;
   const int64_t base = a.prefix[seq], total = a.prefix[a.n_seqs];
@@ -871,87 +906,78 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
   const int b0 = (int)(((u0 + 1) * ctas - 1) / total), b1 = (int)((u1 * ctas - 1) / total);
   if (b0 == b1) return;
   const int kvh = u / s.row_tiles, rt = u - kvh * s.row_tiles;
-  const int row0 = rt * BM, rows = min(BM, s.n * a.G - row0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = rt * a.tile_rows, rows = min(a.tile_rows, s.n * a.G - row0);
   // the unit is the second part of the CTA it begins in the middle of, the first of all others
   const int64_t part0 = (int64_t)b0 * 2 + (total * b0 / ctas >= u0 ? 0 : 1);
   const int parts = b1 - b0 + 1;
   const auto part = [&](int i) { return (i == 0 ? part0 : (int64_t)(b0 + i) * 2) * BM; };
-  const auto join = [&](int r, int from, int step, float& m, float& l, float(&acc)[CPL]) {
-    // 32 parts' statistics at a time, a lane each
-    m = -INFINITY;
-    l = 0.f;
+
+  const int rr = threadIdx.x % J::RT, rest = threadIdx.x / J::RT;
+  const int share = SHARES > 1 ? rest : 0, cb = blockIdx.y / (BM / J::RT);
+  const int r = (int)(blockIdx.y % (BM / J::RT)) * J::RT + rr;
+  const int col = 16 * (SHARES > 1 ? cb : cb * J::CG + rest);
+  const bool live = r < rows;
+  float m = -INFINITY, l = 0.f, acc[16];
 #pragma unroll
-    for (int e = 0; e < CPL; ++e) acc[e] = 0.f;
-    for (int i0 = from; i0 < parts; i0 += 32 * step) {
-      const int mine = i0 + lane * step;
-      const float2 p = mine < parts ? a.part_ml[part(mine) + r] : make_float2(-INFINITY, 0.f);
-      float top = p.x;
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  if (live) {
+#pragma unroll 4
+    for (int i = share; i < parts; i += SHARES) m = fmaxf(m, a.part_ml[part(i) + r].x);
+    const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll 2
+    for (int i = share; i < parts; i += SHARES) {
+      const float2 p = a.part_ml[part(i) + r];
+      const float4* src = reinterpret_cast<const float4*>(a.part_o + part(i) * D) + col / 4 * BM + r;
+      const float f = ex2(p.x - off);
+      l = fmaf(p.y, f, l);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      top = fmaxf(top, m);
-      const float off = top == -INFINITY ? 0.f : top, old = ex2(m - off), f = ex2(p.x - off);
-      m = top;
-      l = l * old + warp_sum(p.y * f);
-#pragma unroll
-      for (int e = 0; e < CPL; ++e) acc[e] *= old;
-      const int count = min(32, (parts - i0 + step - 1) / step);
-#pragma unroll 8
-      for (int j = 0; j < count; ++j) {
-        const float* src = a.part_o + (part(i0 + j * step) + r) * D + lane;
-        const float fj = __shfl_sync(0xffffffffu, f, j);
-#pragma unroll
-        for (int e = 0; e < CPL; ++e) acc[e] = fmaf(src[32 * e], fj, acc[e]);
+      for (int e = 0; e < 4; ++e) {
+        const float4 v = src[e * BM];
+        acc[e * 4] = fmaf(v.x, f, acc[e * 4]);
+        acc[e * 4 + 1] = fmaf(v.y, f, acc[e * 4 + 1]);
+        acc[e * 4 + 2] = fmaf(v.z, f, acc[e * 4 + 2]);
+        acc[e * 4 + 3] = fmaf(v.w, f, acc[e * 4 + 3]);
       }
-    }
-  };
-  const auto store = [&](int r, float l, const float(&acc)[CPL]) {
-    const float inv = 1.f / l;
-    const int nd = (row0 + r) / a.G;
-    bf16* dst = a.out + ((s.start + nd) * a.HQ + kvh * a.G + row0 + r - nd * a.G) * D + lane;
-#pragma unroll
-    for (int e = 0; e < CPL; ++e) dst[32 * e] = f2bf(acc[e] * inv);
-  };
-  float m, l, acc[CPL];
-  if constexpr (!SHARE) {
-    const int r = blockIdx.y * 4 + warp;
-    if (r < rows) {
-      join(r, 0, 1, m, l, acc);
-      store(r, l, acc);
-    }
-  } else {
-    const int r = blockIdx.y;
-    if (r >= rows) return;
-    join(r, warp, 4, m, l, acc);
-#pragma unroll
-    for (int e = 0; e < CPL; ++e) s_o[warp][lane + 32 * e] = acc[e];
-    if (lane == 0) s_ml[warp] = make_float2(m, l);
-    __syncthreads();
-    if (warp == 0) {
-      m = fmaxf(fmaxf(s_ml[0].x, s_ml[1].x), fmaxf(s_ml[2].x, s_ml[3].x));
-      const float off = m == -INFINITY ? 0.f : m;
-      l = 0.f;
-#pragma unroll
-      for (int e = 0; e < CPL; ++e) acc[e] = 0.f;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float f = ex2(s_ml[v].x - off);
-        l = fmaf(s_ml[v].y, f, l);
-#pragma unroll
-        for (int e = 0; e < CPL; ++e) acc[e] = fmaf(s_o[v][lane + 32 * e], f, acc[e]);
-      }
-      store(r, l, acc);
     }
   }
+  if constexpr (SHARES > 1) {
+    s_ml[share][rr] = make_float2(m, l);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s_o[share][rr * 17 + e] = acc[e];
+    __syncthreads();
+    if (share > 0) return;
+#pragma unroll
+    for (int v = 0; v < SHARES; ++v) m = fmaxf(m, s_ml[v][rr].x);
+    const float off = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int v = 0; v < SHARES; ++v) {
+      const float f = ex2(s_ml[v][rr].x - off);
+      l = fmaf(s_ml[v][rr].y, f, l);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] = fmaf(s_o[v][rr * 17 + e], f, acc[e]);
+    }
+  }
+  if (!live) return;
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] *= inv;
+  const int nd = (row0 + r) / a.G;
+  bf16* dst = a.out + ((s.start + nd) * a.HQ + kvh * a.G + row0 + r - nd * a.G) * D + col;
+  *reinterpret_cast<uint4*>(dst) = pack8(acc);
+  *reinterpret_cast<uint4*>(dst + 8) = pack8(acc + 8);
 }
 
 // Rows per CTA tile, by the rows of the largest tree: 16 or 32 (mma.sync; the traffic
 // bounds them), 128 on tcgen05 from 33 on (32 sequences of 6144 positions and 16 nodes
-// of 4 heads: 116 us with mma.sync at 64 rows, 95 here).  Head dim 256: 64 at most, with mma.sync (128 rows would not fit
-// TMEM and shared memory).  And how many CTAs run.
+// of 4 heads: 116 us with mma.sync at 64 rows, 95 here).  Head dim 256: 64 at most, with
+// mma.sync (128 rows would not fit TMEM and shared memory).  More than 128 heads to a
+// kv-head: a node fills no whole tile, 32.  And how many CTAs run.
 static int attn_rows(int max_nodes, int G, int D) {
   const int rows = max_nodes * G;
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : D == 256 ? 64 : 128;
+  return rows <= 16 ? 16 : D == 256 && rows > 32 ? 64 : rows <= 32 || G > 128 ? 32 : 128;
 }
 static int attn_ctas(int bm, int D) { return kAttnSms * (D <= 128 && bm <= 32 ? 2 : 1); }
 
@@ -971,12 +997,14 @@ static AttnSpace attn_space(int bm, int n_seqs, int D) {
 
 template <int D, int BM, int BN>
 static void launch_join(const AttnArgs& a, int ctas, cudaStream_t s) {
-  const int row_tiles = (a.max_nodes * a.G + BM - 1) / BM;
-  const int rows = row_tiles > 1 ? BM : a.max_nodes * a.G;
-  const bool share = (int64_t)a.n_seqs * a.HKV * row_tiles * 4 < ctas;
-  const dim3 grid((unsigned)(a.n_seqs * a.HKV * row_tiles), (unsigned)(share ? rows : (rows + 3) / 4));
-  if (share) attention_join_kernel<D, BM, BN, true><<<grid, 128, 0, s>>>(a, row_tiles, ctas);
-  else attention_join_kernel<D, BM, BN, false><<<grid, 128, 0, s>>>(a, row_tiles, ctas);
+  const int row_tiles = (a.max_nodes * a.G + a.tile_rows - 1) / a.tile_rows;
+  const int units = a.n_seqs * a.HKV * row_tiles;
+  if ((int64_t)units * 4 < ctas)
+    attention_join_kernel<D, BM, BN, 8>
+        <<<dim3(units, AttnJoin<D, BM, 8>::kBlocksY), AttnJoin<D, BM, 8>::kThreads, 0, s>>>(a, row_tiles, ctas);
+  else
+    attention_join_kernel<D, BM, BN, 1>
+        <<<dim3(units, AttnJoin<D, BM, 1>::kBlocksY), AttnJoin<D, BM, 1>::kThreads, 0, s>>>(a, row_tiles, ctas);
 }
 
 template <int D, int WM, int WN>
@@ -996,8 +1024,8 @@ static int launch_attention(const CUtensorMap& kmap, const CUtensorMap& vmap, co
 }
 
 template <int D>
-static int launch_attention_tc(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttnArgs& a,
-                               cudaStream_t s) {
+static int launch_attention_tc(const CUtensorMap& kmap, const CUtensorMap& vmap,
+                               const CUtensorMap& qmap, const AttnArgs& a, cudaStream_t s) {
   using P = AttnTc<D>;
   constexpr size_t bytes = sizeof(typename P::Smem) + 1024;
   static_assert(bytes + 1024 <= 228 * 1024, "shared memory of one SM");
@@ -1006,7 +1034,7 @@ static int launch_attention_tc(const CUtensorMap& kmap, const CUtensorMap& vmap,
       cudaSuccess)
     return check_launch("gdn_attention_tree");
   const int ctas = attn_ctas(P::BM, D);
-  fn<<<ctas, 352, bytes, s>>>(kmap, vmap, a);
+  fn<<<ctas, 384, bytes, s>>>(kmap, vmap, qmap, a);
   launch_join<D, P::BM, P::BN>(a, ctas, s);
   return check_launch("gdn_attention_tree");
 }
@@ -1063,10 +1091,11 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
                       aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
                   "%s: operands and strides must be 16-byte aligned", fn);
   const int G = num_q_heads / num_kv_heads, bm = attn_rows(max_nodes, G, head_dim);
-  // the scan adds up 32-bit tile counts of up to 352 sequences; TMA coordinates are 32 bits
-  const int row_tiles = (max_nodes * G + bm - 1) / bm;
+  const int tile_rows = bm == 128 ? 128 / G * G : bm;
+  // the scan adds up 32-bit tile counts of up to 384 sequences; TMA coordinates are 32 bits
+  const int row_tiles = (max_nodes * G + tile_rows - 1) / tile_rows;
   GDN_UNSUPPORTED((max_len / 64 + 1ll) * num_kv_heads * row_tiles <= (1ll << 22) &&
-                      num_blocks < (1ll << 31) && max_len <= (1 << 30),
+                      num_blocks < (1ll << 31) && max_len <= (1 << 30) && n_tokens < (1ll << 31),
                   "%s: max_len %d with %d kv heads too large", fn, max_len, num_kv_heads);
   GDN_UNSUPPORTED((int64_t)n_seqs * num_kv_heads * row_tiles < (1ll << 31),
                   "%s: too many sequences or heads", fn);
@@ -1096,7 +1125,7 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
   char* ws = static_cast<char*>(workspace);
   const AttnArgs a{(const bf16*)q, q_row_stride, num_blocks, block_size, box, block_tables,
                    table_stride, max_blocks, context_lens, cu_seqlens, n_seqs, parents, max_nodes,
-                   n_tokens, max_len, (bf16*)out, num_q_heads, num_kv_heads, G,
+                   n_tokens, max_len, (bf16*)out, num_q_heads, num_kv_heads, G, tile_rows,
                    scale * 1.4426950408889634f, reinterpret_cast<int64_t*>(ws + sp.prefix),
                    reinterpret_cast<float*>(ws + sp.part_o),
                    reinterpret_cast<float2*>(ws + sp.part_ml), status};
@@ -1104,15 +1133,22 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
 #define GDN_AT(D)                                                    \
   if (bm == 16) return launch_attention<D, 1, 4>(kmap, vmap, a, s);  \
   if (bm == 32) return launch_attention<D, 2, 2>(kmap, vmap, a, s);
-  if (head_dim == 64) {
-    GDN_AT(64)
-    return launch_attention_tc<64>(kmap, vmap, a, s);
-  }
-  if (head_dim == 128) {
-    GDN_AT(128)
-    return launch_attention_tc<128>(kmap, vmap, a, s);
-  }
-  GDN_AT(256)
+  if (head_dim == 64) { GDN_AT(64) }
+  if (head_dim == 128) { GDN_AT(128) }
+  if (head_dim == 256) { GDN_AT(256) }
 #undef GDN_AT
-  return launch_attention<256, 4, 1>(kmap, vmap, a, s);
+  if (head_dim == 256) return launch_attention<256, 4, 1>(kmap, vmap, a, s);
+  // whole nodes of a group's heads: one box brings a row tile's queries in row order
+  const cuuint64_t qdims[3] = {(cuuint64_t)head_dim, (cuuint64_t)num_q_heads, (cuuint64_t)n_tokens};
+  const cuuint64_t qstrides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)q_row_stride * 2};
+  const cuuint32_t qbox[3] = {64, (cuuint32_t)G, (cuuint32_t)(tile_rows / G)};
+  CUtensorMap qmap;
+  if (encode(&qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), qdims, qstrides, qbox,
+             step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    set_error("%s: the queries' tensor map could not be encoded", fn);
+    return GDN_ERR_CUDA;
+  }
+  return head_dim == 64 ? launch_attention_tc<64>(kmap, vmap, qmap, a, s)
+                        : launch_attention_tc<128>(kmap, vmap, qmap, a, s);
 }
