@@ -321,72 +321,41 @@ __global__ void __launch_bounds__(kConvThreads) conv_state_writeback_kernel(
 // ---------------------------------------------------------------------------
 //
 // y[n] = silu(sum_{i<K} w[K-1-i] * x[i-th ancestor of n]); above the root the
-// stored taps, newest first.  A CTA owns rows_per_cta rows x 512 channels (or
-// 128 unaligned ones); its first warp walks every row's K-1 ancestors once and
-// leaves, per row and tap, the row to read.  Values come from conv_point(), so a
-// chain's rows have the bits of the varlen conv.
+// stored taps, newest first.  A CTA owns a sequence and 256 channels (64 unaligned
+// ones): its rows come into shared memory once, the stored taps behind them as K - 1
+// further rows, so that every tap of every node is a row there and the loop over the
+// nodes has no branch.  The arithmetic is conv_point()'s, so a chain's rows have the
+// bits of the varlen conv.
 //
-// 2 + 2 bytes per element of HBM; the ancestors' rows come from L1 / L2, a row ahead,
-// and without a branch: above the root a row stands in for the stored tap, which the
-// few rows concerned then fetch.  Bound by its instructions (some 20 per output: four
-// rows unpacked, addresses, SiLU): 5.2k rows of 8192 channels take 68 us, floor 27,
-// first form 84.
-constexpr int kTreeConvRows = 16;
+// 2 + 2 bytes per element of HBM; 5.2k rows of 8192 channels in trees of 17 to 64: 56 us,
+// floor 27 (ancestors' rows read through L1 and L2 by 16 rows to a CTA, the stored taps
+// by a branch: 68; 128 threads instead of 256: 63; 128 channels instead of 256: 60).
+// Bound by its instructions, some 22 per output: four rows unpacked, the products, SiLU,
+// and what a thread does once for some ten nodes.
+constexpr int kTreeConvThreads = 256;
 
 template <int K, int V>   // channels per thread: 4 (8-byte accesses) or 1
-__global__ void __launch_bounds__(kConvThreads, 9) conv_tree_kernel(
+__global__ void __launch_bounds__(kTreeConvThreads, 6) conv_tree_kernel(
     const bf16* __restrict__ x, int64_t xs, const bf16* __restrict__ pool, int64_t slot_stride,
     int64_t num_slots, const int64_t* __restrict__ ids, const int32_t* __restrict__ cu,
-    int n_seqs, const int32_t* __restrict__ parents, int max_nodes, int64_t n_tokens, int C,
-    const bf16* __restrict__ w, bf16* __restrict__ y, int64_t ys, int rows_per_cta,
-    int32_t* status, const GateArgs gate) {
-  constexpr int T = K - 1;
-  const int64_t t0 = (int64_t)blockIdx.x * rows_per_cta;
-  const int rows = (int)min((int64_t)rows_per_cta, n_tokens - t0);
-  // per row: its slot (-1: leave the row), how many of its K taps are rows, and
-  // those rows' offsets in x (its own where the root is passed)
-  __shared__ int64_t s_slot[kTreeConvRows];
-  __shared__ int64_t s_src[kTreeConvRows][K];
-  __shared__ int s_found[kTreeConvRows];
-  const int c0 = (blockIdx.y * kConvThreads + threadIdx.x) * V;
-  const bool gate_cta = blockIdx.y == gridDim.y - 1;
-  float wv[V * K];
-  if (!gate_cta && c0 < C) {
-#pragma unroll
-    for (int i = 0; i < V * K; ++i) wv[i] = bf2f(w[(int64_t)c0 * K + i]);
-  }
-  if (threadIdx.x < 32) {
-    int r = warp_seq_of(cu, n_seqs, t0);
-    const int lane = threadIdx.x;
-    if (lane < rows) {
-      const int64_t t = t0 + lane;
-      while (r < n_seqs && (int64_t)cu[r + 1] <= t) ++r;
-      int64_t start = 0, slot = -1;
-      int n = 0;
-      if (r < n_seqs && tree_rows(cu, r, n_tokens, max_nodes, status, start, n) && t >= start &&
-          t < start + n) {
-        slot = ids[r];
-        if (!slot_ok(slot, num_slots, status)) slot = -1;
-        int at = (int)(t - start), found = 0;
-#pragma unroll
-        for (int i = 0; i < K; ++i) {
-          s_src[lane][i] = (at >= 0 ? start + at : t) * xs;
-          found += at >= 0;
-          if (at >= 0) at = i + 1 < K ? tree_parent(parents[start + at], at, status) : -1;
-        }
-        s_found[lane] = found;
-      }
-      s_slot[lane] = slot;
-    }
-  }
-  __syncthreads();
-  if (gate_cta) {
-    const int total = rows * gate.H;
-    for (int i = threadIdx.x; i < total; i += kConvThreads) {
-      const int rr = i / gate.H;
-      if (s_slot[rr] < 0) continue;
-      const int h = i - rr * gate.H;
-      const int64_t t = t0 + rr;
+    const int32_t* __restrict__ parents, int max_nodes, int64_t n_tokens, int C,
+    const bf16* __restrict__ w, bf16* __restrict__ y, int64_t ys, int32_t* status,
+    const GateArgs gate) {
+  constexpr int T = K - 1, CH = 64 * V, RG = kTreeConvThreads / 64;
+  extern __shared__ __align__(16) unsigned char conv_smem[];
+  bf16* const tile = reinterpret_cast<bf16*>(conv_smem);   // [max_nodes + T][CH]
+  __shared__ int s_par[kMaxTreeNodes];
+  __shared__ __align__(16) int s_at[kMaxTreeNodes][4];     // the taps' offsets in tile, newest first
+  const int tid = threadIdx.x, cx = tid & 63, ry = tid >> 6;
+  int64_t start;
+  int n;
+  if (!tree_rows(cu, blockIdx.x, n_tokens, max_nodes, status, start, n) || n == 0) return;
+  const int64_t slot = ids[blockIdx.x];
+  if (!slot_ok(slot, num_slots, status)) return;
+  if (blockIdx.y == gridDim.y - 1) {
+    for (int i = tid; i < n * gate.H; i += kTreeConvThreads) {
+      const int rr = i / gate.H, h = i - rr * gate.H;
+      const int64_t t = start + rr;
       const float al = gate.param_bf16 ? bf2f(static_cast<const bf16*>(gate.a_log)[h])
                                        : static_cast<const float*>(gate.a_log)[h];
       const float db = gate.param_bf16 ? bf2f(static_cast<const bf16*>(gate.dt_bias)[h])
@@ -399,67 +368,76 @@ __global__ void __launch_bounds__(kConvThreads, 9) conv_tree_kernel(
     }
     return;
   }
-  if (c0 >= C) return;
-  if constexpr (V == 1) {
-    for (int rr = 0; rr < rows; ++rr) {
-      if (s_slot[rr] < 0) continue;
-      const bf16* taps = pool + s_slot[rr] * slot_stride + (int64_t)c0 * T;
+
+  const int c0 = blockIdx.y * CH + cx * V;
+  const bool live = c0 < C;
+  const bf16* xp = x + (start + ry) * xs + c0;
+  if (live) {
+    for (int r = ry; r < n; r += RG, xp += RG * xs) {
+      if constexpr (V == 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+                         tc::smem_u32(tile + r * CH + cx * V)),
+                     "l"(xp)
+                     : "memory");
+      else
+        tile[r * CH + cx] = *xp;
+    }
+  }
+  tc::cp_async_commit();
+  if (tid < n) s_par[tid] = tree_parent(parents[start + tid], tid, status);
+  float wv[V * K];
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < V * K; ++i) wv[i] = bf2f(w[(int64_t)c0 * K + i]);
+    const bf16* taps = pool + slot * slot_stride + (int64_t)c0 * T;
+    for (int j = ry; j < T; j += RG)                       // row n + j: the j-th newest
+#pragma unroll
+      for (int e = 0; e < V; ++e) tile[(n + j) * CH + cx * V + e] = taps[e * T + T - 1 - j];
+  }
+  __syncthreads();
+  if (tid < n) {
+    int at = tid, above = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      s_at[tid][i] = (at >= 0 ? at : n + above++) * CH;
+      if (at >= 0) at = s_par[at];
+    }
+  }
+  tc::cp_async_wait<0>();
+  __syncthreads();
+  if (!live) return;
+  const bf16* mine = tile + cx * V;
+  bf16* yp = y + (start + ry) * ys + c0;
+#pragma unroll 2
+  for (int r = ry; r < n; r += RG, yp += RG * ys) {
+    const int4 at4 = *reinterpret_cast<const int4*>(s_at[r]);
+    const int at[4] = {at4.x, at4.y, at4.z, at4.w};
+    if constexpr (V == 1) {
       float wn[K];
 #pragma unroll
-      for (int i = 0; i < K; ++i)
-        wn[T - i] = bf2f(i < s_found[rr] ? x[s_src[rr][i] + c0] : taps[T - 1 - (i - s_found[rr])]);
-      y[(t0 + rr) * ys + c0] = f2bf(conv_point<K>(wn, wv));
-    }
-  } else {
-    const bf16* xc = x + c0;
-    const auto load = [&](int rr, uint2(&raw)[K]) {
-      if (rr < rows && s_slot[rr] >= 0) {
+      for (int i = 0; i < K; ++i) wn[T - i] = bf2f(mine[at[i]]);
+      *yp = f2bf(conv_point<K>(wn, wv));
+    } else {
+      uint2 tap[K], out;
 #pragma unroll
-        for (int i = 0; i < K; ++i) raw[i] = *reinterpret_cast<const uint2*>(xc + s_src[rr][i]);
-      }
-    };
-    uint2 cur[K], nxt[K];
-    load(0, cur);
-    bf16* yp = y + t0 * ys + c0;
-    for (int rr = 0; rr < rows; ++rr, yp += ys) {
-      load(rr + 1, nxt);
-      if (s_slot[rr] >= 0) {
-        const int found = s_found[rr];
-        uint2 out;
-        if (found == K) {
-          // channels in pairs: fma.f32x2 rounds each as conv_point()'s fmaf
-          uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+      for (int i = 0; i < K; ++i) tap[i] = *reinterpret_cast<const uint2*>(mine + at[i]);
+      // channels in pairs: fma.f32x2 rounds each as conv_point()'s fmaf
+      uint32_t* o = reinterpret_cast<uint32_t*>(&out);
 #pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            float a0, a1;
+      for (int p = 0; p < 2; ++p) {
+        float a0, a1;
 #pragma unroll
-            for (int i = K - 1; i >= 0; --i) {         // the oldest first
-              const uint32_t u = p == 0 ? cur[i].x : cur[i].y;
-              const float x0 = __uint_as_float(u << 16), x1 = __uint_as_float(u & 0xffff0000u);
-              const float w0 = wv[2 * p * K + T - i], w1 = wv[(2 * p + 1) * K + T - i];
-              if (i == K - 1) tc::fmul2(a0, a1, x0, x1, w0, w1);
-              else tc::ffma2(a0, a1, x0, x1, w0, w1, a0, a1);
-            }
-            const __nv_bfloat162 b2 = __floats2bfloat162_rn(conv_silu(a0), conv_silu(a1));
-            o[p] = *reinterpret_cast<const uint32_t*>(&b2);
-          }
-        } else {                                       // near the root: stored taps
-          const bf16* taps = pool + s_slot[rr] * slot_stride + (int64_t)c0 * T;
-          bf16* o = reinterpret_cast<bf16*>(&out);
-#pragma unroll
-          for (int ch = 0; ch < V; ++ch) {
-            float wn[K];
-#pragma unroll
-            for (int i = 0; i < K; ++i)
-              wn[T - i] = bf2f(i < found ? reinterpret_cast<const bf16*>(&cur[i])[ch]
-                                         : taps[ch * T + T - 1 - (i - found)]);
-            o[ch] = f2bf(conv_point<K>(wn, wv + ch * K));
-          }
+        for (int i = K - 1; i >= 0; --i) {                 // the oldest first
+          const uint32_t u = p == 0 ? tap[i].x : tap[i].y;
+          const float x0 = __uint_as_float(u << 16), x1 = __uint_as_float(u & 0xffff0000u);
+          const float w0 = wv[2 * p * K + T - i], w1 = wv[(2 * p + 1) * K + T - i];
+          if (i == K - 1) tc::fmul2(a0, a1, x0, x1, w0, w1);
+          else tc::ffma2(a0, a1, x0, x1, w0, w1, a0, a1);
         }
-        *reinterpret_cast<uint2*>(yp) = out;
+        const __nv_bfloat162 b2 = __floats2bfloat162_rn(conv_silu(a0), conv_silu(a1));
+        o[p] = *reinterpret_cast<const uint32_t*>(&b2);
       }
-#pragma unroll
-      for (int i = 0; i < K; ++i) cur[i] = nxt[i];
+      *reinterpret_cast<uint2*>(yp) = out;
     }
   }
 }
@@ -624,23 +602,20 @@ extern "C" int gdn_conv_gate_tree(const void* x, int64_t x_row_stride, const voi
               "%s: null pointer", fn);
   const bool vec = channels % 4 == 0 && x_row_stride % 4 == 0 && y_row_stride % 4 == 0 &&
                    ((uintptr_t)x | (uintptr_t)y) % 8 == 0;
-  const int per_cta = vec ? kConvThreads * 4 : kConvThreads;
-  const unsigned cy = (unsigned)((channels + per_cta - 1) / per_cta) + 1;   // + the gate's row
-  // few rows are spread thin, so that a small call is not one CTA's loop
-  const int64_t thin = n_tokens * cy / (4 * sm_count());
-  const int rows = thin >= kTreeConvRows ? kTreeConvRows : thin < 2 ? 2 : (int)thin;
-  const int64_t tiles = (n_tokens + rows - 1) / rows;
-  GDN_UNSUPPORTED(tiles < (1ll << 31) && cy <= 65535, "%s: too many tokens or channels", fn);
+  const int per_cta = vec ? 256 : 64;
+  const int64_t cy = ((int64_t)channels + per_cta - 1) / per_cta + 1;   // + the gate's
+  GDN_UNSUPPORTED(cy <= 65535, "%s: too many channels", fn);
+  const size_t bytes = (size_t)(max_nodes + kernel - 1) * per_cta * 2;  // 34304 at most
   const GateArgs gate{(const bf16*)b, (const bf16*)a, ab_row_stride, num_v_heads, a_log, dt_bias,
                       param_dtype == GDN_DTYPE_BF16, g, (bf16*)beta};
   cudaStream_t s = (cudaStream_t)stream;
-  const dim3 grid((unsigned)tiles, cy);
+  const dim3 grid((unsigned)n_seqs, (unsigned)cy);
 #define GDN_CT(KK, VV)                                                                        \
   if (kernel == KK && vec == (VV > 1))                                                        \
-    conv_tree_kernel<KK, VV><<<grid, kConvThreads, 0, s>>>(                                   \
+    conv_tree_kernel<KK, VV><<<grid, kTreeConvThreads, bytes, s>>>(                           \
         (const bf16*)x, x_row_stride, (const bf16*)conv_pool, slot_stride, num_slots, ids,    \
-        cu_seqlens, n_seqs, parents, max_nodes, n_tokens, channels, (const bf16*)weight,      \
-        (bf16*)y, y_row_stride, rows, status, gate);
+        cu_seqlens, parents, max_nodes, n_tokens, channels, (const bf16*)weight, (bf16*)y,    \
+        y_row_stride, status, gate);
   GDN_CT(2, 4) GDN_CT(3, 4) GDN_CT(4, 4)
   GDN_CT(2, 1) GDN_CT(3, 1) GDN_CT(4, 1)
 #undef GDN_CT
