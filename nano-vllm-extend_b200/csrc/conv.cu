@@ -327,10 +327,11 @@ __global__ void __launch_bounds__(kConvThreads) conv_state_writeback_kernel(
 // nodes has no branch.  The arithmetic is conv_point()'s, so a chain's rows have the
 // bits of the varlen conv.
 //
-// 2 + 2 bytes per element of HBM; 5.2k rows of 8192 channels in trees of 17 to 64: 56 us,
+// 2 + 2 bytes per element of HBM; 5.2k rows of 8192 channels in trees of 17 to 64: 52 us,
 // floor 27 (ancestors' rows read through L1 and L2 by 16 rows to a CTA, the stored taps
-// by a branch: 68; 128 threads instead of 256: 63; 128 channels instead of 256: 60).
-// Bound by its instructions, some 22 per output: four rows unpacked, the products, SiLU,
+// by a branch: 68; 128 threads instead of 256 took 6 us more, 128 channels 4, eight
+// channels to a thread 14; weights and taps by single elements 4).
+// Bound by its instructions, some 20 per output: four rows unpacked, the products, SiLU,
 // and what a thread does once for some ten nodes.
 constexpr int kTreeConvThreads = 256;
 
@@ -385,14 +386,30 @@ __global__ void __launch_bounds__(kTreeConvThreads, 6) conv_tree_kernel(
   }
   tc::cp_async_commit();
   if (tid < n) s_par[tid] = tree_parent(parents[start + tid], tid, status);
+  // V channels' weights, and their stored taps (row n + j of the tile: the j-th newest),
+  // lie side by side: whole words of V elements
+  struct __align__(2 * V) Word { bf16 e[V]; };
   float wv[V * K];
   if (live) {
+    const Word* wp = reinterpret_cast<const Word*>(w + (int64_t)c0 * K);
 #pragma unroll
-    for (int i = 0; i < V * K; ++i) wv[i] = bf2f(w[(int64_t)c0 * K + i]);
-    const bf16* taps = pool + slot * slot_stride + (int64_t)c0 * T;
-    for (int j = ry; j < T; j += RG)                       // row n + j: the j-th newest
+    for (int i = 0; i < K; ++i) {
+      const Word u = wp[i];
 #pragma unroll
-      for (int e = 0; e < V; ++e) tile[(n + j) * CH + cx * V + e] = taps[e * T + T - 1 - j];
+      for (int e = 0; e < V; ++e) wv[i * V + e] = bf2f(u.e[e]);
+    }
+    if (ry == RG - 1) {
+      const Word* sp = reinterpret_cast<const Word*>(pool + slot * slot_stride + (int64_t)c0 * T);
+      Word old[T], row;
+#pragma unroll
+      for (int i = 0; i < T; ++i) old[i] = sp[i];
+#pragma unroll
+      for (int j = 0; j < T; ++j) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) row.e[e] = old[(e * T + T - 1 - j) / V].e[(e * T + T - 1 - j) % V];
+        *reinterpret_cast<Word*>(tile + (n + j) * CH + cx * V) = row;
+      }
+    }
   }
   __syncthreads();
   if (tid < n) {
@@ -600,8 +617,8 @@ extern "C" int gdn_conv_gate_tree(const void* x, int64_t x_row_stride, const voi
   GDN_REQUIRE(x && conv_pool && ids && cu_seqlens && parents && weight && y && b && a && a_log &&
                   dt_bias && g && beta,
               "%s: null pointer", fn);
-  const bool vec = channels % 4 == 0 && x_row_stride % 4 == 0 && y_row_stride % 4 == 0 &&
-                   ((uintptr_t)x | (uintptr_t)y) % 8 == 0;
+  const bool vec = (channels | x_row_stride | y_row_stride | slot_stride) % 4 == 0 &&
+                   ((uintptr_t)x | (uintptr_t)y | (uintptr_t)conv_pool | (uintptr_t)weight) % 8 == 0;
   const int per_cta = vec ? 256 : 64;
   const int64_t cy = ((int64_t)channels + per_cta - 1) / per_cta + 1;   // + the gate's
   GDN_UNSUPPORTED(cy <= 65535, "%s: too many channels", fn);
