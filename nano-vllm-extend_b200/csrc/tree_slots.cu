@@ -31,6 +31,12 @@ __global__ void __launch_bounds__(kSlotThreads) tree_slot_kernel(
     const int64_t t = t0 - HALO + i;
     s_par[i] = t >= 0 && t < n_rows ? parents[t] : -1;
   }
+  if (blockIdx.x == 0) {            // malformed sequences are flagged even where no row finds them
+    int64_t at;
+    int m;
+    for (int i = threadIdx.x; i < n_seqs; i += kSlotThreads)
+      tree_rows(cu, i, n_rows, max_nodes, status, at, m);
+  }
   int r = warp_seq_of(cu, n_seqs, t0 + (threadIdx.x & ~31));
   const int64_t t = t0 + threadIdx.x;
   while (r < n_seqs && (int64_t)cu[r + 1] <= t) ++r;

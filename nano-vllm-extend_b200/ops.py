@@ -179,13 +179,16 @@ def set_debug_checks(on: bool) -> None:
     _DEBUG_CHECKS = bool(on)
 
 
-def check_slot_ids(ids, num_slots: int) -> None:
-    """Raise IndexError for a slot id outside [0, num_slots) and ValueError
-    for a slot id given more than once (the last slot excepted)."""
+def check_slot_ids(ids, num_slots: int, shared: bool = False) -> None:
+    """Raise IndexError for a slot id outside [0, num_slots) and, unless ``shared``
+    (the call only reads the slots), ValueError for a slot id given more than once
+    (the last slot excepted)."""
     v = np.asarray(ids.cpu() if isinstance(ids, torch.Tensor) else ids, np.int64).reshape(-1)
     bad = (v < 0) | (v >= num_slots)
     if bad.any():
         raise IndexError(f"slot id {int(v[bad][0])} outside the pool of {num_slots} slots")
+    if shared:
+        return
     u, n = np.unique(v[v != num_slots - 1], return_counts=True)
     if (n > 1).any():
         raise ValueError(f"slot id {int(u[n > 1][0])} appears {int(n[n > 1][0])} times in "
@@ -233,11 +236,11 @@ def _debug_tree(tree, n_rows: int, accepted=None) -> None:
 
 
 def _debug_checks(ids=None, num_slots: int = 0, cu=None, n_rows: int = 0,
-                  max_seqlen: int | None = None) -> None:
+                  max_seqlen: int | None = None, shared: bool = False) -> None:
     if not _DEBUG_CHECKS or torch.cuda.is_current_stream_capturing():
         return
     if ids is not None:
-        check_slot_ids(ids, num_slots)
+        check_slot_ids(ids, num_slots, shared)
     if cu is not None:
         check_cu_seqlens(cu, n_rows, max_seqlen)
 
@@ -806,7 +809,7 @@ def conv_gate_tree(x: torch.Tensor, state_pool: torch.Tensor, ids: torch.Tensor,
     if not (a_log.is_contiguous() and dt_bias.is_contiguous()):
         a_log, dt_bias = a_log.contiguous(), dt_bias.contiguous()
     if _DEBUG_CHECKS:
-        _debug_checks(ids, state_pool.shape[0])
+        _debug_checks(ids, state_pool.shape[0], shared=True)
         _debug_tree(tree, N)
     y = torch.empty(N, C, dtype=torch.bfloat16, device=dev)
     g = torch.empty(N, vh, dtype=torch.float32, device=dev)
@@ -829,10 +832,7 @@ def _delta_args(k, v, g, beta, s_pool, ids):
     assert g.dtype == torch.float32 and beta.dtype == torch.bfloat16 and g.is_contiguous() and \
         beta.is_contiguous(), "g (fp32) / beta (bf16) must be contiguous"
     _state_view_check(s_pool, HV, DK, DV)
-    ids = _ids64(ids)
-    if _DEBUG_CHECKS:
-        _debug_checks(ids, s_pool.shape[0])
-    return N, HK, HV, DK, DV, ks, vs, ids
+    return N, HK, HV, DK, DV, ks, vs, _ids64(ids)
 
 
 def gated_delta_rule_tree(q, k, v, g, beta, s_pool, ids, cu_seqlens, parents, max_nodes: int,
@@ -851,6 +851,7 @@ def gated_delta_rule_tree(q, k, v, g, beta, s_pool, ids, cu_seqlens, parents, ma
     n_seqs = ids.numel()
     tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, N)
     if _DEBUG_CHECKS:
+        _debug_checks(ids, s_pool.shape[0], shared=True)
         _debug_tree(tree, N)
     if not _aligned_rows(v, vs, 4):
         v, vs = v.clone(memory_format=torch.contiguous_format), HV * DV
@@ -883,7 +884,8 @@ def commit_tree(x, k, v, g, beta, conv_pool, s_pool, ids, cu_seqlens, parents, m
     :func:`recurrent_gdn_inplace` would one after the other (k, v, g, beta as given
     to :func:`gated_delta_rule_tree`); ``conv_pool[ids[r]]`` keeps the last K - 1 of
     its window and the path's rows of ``x`` [N, C], the input of
-    :func:`conv_gate_tree`.  Both pools are updated in place."""
+    :func:`conv_gate_tree`.  Both pools are updated in place, so no slot may be
+    named twice (the two reading operators allow it)."""
     dev = _one_device(x, k, v, g, beta, conv_pool, s_pool, ids, cu_seqlens, parents, accepted)
     N, HK, HV, DK, DV, ks, vs, ids = _delta_args(k, v, g, beta, s_pool, ids)
     C = x.shape[-1]
@@ -897,6 +899,7 @@ def commit_tree(x, k, v, g, beta, conv_pool, s_pool, ids, cu_seqlens, parents, m
     tree = _tree(cu_seqlens, parents, max_nodes, n_seqs, N)
     accepted = _int32(accepted, n_seqs, "accepted")
     if _DEBUG_CHECKS:
+        _debug_checks(ids, s_pool.shape[0])
         _debug_tree(tree, N, accepted)
     _launch("gdn_commit_tree", dev, x.data_ptr(), xs, k.data_ptr(), ks, v.data_ptr(), vs,
             g.data_ptr(), beta.data_ptr(), conv_pool.data_ptr(), _slot_stride(conv_pool), C, K,
@@ -962,7 +965,8 @@ def qk_norm_rope_cache(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache,
     hybrid model's norms); cos_sin fp32 [positions, R], R / 2 cosines then R / 2
     sines: the first R elements of a head are rotated by halves; positions [N] int64;
     k_cache / v_cache bf16 [blocks, block_size, HKV, D] (equal strides, dense heads),
-    written at slot_mapping [N] (block * block_size + token, -1: not stored).
+    written at slot_mapping [N] (block * block_size + token, -1: not stored; of rows
+    that name one slot any may stay).
     Returns the rotated queries [N, HQ, D]; fp32 up to the one rounding at the end."""
     dev = _one_device(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache,
                       slot_mapping)

@@ -57,6 +57,28 @@ def test_malformed_cu_seqlens(ops, cu, bad):  # noqa: F811
     flagged(ops, ValueError)
 
 
+@pytest.mark.parametrize("cu", [c for c, _ in BAD_CU])
+def test_every_operator_flags_malformed_cu_seqlens(ops, cu):  # noqa: F811
+    c = Gdn(1, 2, 64, [4, 5, 3, 0], seed=3)
+    tree = (i32(cu), c.d_par, 5)
+    kc, vc = (torch.zeros(8, 16, 1, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    q, table, ctx = c.d_v[:, :2].contiguous(), i32(np.arange(8).reshape(4, 2)), i32([0] * 4)
+    calls = [
+        lambda: ops.conv_gate_tree(c.d_x, c.d_conv[:, 1], c.d_ids, bf(c.w), *tree, c.d_b, c.d_a,
+                                   f32(c.a_log), f32(c.dt)),
+        lambda: ops.gated_delta_rule_tree(c.d_q, c.d_k, c.d_v, c.d_g, c.d_beta, c.d_pool[:, 1],
+                                          c.d_ids, *tree),
+        lambda: ops.commit_tree(c.d_x, c.d_k, c.d_v, c.d_g, c.d_beta, c.d_conv[:, 1], c.d_pool[:, 1],
+                                c.d_ids, *tree, i32([0, 0, 0, -1])),
+        lambda: ops.tree_slot_map(table, ctx, *tree, 16, c.N),
+        lambda: ops.attention_tree(q, kc, vc, table, ctx, *tree, 32),
+        lambda: ops.attention_tree(q.repeat(1, 8, 1), kc, vc, table, ctx, *tree, 32),
+    ]
+    for call in calls:
+        call()
+        flagged(ops, ValueError)
+
+
 @pytest.mark.parametrize("row,parent", [(2, 2), (1, 7), (3, -5), (0, 0), (4, 1 << 30), (3, -(1 << 31))])
 def test_malformed_parents(ops, row, parent):  # noqa: F811
     lens = [5, 20, 6]

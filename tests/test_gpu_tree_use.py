@@ -201,3 +201,14 @@ def test_a_slot_named_twice_is_read_twice(ops):  # noqa: F811
     assert torch.equal(both[:6], alone[:6])
     c.d_ids[0] = c.d_ids[1] = c.ids[1]
     assert torch.equal(c.delta(ops, False)[6:], alone[6:])
+    ops.set_debug_checks(True)                          # (they let the pool's last slot be named twice)
+    try:
+        c.d_ids[:] = 0
+        c.delta(ops, False)
+        with pytest.raises(ValueError, match="appears 2 times"):
+            c.commit(ops, [1, 1])
+        c.d_ids[1] = -1
+        with pytest.raises(IndexError):
+            c.delta(ops, False)
+    finally:
+        ops.set_debug_checks(False)
