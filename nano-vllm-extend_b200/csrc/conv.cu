@@ -327,13 +327,22 @@ __global__ void __launch_bounds__(kConvThreads) conv_state_writeback_kernel(
 // nodes has no branch.  The arithmetic is conv_point()'s, so a chain's rows have the
 // bits of the varlen conv.
 //
-// 2 + 2 bytes per element of HBM; 5.2k rows of 8192 channels in trees of 17 to 64: 52 us,
+// 2 + 2 bytes per element of HBM; 5.2k rows of 8192 channels in trees of 17 to 64: 50 us,
 // floor 27 (ancestors' rows read through L1 and L2 by 16 rows to a CTA, the stored taps
 // by a branch: 68; 128 threads instead of 256 took 6 us more, 128 channels 4, eight
-// channels to a thread 14; weights and taps by single elements 4).
+// channels to a thread 14; weights and taps by single elements 4, conv_silu() 3).
 // Bound by its instructions, some 20 per output: four rows unpacked, the products, SiLU,
 // and what a thread does once for some ten nodes.
 constexpr int kTreeConvThreads = 256;
+
+// a / (1 + 2^(-a log2 e)) by the hardware's power and reciprocal, subnormals taken as
+// zero: nothing of that size survives the sum with 1, so the results are conv_silu()'s.
+__device__ __forceinline__ float tree_silu(float a) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return a * r;
+}
 
 template <int K, int V>   // channels per thread: 4 (8-byte accesses) or 1
 __global__ void __launch_bounds__(kTreeConvThreads, 6) conv_tree_kernel(
@@ -451,7 +460,7 @@ __global__ void __launch_bounds__(kTreeConvThreads, 6) conv_tree_kernel(
           if (i == K - 1) tc::fmul2(a0, a1, x0, x1, w0, w1);
           else tc::ffma2(a0, a1, x0, x1, w0, w1, a0, a1);
         }
-        const __nv_bfloat162 b2 = __floats2bfloat162_rn(conv_silu(a0), conv_silu(a1));
+        const __nv_bfloat162 b2 = __floats2bfloat162_rn(tree_silu(a0), tree_silu(a1));
         o[p] = *reinterpret_cast<const uint32_t*>(&b2);
       }
       *reinterpret_cast<uint2*>(yp) = out;
