@@ -1111,12 +1111,16 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
   const cuuint64_t strides[3] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2,
                                  (cuuint64_t)block_stride * 2};
   const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, step[4] = {1, 1, 1, 1};
+  // fetches into L2 no wider than a position's head: with 256 bytes, head dim 64 read half of
+  // its neighbour heads' data too, long before they were wanted (444 MB where 302 are needed)
+  const auto promotion = head_dim == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                        : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
   CUtensorMap kmap, vmap;
   const auto make = [&](CUtensorMap* m, const void* p) {
     return encode != nullptr &&
            encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, boxes,
-                  step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                  step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promotion,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
   if (!make(&kmap, k_cache) || !make(&vmap, v_cache)) {
     set_error("%s: the caches' tensor maps could not be encoded", fn);
