@@ -1019,7 +1019,7 @@ static int launch_attention(const CUtensorMap& kmap, const CUtensorMap& vmap, co
     return check_launch("gdn_attention_tree");
   const int ctas = attn_ctas(P::BM, D);
   fn<<<ctas, 32 * (P::NC + 1), bytes, s>>>(kmap, vmap, a);
-  launch_join<D, P::BM, P::BN>(a, ctas, s);
+  if (a.max_len > P::BN) launch_join<D, P::BM, P::BN>(a, ctas, s);   // else no unit is cut
   return check_launch("gdn_attention_tree");
 }
 
@@ -1035,7 +1035,7 @@ static int launch_attention_tc(const CUtensorMap& kmap, const CUtensorMap& vmap,
     return check_launch("gdn_attention_tree");
   const int ctas = attn_ctas(P::BM, D);
   fn<<<ctas, 384, bytes, s>>>(kmap, vmap, qmap, a);
-  launch_join<D, P::BM, P::BN>(a, ctas, s);
+  if (a.max_len > P::BN) launch_join<D, P::BM, P::BN>(a, ctas, s);   // else no unit is cut
   return check_launch("gdn_attention_tree");
 }
 

@@ -720,28 +720,29 @@ def decode_fused(mixed: torch.Tensor, z: torch.Tensor, b: torch.Tensor, a: torch
 def _launch(name: str, device: torch.device, *args) -> None:
     """Call entry point ``name`` with its device's status word and current stream,
     on that device."""
-    fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, status_word(device).data_ptr(), _stream_ptr(device))
+    fn, idx = getattr(_lib.load(), name), device.index
+    st = _STATUS.get(idx)
+    if st is None:
+        st = status_word(device)
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    if idx == torch._C._cuda_getDevice():
+        rc = fn(*args, st.data_ptr(), stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, status_word(device).data_ptr(), _stream_ptr(device))
+            rc = fn(*args, st.data_ptr(), stream)
     if rc:
         _lib.check(rc, name)
 
 
 def _one_device(*ts) -> torch.device:
-    idx = ts[0].get_device()
-    for t in ts:
-        if t is not None and t.get_device() != idx:
-            idx = -1
-    assert idx >= 0, "GDN operators take CUDA tensors of one device"
+    where = {t.get_device() for t in ts if t is not None}
+    assert len(where) == 1 and -1 not in where, "GDN operators take CUDA tensors of one device"
     return ts[0].device
 
 
 def _int32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    assert t.dim() == 1 and t.numel() == n, f"{name} must have {n} entries"
-    if t.dtype != torch.int32 or not t.is_contiguous():
+    assert t.shape == (n,), f"{name} must have {n} entries"
+    if t.dtype is not torch.int32 or not t.is_contiguous():
         assert not t.is_floating_point(), f"{name} must hold integers"
         t = t.to(torch.int32).contiguous()
     return t

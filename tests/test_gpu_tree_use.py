@@ -212,3 +212,16 @@ def test_a_slot_named_twice_is_read_twice(ops):  # noqa: F811
             c.delta(ops, False)
     finally:
         ops.set_debug_checks(False)
+
+
+@pytest.mark.parametrize("D,HQ", [(128, 2), (128, 8), (64, 2), (256, 4)])
+@pytest.mark.parametrize("most", [64, 65, 128, 129])
+def test_attention_within_one_tile(ops, D, HQ, most):  # noqa: F811
+    """Bounds around one tile of positions, where no joining launch follows."""
+    ctx, lens = [most - 9, 0, 30, 11], [9, 1, 0, 6]
+    c, trees = Paged(1, D, 32, ctx, lens, most), R.make_trees(lens, 5)
+    assert c.most == most
+    q = rnd(np.random.default_rng(most), sum(lens), HQ, D)
+    ref, size = R.attention(q, c.ks, c.vs, ctx, trees, D ** -0.5)
+    attn_close(attend(ops, c, bf(q), lens, trees), ref, size)
+    assert ops.check_status() == 0
