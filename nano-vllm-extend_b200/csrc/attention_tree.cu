@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(384, 1)
           if (row < rows) anc = sm.anc[segs & 1][node];
           wait(sm.full[T % ST], (T / ST) & 1);
           unsigned char* vt = &sm.kv[T % ST][1][0][0];
-#pragma unroll 1
+#pragma unroll 4
           for (int i = r; i < BN * (D / 8); i += 128) {
             const int vrow = i / (D / 8), c = i - vrow * (D / 8), j = p_tile + vrow - s.ctx;
             if (j < 0) continue;
