@@ -559,17 +559,19 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
 // mma.sync reaches a quarter of the tensor cores' rate, and 128 rows need 64 products
 // per byte: with it, 32 trees of 16 to 32 nodes over 4 to 8 thousand positions took
 // 214 us against 62 of memory traffic.  Here S = Q K^T (128 x 64) and O += P V (128 x D)
-// are issued by a thread each, from shared memory into TMEM; two groups of four warps, a thread
-// per row, take the tiles in turn: read S (no exchange between lanes), write P as bf16
-// into shared memory and correct O.  Each group has its own S, P, running maximum, sum
+// are issued by a thread each, from shared memory into TMEM; two groups of four warps, a
+// thread per row, take the tiles in turn: read S (no exchange between lanes), write P as
+// bf16 into shared memory and correct O.  Each group has its own S, P, running maximum, sum
 // and O, joined at the end of a segment, so that the two chains of a tile (product,
 // softmax, product) never wait for one another (one group and one issuing thread: 144
 // us).  The TMA producer keeps ST - 1 further tiles under way, and one more warp brings the
 // next segment's queries (a box of whole nodes' heads) and its nodes' ancestors: what a
 // segment does once is what is left above the memory traffic (queries through registers
-// when the segment began: 105 us, now 90; a longer context costs 6.3 TB/s).  O is corrected only when a row's maximum has
-// grown by more than 2^8 since its last correction: until then its probabilities are
-// measured against the older maximum, which the final division cancels.
+// when the segment began: 105 us, now 90; a longer context costs 6.3 TB/s).
+//
+// O is corrected only when a row's maximum has grown by more than 2^8 since its last
+// correction: until then its probabilities are measured against the older maximum, which
+// the final division cancels.
 // ---------------------------------------------------------------------------
 template <int D>
 struct AttnTc {
