@@ -414,11 +414,11 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
     if constexpr (ST == GROUPS) fetch(i + ST, nxt);
     else fetch(i + ST, unit_of(i + ST, at_nxt.step(ST - GROUPS, a.HV), raw_of(at_nxt.step(ST - GROUPS, a.HV)), nullptr));
   };
+  int turn = 0;                                      // units computed: an empty one holds no warp up
   for (int i = group; i < count; i += GROUPS) {
     const DeltaAt at_after = at_nxt.step(GROUPS, a.HV);
     if (at_after.seq != at_nxt.seq) after = raw_of(at_after);
     const int n = cur.n;
-    int* par = gs.par[(i / GROUPS) & 1];
     if (n == 0) {                                    // nothing to compute: the buffer is free at once
       if (tid == 0) {
         await_state(i);
@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
       if constexpr (NORM) copy_vals(1, a.z, a.zs, nxt);
       tc::cp_async_commit();
     } else {
+      int* par = gs.par[turn++ & 1];
       for (int j = tid; j < TN * (TN + 1); j += NT) (&gs.dec[0][0])[j] = 0.f;
       if (tid < TN) {
         const bool on = tid < n;
