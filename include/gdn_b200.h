@@ -329,7 +329,11 @@ int gdn_decode_fused_static(const void* mixed, int64_t mixed_row_stride,
  *    is flagged GDN_STATUS_BAD_TREE, outputs of its sequence are then
  *    unspecified and its state is left alone.  Nothing is read out of bounds.
  *  - A row that holds NaN or infinities makes its own outputs and its
- *    descendants' NaN (or infinite), never those of other nodes.
+ *    descendants' NaN (or infinite), never those of other nodes: in the conv the
+ *    channel that holds them; in the delta rule without the norm the value column
+ *    of an element of v, or of a state's column that holds them, and every column
+ *    of the heads for those of q, k, g and beta; in attention the kv-head's
+ *    query heads, whole.
  */
 
 /*

@@ -40,10 +40,11 @@
 // instructions per warp and unit, most of them the same in every warp: hence few
 // warps per unit, with 32 columns each).
 //
-// A node whose own d is not finite (a NaN or infinity in its row) must not reach
-// nodes that do not descend from it: zero coefficients would still turn it into
-// NaN, so its d is set to zero for the products and its own and its descendants'
-// outputs are set to NaN at the end.
+// A d that is not finite (a NaN or infinity in the node's row, in the state, or past
+// the largest value) must not reach nodes that do not descend from it: zero
+// coefficients would still turn it into NaN, so it is set to zero for the products and
+// the outputs of its node and the node's descendants are set to NaN, in its value
+// column alone, as the recurrence has it.
 #include "mma_util.cuh"
 #include "tc_util.cuh"
 #include "tmap.cuh"
@@ -137,7 +138,8 @@ __device__ __forceinline__ void solve8(float (&r)[MT][4], const float* at, int l
   }
 }
 
-// The same with nodes taken out whose d is not finite; returns them as bits.
+// The same with what is not finite taken out; returns it as bits, the first column's
+// eight nodes, then the second's.
 template <int AP>
 __device__ __noinline__ unsigned solve8_guarded(float4& s, const float* at, int lane) {
   unsigned bad = 0;
@@ -146,13 +148,15 @@ __device__ __noinline__ unsigned solve8_guarded(float4& s, const float* at, int 
     const int from = (lane & ~3) | (i >> 1);
     float x = __shfl_sync(0xffffffffu, i & 1 ? s.y : s.x, from);
     float y = __shfl_sync(0xffffffffu, i & 1 ? s.w : s.z, from);
-    if (!(fabsf(x) <= 3.0e38f && fabsf(y) <= 3.0e38f)) {
+    if (!isfinite(x)) {
       bad |= 1u << i;
-      x = y = 0.f;
-      if (lane == from) {
-        if (i & 1) s.y = s.w = 0.f;
-        else s.x = s.z = 0.f;
-      }
+      x = 0.f;
+      if (lane == from) (i & 1 ? s.y : s.x) = 0.f;
+    }
+    if (!isfinite(y)) {
+      bad |= 256u << i;
+      y = 0.f;
+      if (lane == from) (i & 1 ? s.w : s.z) = 0.f;
     }
     const float2 a = *reinterpret_cast<const float2*>(at + i * AP + 2 * (lane & 3));
     s.x = fmaf(a.x, x, s.x);
@@ -161,6 +165,14 @@ __device__ __noinline__ unsigned solve8_guarded(float4& s, const float* at, int 
     s.w = fmaf(a.y, y, s.w);
   }
   return bad;
+}
+
+// The nodes of block `blk` (of eight) on the path of `node`, as bits.
+__device__ __noinline__ unsigned path_in_block(const int* par, int node, int blk) {
+  unsigned on = 0;
+  for (int j = node; j >= blk * 8; j = par[j])
+    if (j < blk * 8 + 8) on |= 1u << (j - blk * 8);
+  return on;
 }
 
 struct DeltaArgs {
@@ -578,7 +590,6 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
       tc::cp_async_commit();
       group_sync();                                  // the factors are complete
 
-      unsigned long long bad = 0;
 #pragma unroll
       for (int blk = 0; blk < KT; ++blk) {
         if (blk * 8 < n) {
@@ -591,16 +602,28 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
           for (int e = 0; e < 4 * MT; ++e) size += fabsf(r[e / 4][e % 4]);
           // not finite where a part is not (or where the sum ran over)
           if (__any_sync(0xffffffffu, !(size <= 3.0e38f))) {
+            unsigned bad[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               float4 t = make_float4(s[mt][0], s[mt][1], s[mt][2], s[mt][3]);
-              bad |= (unsigned long long)solve8_guarded<P::AP>(t, &gs.at[blk * 8][blk * 8], lane)
-                     << (blk * 8);
+              bad[mt] = solve8_guarded<P::AP>(t, &gs.at[blk * 8][blk * 8], lane);
               r[mt][0] = t.x;
               r[mt][1] = t.y;
               r[mt][2] = t.z;
               r[mt][3] = t.w;
             }
+            // (a sum in an accumulator that is NaN stays NaN)
+#pragma unroll
+            for (int t8 = blk; t8 < KT; ++t8)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const unsigned on = path_in_block(par, t8 * 8 + 2 * tq + e, blk);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  if (bad[mt] & on) acc[KT + t8][mt][e] = __int_as_float(0x7fffffff);
+                  if (bad[mt] >> 8 & on) acc[KT + t8][mt][2 + e] = __int_as_float(0x7fffffff);
+                }
+              }
           }
           // this block's d as an A operand, into the later blocks and the outputs
           uint32_t hi[MT][4], lo[MT][4];
@@ -632,22 +655,6 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
           }
         }
       }
-      if (__any_sync(0xffffffffu, bad != 0)) {
-        bad = (unsigned long long)__reduce_or_sync(0xffffffffu, (unsigned)(bad >> 32)) << 32 |
-              __reduce_or_sync(0xffffffffu, (unsigned)bad);
-#pragma unroll
-        for (int t8 = 0; t8 < KT; ++t8)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            for (int j = t8 * 8 + 2 * tq + e; j >= 0; j = par[j])
-              if (bad >> j & 1) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-                  acc[KT + t8][mt][e] = acc[KT + t8][mt][2 + e] = __int_as_float(0x7fffffff);
-                break;
-              }
-      }
-
       if constexpr (NORM) {
 #pragma unroll
         for (int t8 = 0; t8 < KT; ++t8)

@@ -6,6 +6,7 @@ Finite outputs: the tolerances of test_gpu_tree.py.
 """
 import numpy as np
 import pytest
+import torch
 
 import _tree_reference as R
 from test_gpu_tree import Gdn, close, host, ops  # noqa: F401
@@ -20,6 +21,55 @@ def check(got, ref, hit):
     fine = ~hit
     assert np.isfinite(got[fine]).all(), f"{(~np.isfinite(got[fine])).sum()} elements too many"
     close(np.where(hit, ref, got), ref, 2.0 ** -12)
+
+
+def descendants(c, r, node):
+    """Rows of the batch that see node `node` of sequence r."""
+    start = sum(c.lens[:r])
+    rows = np.zeros(c.N, bool)
+    for i, par in enumerate(c.trees[r]):
+        rows[start + i] = node in R.ancestors(c.trees[r], i)
+    return rows
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("HV,D,n", [(2, 128, 7), (4, 64, 8), (2, 64, 15), (2, 128, 30), (2, 64, 64),
+                                    (1, 128, 64)])
+def test_one_element_of_a_value(ops, HV, D, n, bad):  # noqa: F811
+    c = Gdn(1, HV, D, [3, n, 2], seed=n, wide=3)
+    ref, hit = c.delta_ref(False), np.zeros((c.N, HV, D), bool)
+    for node, h, col in ((1, 0, 5), (n // 2, HV - 1, D - 1), (n - 1, 0, D // 2)):
+        c.d_v[3 + node, h, col] = bad
+        hit[:, h, col] |= descendants(c, 1, node)
+    check(c.delta(ops, False), ref, hit)
+    assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("D,n", [(128, 7), (64, 16), (128, 30), (64, 40), (128, 64)])
+def test_one_element_of_a_state(ops, D, n, bad):  # noqa: F811
+    c = Gdn(1, 2, D, [3, n, 2], seed=n, wide=3)
+    ref, hit = c.delta_ref(False), np.zeros((c.N, 2, D), bool)
+    c.d_pool[c.ids[1], 1, 1, 9, 3] = bad
+    hit[3:3 + n, 1, 3] = True
+    check(c.delta(ops, False), ref, hit)
+
+
+def test_large_finite_updates_stay(ops):  # noqa: F811
+    """An update near the type's largest value is finite, and so are the outputs that a small
+    decay or write strength leaves of it."""
+    c = Gdn(1, 2, 64, [3], seed=1, chain=True)
+    kd = 2 * 64
+    c.y[:, kd:] = 0.0
+    c.y[0, kd] = 3.2e38
+    c.y[0] = torch.from_numpy(c.y[0]).to(torch.bfloat16).double().numpy()
+    c.beta[0] = 1.0
+    c.g[1:] = -40.0
+    c.upload()
+    got = host(c.delta(ops, False))
+    ref = c.delta_ref(False)
+    assert np.isfinite(ref).all() and np.isfinite(got).all()
+    close(got, ref, 2.0 ** -12)
 
 
 @pytest.mark.parametrize("D,n,groups", [(128, 8, 3), (128, 16, 2), (128, 30, 2), (128, 64, 1), (64, 8, 4),
