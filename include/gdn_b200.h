@@ -437,7 +437,8 @@ int gdn_qk_norm_rope_cache(const void* q, int64_t q_row_stride,
  * rows of max_blocks pages (row stride table_stride); context_lens: int32
  * [n_seqs]; max_len bounds context_lens[r] + the sequence's rows, a longer one
  * is skipped and flagged GDN_STATUS_BAD_SEQLEN.  A page outside the cache is
- * flagged GDN_STATUS_BAD_SLOT, never read.  scores are scaled by `scale` > 0.
+ * flagged GDN_STATUS_BAD_SLOT, never read, and all outputs of its sequence are NaN.
+ * scores are scaled by `scale` > 0.
  * out: bf16 [n_tokens, num_q_heads, head_dim].  head_dim 64, 128 or 256.
  * workspace: device scratch of gdn_attention_tree_workspace_bytes() bytes,
  * 16-byte aligned, used only during the call.

@@ -27,7 +27,8 @@
 // In the tiles that hold nodes or reach behind them, value rows behind the last node
 // are zeroed in shared memory, and so are nodes' rows that are not finite, which must
 // not reach nodes off their path (probability zero times NaN); the nodes that do see
-// one of those get NaN outputs.
+// one of those get NaN outputs.  So does a whole sequence with a missing page, whose
+// positions hold whatever tile stood in shared memory before.
 #include "mma_util.cuh"
 #include "tc_util.cuh"
 #include "tmap.cuh"
@@ -160,18 +161,21 @@ __device__ __forceinline__ bool attn_run(const AttnArgs& a, AttnScan& sc, int64_
 
 // The producer warp's part of a segment: `seg` tiles from tile0 on into the ring of
 // stages (tile number `it` of this CTA comes first).  A lane per box looks its page up,
-// 32 boxes ahead; a missing page is flagged and its positions are left as they are.
+// 32 boxes ahead; a missing page is flagged and not read, and `gone` of its stage and of
+// the segment's later ones says so.
 template <int D, int BN, int ST>
 __device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMap& kmap,
                                              const CUtensorMap& vmap, uint32_t kv0,
                                              unsigned long long* fulls, unsigned long long* empties,
-                                             int seq, int kvh, int len, int tile0, int seg, int it) {
+                                             int* gone, int seq, int kvh, int len, int tile0, int seg, int it) {
   constexpr int HALVES = D / 64;
   const int lane = threadIdx.x & 31;
   const int per_tile = BN / a.box;                   // boxes of a tile
+  unsigned missed = 0;
   for (int b0 = 0; b0 < seg * per_tile; b0 += 32) {
     const int p_box = (tile0 * per_tile + b0 + lane) * a.box;
     int page = -2, row = 0;                          // -2: nothing to load
+    bool bad = false;
     if (b0 + lane < seg * per_tile && p_box < len) {
       const int blk = p_box / a.block_size;
       row = p_box - blk * a.block_size;
@@ -179,9 +183,10 @@ __device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMa
       if (page < 0 || page >= a.num_blocks) {
         if (a.status) atomicOr(a.status, GDN_STATUS_BAD_SLOT);
         page = -2;
+        bad = true;
       }
     }
-    const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+    const unsigned there = __ballot_sync(0xffffffffu, page >= 0), lack = __ballot_sync(0xffffffffu, bad);
     const int boxes = min(32, seg * per_tile - b0);
     for (int i = 0; i < boxes; ++i) {
       const int in_tile = (b0 + i) % per_tile;
@@ -196,11 +201,16 @@ __device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMa
           // the boxes of this tile that this round of 32 issues; the tile's last
           // round makes the arrival
           const int m = min(per_tile - in_tile, boxes - i);
-          const int live = __popc(there >> i & (m == 32 ? 0xffffffffu : (1u << m) - 1));
-          const uint32_t bytes = (uint32_t)live * a.box * D * 4;
-          if (in_tile + m == per_tile) tc::mbar_expect_tx(full, bytes);
-          else asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full),
-                            "r"(bytes) : "memory");
+          const unsigned of_tile = m == 32 ? 0xffffffffu : (1u << m) - 1;
+          const uint32_t bytes = (uint32_t)__popc(there >> i & of_tile) * a.box * D * 4;
+          missed |= lack >> i & of_tile;
+          if (in_tile + m == per_tile) {
+            gone[stage] = missed != 0;
+            tc::mbar_expect_tx(full, bytes);
+          } else {
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full), "r"(bytes)
+                         : "memory");
+          }
         }
         if (pg >= 0) {
 #pragma unroll
@@ -236,7 +246,7 @@ struct Attn {
     unsigned long long anc[kMaxTreeNodes];
     unsigned long long full[ST], empty[ST], bad;
     AttnScan scan;
-    int par[kMaxTreeNodes];
+    int par[kMaxTreeNodes], gone[ST];
   };
 };
 
@@ -292,8 +302,8 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
     const int len = s.ctx + s.n;
 
     if (warp == NC) {
-      attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, seq,
-                              kvh, len, tile0, seg, it);
+      attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, sm.gone,
+                              seq, kvh, len, tile0, seg, it);
     } else {
       // ---- consumers ----
       const auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(NC * 32) : "memory"); };
@@ -348,6 +358,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
           if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
           tc::mbar_wait(tc::smem_u32(&sm.full[stage]), ((it + t) / ST) & 1, kAttnWait);
         }
+        if (t == seg - 1 && sm.gone[stage]) sum[0] = sum[1] = __int_as_float(0x7fffffff);   // and so the outputs
         const int p_tile = (tile0 + t) * BN;
         const bool edge = p_tile + BN > s.ctx;       // holds nodes or positions behind them
         if (edge) {
@@ -586,7 +597,7 @@ struct AttnTc {
         q_empty[2], anc_full[2];
     AttnScan scan;
     uint32_t tmem;
-    int par[kMaxTreeNodes];
+    int par[kMaxTreeNodes], gone[ST];
   };
 };
 
@@ -649,8 +660,8 @@ __global__ void __launch_bounds__(384, 1)
     const int seg = (int)min((int64_t)(s.tiles - tile0), w1 - w);
 
     if (warp == 8) {
-      attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, seq,
-                              kvh, s.ctx + s.n, tile0, seg, it);
+      attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, sm.gone,
+                              seq, kvh, s.ctx + s.n, tile0, seg, it);
     } else if (warp == 11) {
       // ---- the segment's queries and ancestors, while the one before is worked on ----
       const int b = segs & 1;
@@ -728,10 +739,11 @@ __global__ void __launch_bounds__(384, 1)
         const int T = it + t, p_tile = (tile0 + t) * BN;
         const bool edge = p_tile + BN > s.ctx;       // holds nodes or positions behind them
         unsigned long long anc = 0;
+        if (edge || t + 2 >= seg) wait(sm.full[T % ST], (T / ST) & 1);
+        if (t + 2 >= seg && sm.gone[T % ST]) sum = __int_as_float(0x7fffffff);   // and so the outputs
         if (edge) {
           wait(sm.anc_full[segs & 1], (segs >> 1) & 1);
           if (row < rows) anc = sm.anc[segs & 1][node];
-          wait(sm.full[T % ST], (T / ST) & 1);
           unsigned char* vt = &sm.kv[T % ST][1][0][0];
 #pragma unroll 4
           for (int i = r; i < BN * (D / 8); i += 128) {

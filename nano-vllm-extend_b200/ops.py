@@ -1014,7 +1014,8 @@ def attention_tree(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, 
     q [N, HQ, D] bf16 (row views allowed), caches bf16 [blocks, block_size, HKV, D],
     block_tables int32 [n_seqs, max_blocks], context_lens [n_seqs]; max_len bounds
     context_lens[r] + the sequence's nodes (a longer sequence is skipped and
-    flagged).  ``scale`` defaults to D ** -0.5.  Returns out [N, HQ, D]."""
+    flagged; one with a page that is not there is flagged and its outputs are NaN).
+    ``scale`` defaults to D ** -0.5.  Returns out [N, HQ, D]."""
     dev = _one_device(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, parents)
     N, HQ, D, qs = _bf16_heads(q, "q")
     assert k_cache.dim() == 4
