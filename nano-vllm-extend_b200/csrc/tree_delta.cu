@@ -80,6 +80,7 @@ struct TreeDelta {
     float d0[TN], eg[TN], beta[TN];
     float norm[2 * TN];                              // 1 / |k|, scale / |q|
     __align__(16) float ssum[TN][NW];
+    int lost;                                        // a state did not come in time: the group has given up
     int par[2][TN];                                  // alternating: slow warps may still walk the last unit's
     // values and gates: each thread's own pieces, [node of the thread][thread]
     __align__(16) unsigned char vals[2][AHEAD ? TN / 4 * NT * MT * 4 : 16];
@@ -195,6 +196,7 @@ struct DeltaArgs {
   const bf16* nw;
   float eps;
   bool vec;
+  uint32_t wait;        // polls for a state's copy
   int32_t* status;
 };
 
@@ -267,9 +269,11 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
     }
     return d;
   };
-  // the state of the CTA's i-th unit into its buffer (one thread)
+  // the state of the CTA's i-th unit into its buffer (one thread of its group)
+  int asked = -1;                                    // the last unit it asked for
   const auto fetch = [&](int i, const DeltaUnit& d) {
     if (i >= count) return;
+    asked = i;
     const uint32_t bar = tc::smem_u32(&sm.full[i % ST]);
     if (d.n == 0) {
       tc::mbar_arrive(bar);
@@ -285,18 +289,18 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
     for (int b = 0; b < ST; ++b) tc::mbar_init(tc::smem_u32(&sm.full[b]), 1);
     tc::mbar_init_fence();
   }
+  if (tid == 0) gs.lost = 0;
   if (threadIdx.x == NT - 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(&pool) : "memory");
   DeltaAt at_cur = first.step(group, a.HV), at_nxt = at_cur.step(GROUPS, a.HV);
   const DeltaRaw raw_cur = raw_of(at_cur), raw_nxt = raw_of(at_nxt);
   __syncthreads();
-  // bounded: the state of the CTA's i-th unit has arrived
+  // bounded: the state of the CTA's i-th unit has arrived, or the group gives up at its
+  // next barrier
   const auto await_state = [&](int i) {
-    const uint32_t bar = tc::smem_u32(&sm.full[i % ST]);
-    if (!tc::mbar_wait(bar, (i / ST) & 1, kDeltaWait)) {
-      if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
-      tc::mbar_wait(bar, (i / ST) & 1, kDeltaWait);
-    }
+    if (tc::mbar_wait(tc::smem_u32(&sm.full[i % ST]), (i / ST) & 1, a.wait)) return;
+    gs.lost = 1;
+    if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
   };
 
   // a unit's scalars, loaded ahead
@@ -431,11 +435,8 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
     const DeltaAt at_after = at_nxt.step(GROUPS, a.HV);
     if (at_after.seq != at_nxt.seq) after = raw_of(at_after);
     const int n = cur.n;
-    if (n == 0) {                                    // nothing to compute: the buffer is free at once
-      if (tid == 0) {
-        await_state(i);
-        refill(i);
-      }
+    if (n == 0) {                                    // nothing to compute, and no copy: the buffer is free
+      if (tid == 0) refill(i);
       tc::cp_async_wait<0>();                        // the next unit's rows go where these went
       load_rows(nxt);
       copy_vals(0, a.v, a.vs, nxt);
@@ -548,6 +549,7 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
         }
       }
       group_sync();                                  // decays complete; state and rows are used up
+      if (gs.lost) break;                            // (set before this barrier only: all see the same)
       if (tid == 0) refill(i);
       load_rows(nxt);
 
@@ -712,6 +714,14 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
     nxt = unit_of(i + 2 * GROUPS, at_after, after, flags);
     at_nxt = at_after;
   }
+  // a group that gave up leaves its units' outputs as they were; what it asked for may
+  // still land in shared memory
+  if (gs.lost) {
+    tc::cp_async_wait<0>();
+    if (tid == 0)
+      for (int i = asked; i > asked - ST && i >= 0; i -= GROUPS)
+        tc::mbar_wait(tc::smem_u32(&sm.full[i % ST]), (i / ST) & 1, kDeltaWait);
+  }
 }
 
 template <int D, int TN>
@@ -798,7 +808,7 @@ extern "C" int gdn_delta_rule_tree(const void* q, int64_t q_row_stride, const vo
                     rep == 1 ? 0u : (unsigned)(((1ull << 32) + rep - 1) / rep), scale,
                     (const bf16*)z, z_row_stride, (const bf16*)norm_weight, norm_eps,
                     aligned16(q) && aligned16(k) && q_row_stride % 8 == 0 && k_row_stride % 8 == 0,
-                    status};
+                    wait_limit(kDeltaWait), status};
   cudaStream_t s = (cudaStream_t)stream;
 #define GDN_TDN(D)                                             \
   if (max_nodes <= 8) return launch_tree_delta<D, 8>(pool, a, s);   \

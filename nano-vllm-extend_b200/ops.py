@@ -156,9 +156,10 @@ def poll_status(device=None) -> int:
 
 
 def set_wait_limit(polls: int | None) -> None:
-    """Test hook (gdn_set_wait_limit): the poll limit of the head-per-CTA
-    decode form's bounded wait for its state copy; None restores the
-    default.  Calls made while a limit is set give invalid results."""
+    """Test hook (gdn_set_wait_limit): the poll limit of the bounded waits of
+    the head-per-CTA decode form and of :func:`gated_delta_rule_tree` for their
+    state copies; None restores the default.  Calls made while a limit is set
+    give invalid results."""
     _lib.load().gdn_set_wait_limit(-1 if polls is None else int(polls))
 
 
