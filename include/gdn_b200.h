@@ -71,8 +71,8 @@ const char* gdn_last_error(void);
  * gdn_decode_fused's head-per-CTA form for its state bulk copy gives up: that
  * launch then ORs GDN_STATUS_TIMEOUT into *status, waits (with the normal
  * limit) for the copy it has in flight, leaves the recurrent state untouched
- * and returns; the context stays usable.  gdn_delta_rule_tree's waits for its
- * states follow it too: what gave up leaves its outputs as they were.  0 makes a
+ * and returns; the context stays usable.  The waits of gdn_delta_rule_tree and
+ * gdn_attention_tree follow it too: what gave up leaves its outputs as they were.  0 makes a
  * wait give up at once; a negative value restores the default.  Not for production
  * use: calls made while an override is set give invalid results by design.
  */

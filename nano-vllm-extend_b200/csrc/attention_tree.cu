@@ -60,9 +60,28 @@ struct AttnArgs {
   float scale_log2;
   int64_t* prefix;                // [n_seqs + 1]: tiles before each sequence's
   float* part_o;                  // [CTAs][2][D / 4][BM][4]: rows side by side
-  float2* part_ml;                // [CTAs][2][BM]: maximum (base 2), sum
+  float2* part_ml;                // [CTAs][2][BM]: maximum (base 2; NaN: no part, the CTA gave up), sum
+  uint32_t wait;                  // polls
   int32_t* status;
 };
+
+// A wait that runs out (never, unless a copy is lost) ends the CTA's work: `lost` of the
+// thread, flagged in the status word.  A thread that is lost waits for nothing more, issues
+// no copy and no product, arrives at no barrier and clears no values; it runs through the
+// rest of the CTA's tiles all the same, as the named barriers count it.  Threads that
+// depend on it run out of polls in their turn, once each.  Rows that may hold anything of
+// this are not written, and their parts say so to the joining kernel.
+__device__ __forceinline__ void attn_wait(unsigned long long& bar, uint32_t parity, bool& lost,
+                                          const AttnArgs& a) {
+  if (lost || tc::mbar_wait(tc::smem_u32(&bar), parity, a.wait)) return;
+  lost = true;
+  if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
+}
+
+// What was issued lands before the CTA ends (the normal limit, whatever a test has set).
+__device__ __forceinline__ void attn_drain(unsigned long long& bar, uint32_t parity) {
+  tc::mbar_wait(tc::smem_u32(&bar), parity, kAttnWait);
+}
 
 // A sequence as attention sees it; n = 0: nothing to compute.
 struct AttnSeq {
@@ -167,7 +186,8 @@ template <int D, int BN, int ST>
 __device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMap& kmap,
                                              const CUtensorMap& vmap, uint32_t kv0,
                                              unsigned long long* fulls, unsigned long long* empties,
-                                             int* gone, int seq, int kvh, int len, int tile0, int seg, int it) {
+                                             int* gone, int seq, int kvh, int len, int tile0, int seg, int it,
+                                             bool& lost, int& issued) {
   constexpr int HALVES = D / 64;
   const int lane = threadIdx.x & 31;
   const int per_tile = BN / a.box;                   // boxes of a tile
@@ -194,10 +214,11 @@ __device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMa
       const int pg = __shfl_sync(0xffffffffu, page, i), rw = __shfl_sync(0xffffffffu, row, i);
       if (lane == 0) {
         const uint32_t full = tc::smem_u32(&fulls[stage]);
-        if (in_tile == 0 &&
-            !tc::mbar_wait(tc::smem_u32(&empties[stage]), ((t / ST) & 1) ^ 1, kAttnWait) && a.status)
-          atomicOr(a.status, GDN_STATUS_TIMEOUT);
-        if (in_tile == 0 || i == 0) {
+        if (in_tile == 0) {
+          attn_wait(empties[stage], ((t / ST) & 1) ^ 1, lost, a);
+          if (!lost) issued = t + 1;
+        }
+        if (!lost && (in_tile == 0 || i == 0)) {
           // the boxes of this tile that this round of 32 issues; the tile's last
           // round makes the arrival
           const int m = min(per_tile - in_tile, boxes - i);
@@ -212,7 +233,7 @@ __device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMa
                          : "memory");
           }
         }
-        if (pg >= 0) {
+        if (!lost && pg >= 0) {
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
@@ -228,6 +249,14 @@ __device__ __forceinline__ void attn_produce(const AttnArgs& a, const CUtensorMa
       __syncwarp();
     }
   }
+  lost = __shfl_sync(0xffffffffu, lost, 0);
+}
+
+// The producer warp's last tiles have landed.
+template <int ST>
+__device__ __forceinline__ void attn_produced(unsigned long long* fulls, int issued) {
+  if ((threadIdx.x & 31) == 0)
+    for (int t = max(0, issued - ST); t < issued; ++t) attn_drain(fulls[t % ST], (t / ST) & 1);
 }
 
 template <int D, int WM, int WN>
@@ -246,7 +275,7 @@ struct Attn {
     unsigned long long anc[kMaxTreeNodes];
     unsigned long long full[ST], empty[ST], bad;
     AttnScan scan;
-    int par[kMaxTreeNodes], gone[ST];
+    int par[kMaxTreeNodes], gone[ST], lost;
   };
 };
 
@@ -281,13 +310,15 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
       tc::mbar_init(tc::smem_u32(&sm.empty[i]), NC);
     }
     tc::mbar_init_fence();
+    sm.lost = 0;
   }
   int64_t w0, w1, seq_base;
   int seq;
   if (!attn_run<BM, BN, NC + 1>(a, sm.scan, w0, w1, seq, seq_base)) return;
 
   // ---- the run, a segment (part of a unit) at a time; every warp keeps the same place ----
-  int it = 0;                                        // tiles of this CTA so far
+  int it = 0, issued = 0;                            // tiles of this CTA so far; the producer's
+  bool lost = false;
   AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
   for (int64_t w = w0; w < w1;) {
     const int mine = s.tiles * s.row_tiles * a.HKV;  // at most 2^22 (host check)
@@ -302,8 +333,9 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
     const int len = s.ctx + s.n;
 
     if (warp == NC) {
-      attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, sm.gone,
-                              seq, kvh, len, tile0, seg, it);
+      if (!lost)
+        attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, sm.gone,
+                                seq, kvh, len, tile0, seg, it, lost, issued);
     } else {
       // ---- consumers ----
       const auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(NC * 32) : "memory"); };
@@ -354,10 +386,9 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
 
       for (int t = 0; t < seg; ++t) {
         const int stage = (it + t) % ST;
-        if (!tc::mbar_wait(tc::smem_u32(&sm.full[stage]), ((it + t) / ST) & 1, kAttnWait)) {
-          if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
-          tc::mbar_wait(tc::smem_u32(&sm.full[stage]), ((it + t) / ST) & 1, kAttnWait);
-        }
+        attn_wait(sm.full[stage], ((it + t) / ST) & 1, lost, a);
+        if (lost) sm.lost = 1;
+        __syncwarp();
         if (t == seg - 1 && sm.gone[stage]) sum[0] = sum[1] = __int_as_float(0x7fffffff);   // and so the outputs
         const int p_tile = (tile0 + t) * BN;
         const bool edge = p_tile + BN > s.ctx;       // holds nodes or positions behind them
@@ -365,7 +396,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
           unsigned char* vt = &sm.kv[stage][1][0][0];
           for (int i = tid; i < BN * (D / 8); i += NC * 32) {
             const int r = i / (D / 8), c = i - r * (D / 8), j = p_tile + r - s.ctx;
-            if (j < 0) continue;
+            if (j < 0 || lost) continue;
             uint4* p = reinterpret_cast<uint4*>(vt + tile_at<BN>(r, c));
             float f[8];
             unpack8(*p, f);
@@ -466,7 +497,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
         }
         if (edge) tc::fence_async_smem();            // our writes before the next copy's
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.empty[stage]));
+        if (lane == 0 && !lost) tc::mbar_arrive(tc::smem_u32(&sm.empty[stage]));
       }
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
@@ -477,7 +508,11 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
       const int64_t part = ((int64_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * BM;
       const unsigned long long bad = masks ? *reinterpret_cast<volatile unsigned long long*>(&sm.bad) : 0;
 
+      // a warp is lost with any of its lanes, and with a warp that was to clear values for it
+      const float2 no_part = make_float2(__int_as_float(0x7fffffff), 0.f);
+
       if constexpr (WN == 1) {
+        const bool failed = __any_sync(0xffffffffu, lost || *reinterpret_cast<volatile int*>(&sm.lost));
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           if (my_row[hh] >= rows) continue;
@@ -485,7 +520,8 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
           const float inv = whole ? 1.f / sum[hh] : 1.f;
           const int r = wm * 16 + gr + hh * 8;
           const int64_t at = (s.start + node[hh]) * a.HQ + kvh * a.G + my_row[hh] - node[hh] * a.G;
-          if (!whole && tq == 0) a.part_ml[part + r] = make_float2(mx[hh], sum[hh]);
+          if (!whole && tq == 0) a.part_ml[part + r] = failed ? no_part : make_float2(mx[hh], sum[hh]);
+          if (failed) continue;
 #pragma unroll
           for (int i = 0; i < D / 8; ++i) {
             float u = o[i][hh * 2] * inv, v = o[i][hh * 2 + 1] * inv;
@@ -505,6 +541,8 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
         for (int hh = 0; hh < 2; ++hh)
           if (tq == 0) sm.ml[wn * BM + wm * 16 + gr + hh * 8] = make_float2(mx[hh], sum[hh]);
         sync();
+        // (no consumer waits for a tile between this barrier and the next: all see the same)
+        const bool failed = *reinterpret_cast<volatile int*>(&sm.lost) != 0;
         float inv[2];
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
@@ -520,7 +558,8 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
           }
           inv[hh] = ex2(mx[hh] - off) * (whole ? 1.f / l : 1.f);
           if (anc[hh] & bad) inv[hh] = __int_as_float(0x7fffffff);
-          if (!whole && wn == 0 && tq == 0 && my_row[hh] < rows) a.part_ml[part + r] = make_float2(m, l);
+          if (!whole && wn == 0 && tq == 0 && my_row[hh] < rows)
+            a.part_ml[part + r] = failed ? no_part : make_float2(m, l);
         }
 #pragma unroll
         for (int cq = 0; cq < D / 32; ++cq) {
@@ -535,7 +574,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
           for (int i = tid; i < BM * 8; i += NC * 32) {
             // a whole unit's rows are written along their columns, parts along the rows
             const int r = whole ? i >> 3 : i % BM, c = (whole ? i & 7 : i / BM) * 4, row = row0 + r;
-            if (row < rows) {
+            if (row < rows && !failed) {
               float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
               for (int v = 0; v < WN; ++v) {
@@ -562,6 +601,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
     it += seg;
     w += seg;
   }
+  if (warp == NC) attn_produced<ST>(sm.full, issued);
 }
 
 // ---------------------------------------------------------------------------
@@ -597,7 +637,7 @@ struct AttnTc {
         q_empty[2], anc_full[2];
     AttnScan scan;
     uint32_t tmem;
-    int par[kMaxTreeNodes], gone[ST];
+    int par[kMaxTreeNodes], gone[ST], lost;
   };
 };
 
@@ -629,6 +669,7 @@ __global__ void __launch_bounds__(384, 1)
       tc::mbar_init(bar(sm.q_empty[i]), 9);           // the last S, and the softmax warps
     }
     tc::mbar_init_fence();
+    sm.lost = 0;                                     // set by softmax threads alone
   }
   int64_t w0, w1, seq_base;
   int seq;
@@ -639,14 +680,11 @@ __global__ void __launch_bounds__(384, 1)
   tc::fence_after();
   const uint32_t tmem = sm.tmem;
 
-  // a bounded wait; one that gives up is flagged and waits once more
-  const auto wait = [&](unsigned long long& b, uint32_t parity) {
-    if (tc::mbar_wait(bar(b), parity, kAttnWait)) return;
-    if (a.status) atomicOr(a.status, GDN_STATUS_TIMEOUT);
-    tc::mbar_wait(bar(b), parity, kAttnWait);
-  };
+  bool lost = false;
+  const auto wait = [&](unsigned long long& b, uint32_t parity) { attn_wait(b, parity, lost, a); };
 
   int it = 0, segs = 0;                              // tiles and segments of this CTA so far
+  int issued = 0;                                    // what the warp's lane 0 has under way goes up to here
   AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
   for (int64_t w = w0; w < w1;) {
     const int mine = s.tiles * s.row_tiles * a.HKV;  // at most 2^22 (host check)
@@ -660,20 +698,23 @@ __global__ void __launch_bounds__(384, 1)
     const int seg = (int)min((int64_t)(s.tiles - tile0), w1 - w);
 
     if (warp == 8) {
-      attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, sm.gone,
-                              seq, kvh, s.ctx + s.n, tile0, seg, it);
+      if (!lost)
+        attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, sm.gone,
+                                seq, kvh, s.ctx + s.n, tile0, seg, it, lost, issued);
     } else if (warp == 11) {
       // ---- the segment's queries and ancestors, while the one before is worked on ----
       const int b = segs & 1;
       wait(sm.q_empty[b], ((segs >> 1) & 1) ^ 1);
-      if (lane == 0) {
+      lost = __any_sync(0xffffffffu, lost);
+      if (lane == 0 && !lost) {
+        issued = segs + 1;
         tc::mbar_expect_tx(bar(sm.q_full[b]), (uint32_t)a.tile_rows * D * 2);
 #pragma unroll
         for (int hf = 0; hf < P::HALVES; ++hf)
           tc::tma_load_3d(tc::smem_u32(&sm.q[b][hf][0]), &qmap, hf * 64, kvh * a.G,
                           (int)s.start + rt * (a.tile_rows / a.G), bar(sm.q_full[b]));
       }
-      if ((tile0 + seg) * BN > s.ctx) {              // the segment reaches the nodes
+      if ((tile0 + seg) * BN > s.ctx && !lost) {     // the segment reaches the nodes
         for (int j = lane; j < s.n; j += 32) sm.par[j] = tree_parent(a.parents[s.start + j], j, a.status);
         __syncwarp();
         for (int j = lane; j < s.n; j += 32) {
@@ -684,7 +725,7 @@ __global__ void __launch_bounds__(384, 1)
         if (lane == 0) sm.bad[b] = 0;
         __syncwarp();
       }
-      if (lane == 0) tc::mbar_arrive(bar(sm.anc_full[b]));
+      if (lane == 0 && !lost) tc::mbar_arrive(bar(sm.anc_full[b]));
       __syncwarp();
     } else if (warp >= 9) {
       // ---- products: a thread for S, one for O.  (One thread for both took 2200 cycles
@@ -696,6 +737,7 @@ __global__ void __launch_bounds__(384, 1)
         for (int T = it; T < it + seg; ++T) {
           wait(sm.full[T % ST], (T / ST) & 1);
           wait(sm.s_free[T & 1], ((T >> 1) & 1) ^ 1);
+          if (lost) break;
           tc::fence_after();
           const uint64_t kd = tc::smem_desc(tc::smem_u32(&sm.kv[T % ST][0][0][0]), 16, 1024);
 #pragma unroll
@@ -705,13 +747,15 @@ __global__ void __launch_bounds__(384, 1)
                          kd + ((x >> 2) * (BN * 128) + (x & 3) * 32) / 16,
                          tc::idesc_bf16(BM, BN, false, false), x > 0);
           tc::mma_commit(bar(sm.s_full[T & 1]));
+          issued = T + 1;
         }
-        tc::mma_commit(bar(sm.q_empty[segs & 1]));
+        if (!lost) tc::mma_commit(bar(sm.q_empty[segs & 1]));
       } else if (lane == 0) {
         for (int t = 0; t < seg; ++t) {
           const int T = it + t;
           wait(sm.full[T % ST], (T / ST) & 1);
           wait(sm.p_full[T & 1], (T >> 1) & 1);
+          if (lost) break;
           tc::fence_after();
           const uint64_t pd = tc::smem_desc(tc::smem_u32(&sm.p[T & 1][0]), 16, 1024);
           const uint64_t vd = tc::smem_desc(tc::smem_u32(&sm.kv[T % ST][1][0][0]), BN * 128, 1024);
@@ -721,6 +765,7 @@ __global__ void __launch_bounds__(384, 1)
                          tc::idesc_bf16(BM, D, false, true), (t > 1 || x > 0) ? 1u : 0u);
           tc::mma_commit(bar(sm.empty[T % ST]));
           tc::mma_commit(bar(sm.pv_done[T & 1]));
+          issued = T + 1;
         }
       }
       __syncwarp();
@@ -748,7 +793,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll 4
           for (int i = r; i < BN * (D / 8); i += 128) {
             const int vrow = i / (D / 8), c = i - vrow * (D / 8), j = p_tile + vrow - s.ctx;
-            if (j < 0) continue;
+            if (j < 0 || lost) continue;
             uint4* p = reinterpret_cast<uint4*>(vt + tile_at<BN>(vrow, c));
             float f[8];
             unpack8(*p, f);
@@ -762,12 +807,13 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
         wait(sm.s_full[grp], (T >> 1) & 1);
+        __syncwarp();
         tc::fence_after();
         float x[2][32];
         tc::tmem_ld32x2(tl + P::kColS + grp * 64, tl + P::kColS + grp * 64 + 32, x[0], x[1]);
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(bar(sm.s_free[grp]));
+        if (lane == 0 && !lost) tc::mbar_arrive(bar(sm.s_free[grp]));
         if (edge) {                                  // a bit per position that the row sees
           const int nodes_at = s.ctx - p_tile;       // > -64, as the tile holds a node
           const unsigned long long see =
@@ -817,7 +863,7 @@ __global__ void __launch_bounds__(384, 1)
         tc::fence_before();
         if (edge) asm volatile("bar.sync %0, 128;" ::"r"(grp + 1) : "memory");   // every value row is clean
         else __syncwarp();
-        if (lane == 0) tc::mbar_arrive(bar(sm.p_full[grp]));
+        if (lane == 0 && !lost) tc::mbar_arrive(bar(sm.p_full[grp]));
       }
       // join the groups: each waits for its own last product, which leaves its P free
       bool has[2];
@@ -827,11 +873,17 @@ __global__ void __launch_bounds__(384, 1)
         has[v] = T >= it;
         if (has[v] && v == grp) wait(sm.pv_done[v], (T >> 1) & 1);
       }
+      const bool masks = (tile0 + seg) * BN > s.ctx;
+      if (masks) wait(sm.anc_full[segs & 1], (segs >> 1) & 1);
+      if (lost) sm.lost = 1;
+      __syncwarp();
       const auto ml = [&](int g) -> float2& { return reinterpret_cast<float2*>(&sm.p[g][0])[r]; };
       ml(grp) = make_float2(ref, sum);
       tc::fence_before();
       sync_all();
       tc::fence_after();
+      // (no thread that sets it waits between this barrier and the next: all see the same)
+      const bool failed = *reinterpret_cast<volatile int*>(&sm.lost) != 0;
       const float2 ml0 = ml(0), ml1 = ml(1);
       const float top = fmaxf(ml0.x, ml1.x), off = top == -INFINITY ? 0.f : top;
       float f0 = ex2(ml0.x - off), f1 = ex2(ml1.x - off);
@@ -839,15 +891,14 @@ __global__ void __launch_bounds__(384, 1)
       const bool whole = tile0 == 0 && seg == s.tiles;
       const int64_t part = ((int64_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * BM;
       bool nan = false;                              // the row sees a value row that is not finite
-      if ((tile0 + seg) * BN > s.ctx) {
-        wait(sm.anc_full[segs & 1], (segs >> 1) & 1);
+      if (masks)
         nan = row < rows && (sm.anc[segs & 1][node] &
                              *reinterpret_cast<volatile unsigned long long*>(&sm.bad[segs & 1])) != 0;
-      }
       const float inv = nan ? __int_as_float(0x7fffffff) : whole ? 1.f / l : 1.f;
       f0 *= inv;
       f1 *= inv;
-      if (!whole && grp == 0 && row < rows) a.part_ml[part + r] = make_float2(top, l);
+      if (!whole && grp == 0 && row < rows)
+        a.part_ml[part + r] = failed ? make_float2(__int_as_float(0x7fffffff), 0.f) : make_float2(top, l);
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
         const int c = grp * (D / 2) + i * 32;        // a half of the columns each
@@ -862,7 +913,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = fmaf(y[e], v == 0 ? f0 : f1, o[e]);
           }
-        if (row < rows) {
+        if (row < rows && !failed) {
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8)
@@ -877,11 +928,19 @@ __global__ void __launch_bounds__(384, 1)
       }
       tc::fence_before();
       sync_all();                                    // masks and O are used up
-      if (lane == 0) tc::mbar_arrive(bar(sm.q_empty[segs & 1]));
+      if (lane == 0 && !lost) tc::mbar_arrive(bar(sm.q_empty[segs & 1]));
     }
     it += seg;
     ++segs;
     w += seg;
+  }
+  // what is under way ends before the CTA does, and before its TMEM is given back
+  if (warp == 8) attn_produced<ST>(sm.full, issued);
+  if (lane == 0 && issued > 0) {
+    if (warp == 9) attn_drain(sm.s_full[(issued - 1) & 1], ((issued - 1) >> 1) & 1);
+    if (warp == 10) attn_drain(sm.pv_done[(issued - 1) & 1], ((issued - 1) >> 1) & 1);
+    if (warp == 11)
+      for (int i = max(0, issued - 2); i < issued; ++i) attn_drain(sm.q_full[i & 1], (i >> 1) & 1);
   }
   tc::fence_before();
   __syncthreads();
@@ -932,11 +991,16 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
   const int col = 16 * (SHARES > 1 ? cb : cb * J::CG + rest);
   const bool live = r < rows;
   float m = -INFINITY, l = 0.f, acc[16];
+  bool lack = false;                                 // of a part whose CTA gave up
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = 0.f;
   if (live) {
 #pragma unroll 4
-    for (int i = share; i < parts; i += SHARES) m = fmaxf(m, a.part_ml[part(i) + r].x);
+    for (int i = share; i < parts; i += SHARES) {
+      const float x = a.part_ml[part(i) + r].x;
+      lack |= isnan(x);
+      m = fmaxf(m, x);
+    }
     const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll 2
     for (int i = share; i < parts; i += SHARES) {
@@ -955,13 +1019,16 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
     }
   }
   if constexpr (SHARES > 1) {
-    s_ml[share][rr] = make_float2(m, l);
+    s_ml[share][rr] = make_float2(lack ? __int_as_float(0x7fffffff) : m, l);
 #pragma unroll
     for (int e = 0; e < 16; ++e) s_o[share][rr * 17 + e] = acc[e];
     __syncthreads();
     if (share > 0) return;
 #pragma unroll
-    for (int v = 0; v < SHARES; ++v) m = fmaxf(m, s_ml[v][rr].x);
+    for (int v = 0; v < SHARES; ++v) {
+      lack |= isnan(s_ml[v][rr].x);
+      m = fmaxf(m, s_ml[v][rr].x);
+    }
     const float off = m == -INFINITY ? 0.f : m;
     l = 0.f;
 #pragma unroll
@@ -974,7 +1041,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
       for (int e = 0; e < 16; ++e) acc[e] = fmaf(s_o[v][rr * 17 + e], f, acc[e]);
     }
   }
-  if (!live) return;
+  if (!live || lack) return;
   const float inv = 1.f / l;
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] *= inv;
@@ -1146,7 +1213,7 @@ extern "C" int gdn_attention_tree(const void* q, int64_t q_row_stride, const voi
                    n_tokens, max_len, (bf16*)out, num_q_heads, num_kv_heads, G, tile_rows,
                    scale * 1.4426950408889634f, reinterpret_cast<int64_t*>(ws + sp.prefix),
                    reinterpret_cast<float*>(ws + sp.part_o),
-                   reinterpret_cast<float2*>(ws + sp.part_ml), status};
+                   reinterpret_cast<float2*>(ws + sp.part_ml), wait_limit(kAttnWait), status};
   cudaStream_t s = (cudaStream_t)stream;
 #define GDN_AT(D)                                                    \
   if (bm == 16) return launch_attention<D, 1, 4>(kmap, vmap, a, s);  \

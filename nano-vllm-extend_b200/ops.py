@@ -157,9 +157,9 @@ def poll_status(device=None) -> int:
 
 def set_wait_limit(polls: int | None) -> None:
     """Test hook (gdn_set_wait_limit): the poll limit of the bounded waits of
-    the head-per-CTA decode form and of :func:`gated_delta_rule_tree` for their
-    state copies; None restores the default.  Calls made while a limit is set
-    give invalid results."""
+    the head-per-CTA decode form, :func:`gated_delta_rule_tree` and
+    :func:`attention_tree`; None restores the default.  Calls made while a limit
+    is set give invalid results."""
     _lib.load().gdn_set_wait_limit(-1 if polls is None else int(polls))
 
 
