@@ -5,11 +5,12 @@ and ``lens_q`` from it (qwen3_5.py:869-881).  The dataclass keeps every field
 of the reference's Context, in the same order, so ``set_context`` calls
 written for the reference work unchanged.  When the layer is installed into
 the reference engine (:func:`layer.install`), it reads the engine's own
-context instead of this one.
+context instead of this one, but for steps of drafted trees, which the engine's
+context has no place for: see :func:`step_context`.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -42,6 +43,8 @@ class DraftContext(Context):
     follows the stored context.  The layers leave their slots' state as it is until the
     accepted paths are committed (layer.commit_drafts)."""
     draft_parents: torch.Tensor | None = None
+    # the engine's context when an installed layer first read this one
+    engine: object | None = field(default=None, repr=False, compare=False)
 
 
 _CONTEXT = Context()
@@ -65,7 +68,9 @@ def set_context(cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0, max_seqlen
 
 
 def set_draft_context(cu_seqlens, draft_parents, max_nodes, linear_state_ids):
-    """Make the step one of drafted trees (:class:`DraftContext`)."""
+    """Make the step one of drafted trees (:class:`DraftContext`), for layers installed
+    into an engine too.  The tensors are read again when the accepted paths are committed,
+    so they keep their contents until then."""
     global _CONTEXT
     _CONTEXT = DraftContext(cu_seqlens, cu_seqlens, max_nodes, max_nodes,
                             linear_state_ids=linear_state_ids, draft_parents=draft_parents)
@@ -74,3 +79,23 @@ def set_draft_context(cu_seqlens, draft_parents, max_nodes, linear_state_ids):
 def reset_context():
     global _CONTEXT
     _CONTEXT = Context()
+
+
+def step_context(engine_context):
+    """The step's context for a layer installed into an engine whose own one is
+    ``engine_context()``: the drafted trees of :func:`set_draft_context` where these are
+    set, else the engine's.  An engine never resets this module's context, so a step of
+    drafted trees lasts until the engine sets or resets its own, at the latest: from the
+    first layer's read on it belongs to the engine's context of that moment, and is
+    dropped once that is another object, as each ``set_context`` and ``reset_context``
+    makes one (an engine that changes its context in place calls this module's
+    :func:`reset_context` after the step)."""
+    own, step = _CONTEXT, engine_context()
+    if not isinstance(own, DraftContext):
+        return step
+    if own.engine is None:
+        own.engine = step
+    if own.engine is step:
+        return own
+    reset_context()
+    return step

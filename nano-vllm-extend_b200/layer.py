@@ -305,7 +305,8 @@ def install(qwen3_5_module=None, parallel_module=None, context_module=None):
     Call after importing the reference package and before the model is
     built (ModelRunner constructs Qwen3_5ForCausalLM, whose decoder layers
     look the class up by its module-global name).  The installed subclass
-    reads the engine's own parallel state and per-step context.  Returns
+    reads the engine's own parallel state and per-step context, and steps of
+    drafted trees as :func:`context.set_draft_context` has them.  Returns
     the class that was replaced (pass it to :func:`uninstall`)."""
     if qwen3_5_module is None:
         import nanovllm.models.qwen3_5 as qwen3_5_module  # noqa: PLC0415
@@ -317,7 +318,8 @@ def install(qwen3_5_module=None, parallel_module=None, context_module=None):
 
     class Qwen3_5GatedDeltaNetB200(Qwen3_5GatedDeltaNet):
         def __init__(self, config):
-            super().__init__(config, parallel=P, get_context=Cx.get_context)
+            super().__init__(config, parallel=P,
+                             get_context=lambda: _context.step_context(Cx.get_context))
 
     previous = qwen3_5_module.Qwen3_5GatedDeltaNet
     qwen3_5_module.Qwen3_5GatedDeltaNet = Qwen3_5GatedDeltaNetB200
