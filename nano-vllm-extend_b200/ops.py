@@ -745,6 +745,9 @@ def _int32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     assert t.shape == (n,), f"{name} must have {n} entries"
     if t.dtype is not torch.int32 or not t.is_contiguous():
         assert not t.is_floating_point(), f"{name} must hold integers"
+        if t.dtype == torch.int64:
+            # what 32 bits cannot hold stays out of range, and is flagged as such
+            t = t.clamp(-2 ** 31, 2 ** 31 - 1)
         t = t.to(torch.int32).contiguous()
     return t
 
