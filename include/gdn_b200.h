@@ -405,8 +405,8 @@ int gdn_commit_tree(const void* x, int64_t x_row_stride,
  * fp32 arithmetic, rounded once.  q, k, v: bf16 rows of their heads (row strides
  * given); q_weight, k_weight: bf16 [head_dim]; cos_sin: fp32 [max_position,
  * rotary_dim], cosines then sines; positions: int64 [n_tokens], one outside the
- * table is flagged GDN_STATUS_BAD_POSITION and its row's queries and keys are not
- * written.  k_cache / v_cache: bf16, element (block, token, head, d) at
+ * table is flagged GDN_STATUS_BAD_POSITION and nothing of its row is written.
+ * k_cache / v_cache: bf16, element (block, token, head, d) at
  * block*block_stride + token*token_stride + head*head_stride + d, both alike;
  * slot_mapping: int32 [n_tokens], block * block_size + token, -1 to store
  * nothing; one outside the cache is flagged GDN_STATUS_BAD_SLOT and not stored.

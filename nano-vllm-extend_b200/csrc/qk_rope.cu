@@ -69,7 +69,8 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_rope_kernel(
   int64_t cache = -1;                         // the slot's place in the caches
   if (slot >= 0 && slot < num_blocks * block_size) {
     const int page = slot / block_size;
-    cache = page * block_stride + (int64_t)(slot - page * block_size) * token_stride;
+    // (a row without a position has no key: its value would stand beside an older one)
+    if (placed) cache = page * block_stride + (int64_t)(slot - page * block_size) * token_stride;
   } else if (slot != -1 && status && sub == 0 && h0 + NH > HQ) {
     atomicOr(status, GDN_STATUS_BAD_SLOT);
   }
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_rope_kernel(
         *reinterpret_cast<uint2*>(dst + da) = ra[u];
         *reinterpret_cast<uint2*>(dst + db) = rb[u];
         dst = nullptr;
-      } else if (placed) {
+      } else {
         dst = k_cache + cache + (h - HQ) * head_stride;
       }
     }
