@@ -336,7 +336,8 @@ __global__ void __launch_bounds__(kConvThreads) conv_state_writeback_kernel(
 constexpr int kTreeConvThreads = 256;
 
 // a / (1 + 2^(-a log2 e)) by the hardware's power and reciprocal, subnormals taken as
-// zero: nothing of that size survives the sum with 1, so the results are conv_silu()'s.
+// zero: a power of that size does not survive the sum with 1, and a reciprocal of that
+// size (a below -87) belongs to results below 2^-119, which conv_silu() gives as zero too.
 __device__ __forceinline__ float tree_silu(float a) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.4426950408889634f));
