@@ -275,7 +275,7 @@ struct Attn {
     unsigned long long anc[kMaxTreeNodes];
     unsigned long long full[ST], empty[ST], bad;
     AttnScan scan;
-    int par[kMaxTreeNodes], gone[ST], lost;
+    int par[kMaxTreeNodes], gone[ST], lost, issued;
   };
 };
 
@@ -310,14 +310,14 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
       tc::mbar_init(tc::smem_u32(&sm.empty[i]), NC);
     }
     tc::mbar_init_fence();
-    sm.lost = 0;
+    sm.lost = sm.issued = 0;
   }
   int64_t w0, w1, seq_base;
   int seq;
   if (!attn_run<BM, BN, NC + 1>(a, sm.scan, w0, w1, seq, seq_base)) return;
 
   // ---- the run, a segment (part of a unit) at a time; every warp keeps the same place ----
-  int it = 0, issued = 0;                            // tiles of this CTA so far; the producer's
+  int it = 0;                                        // tiles of this CTA so far
   bool lost = false;
   AttnSeq s = attn_seq<BM, BN>(a, seq, nullptr);
   for (int64_t w = w0; w < w1;) {
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
     if (warp == NC) {
       if (!lost)
         attn_produce<D, BN, ST>(a, kmap, vmap, tc::smem_u32(&sm.kv[0][0][0][0]), sm.full, sm.empty, sm.gone,
-                                seq, kvh, len, tile0, seg, it, lost, issued);
+                                seq, kvh, len, tile0, seg, it, lost, sm.issued);
     } else {
       // ---- consumers ----
       const auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(NC * 32) : "memory"); };
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
     it += seg;
     w += seg;
   }
-  if (warp == NC) attn_produced<ST>(sm.full, issued);
+  if (warp == NC) attn_produced<ST>(sm.full, sm.issued);
 }
 
 // ---------------------------------------------------------------------------
