@@ -439,7 +439,9 @@ int gdn_qk_norm_rope_cache(const void* q, int64_t q_row_stride,
  * [n_seqs]; max_len bounds context_lens[r] + the sequence's rows, a longer one
  * is skipped and flagged GDN_STATUS_BAD_SEQLEN.  A page outside the cache is
  * flagged GDN_STATUS_BAD_SLOT, never read, and all outputs of its sequence are NaN.
- * scores are scaled by `scale` > 0.
+ * scores are scaled by `scale` > 0.  fp32 sums and softmax; the second product takes the
+ * probabilities to 16 bits where max_nodes x num_q_heads / num_kv_heads is at most 16
+ * (the decode step), else rounded to bf16.
  * out: bf16 [n_tokens, num_q_heads, head_dim].  head_dim 64, 128 or 256.
  * workspace: device scratch of gdn_attention_tree_workspace_bytes() bytes,
  * 16-byte aligned, used only during the call.

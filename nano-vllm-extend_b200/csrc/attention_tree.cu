@@ -21,8 +21,13 @@
 // page, 128-byte swizzle) into a ring of stages, across unit borders; WM warps over
 // rows x WN warps over positions run one pass with the softmax's running maximum
 // and sum, scores and probabilities in registers (the score tile's accumulators are
-// the next product's A operand).  Sums and statistics are fp32; the probabilities are
-// rounded to bf16 as an operand of the second product, as the values are bf16.
+// the next product's A operand).  Sums and statistics are fp32.  The second product takes
+// the probabilities in bf16, as the values are: with 16 rows, where the traffic bounds it, as
+// two parts (rounded, and what that leaves: 16 bits), which takes 0.7 % longer and leaves
+// the output's own rounding as the only error of note (1.7e-3 relative to 64 bits); with
+// more rows rounded once (2.1e-3 to 2.3e-3), as two parts take 11 to 19 % there with
+// mma.sync (128 sequences of 8 nodes and 2303 positions 138 us instead of 123) and 8 % on
+// tcgen05 (32 of 16 to 32 nodes 100 us instead of 92, the parts in TMEM).
 //
 // In the tiles that hold nodes or reach behind them, value rows behind the last node
 // are zeroed in shared memory, and so are nodes' rows that are not finite, which must
@@ -268,6 +273,7 @@ struct Attn {
   static constexpr int CTAS = D <= 128 ? 2 : 1;                   // per SM
   static constexpr int STAGE = 2 * BN * D * 2;                    // bytes of keys and values
   static constexpr int ST = 3;
+  static constexpr int PARTS = WM == 1 ? 2 : 1;                   // of a probability
   struct Smem {
     __align__(1024) unsigned char kv[ST][2][HALVES][BN * 128];
     __align__(16) float join[WN > 1 ? WN * BM * 36 : 4];          // 32 columns at a time
@@ -446,7 +452,6 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
                   }
             }
             // running maximum and sum; scaled to base 2 (scale > 0) within the exponent's argument
-            uint32_t pa[XT / 16][4];
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
               float m = -INFINITY;
@@ -479,20 +484,24 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
             }
 #pragma unroll
             for (int i = 0; i < XT / 16; ++i) {
-              pa[i][0] = mm::pack2(x[2 * i][0], x[2 * i][1]);
-              pa[i][1] = mm::pack2(x[2 * i][2], x[2 * i][3]);
-              pa[i][2] = mm::pack2(x[2 * i + 1][0], x[2 * i + 1][1]);
-              pa[i][3] = mm::pack2(x[2 * i + 1][2], x[2 * i + 1][3]);
-            }
+              uint32_t pa[P::PARTS][4];
 #pragma unroll
-            for (int i = 0; i < XT / 16; ++i)
+              for (int e = 0; e < 4; ++e) {
+                const float* f = &x[2 * i + (e >> 1)][(e & 1) * 2];
+                if constexpr (P::PARTS == 2) mm::split2(f[0], f[1], pa[0][e], pa[1][e]);
+                else pa[0][e] = mm::pack2(f[0], f[1]);
+              }
 #pragma unroll
               for (int c = 0; c < D / 8; c += 2) {
                 uint32_t b[4];
                 mm::ldsm4t(b, v_base + tile_at<BN>(p0 + i * 16 + (lane & 15), c + (lane >> 4)));
-                mm::mma16816(o[c], pa[i], b[0], b[1]);
-                mm::mma16816(o[c + 1], pa[i], b[2], b[3]);
+#pragma unroll
+                for (int v = 0; v < P::PARTS; ++v) {
+                  mm::mma16816(o[c], pa[v], b[0], b[1]);
+                  mm::mma16816(o[c + 1], pa[v], b[2], b[3]);
+                }
               }
+            }
           }
         }
         if (edge) tc::fence_async_smem();            // our writes before the next copy's

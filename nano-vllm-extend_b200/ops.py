@@ -1019,7 +1019,9 @@ def attention_tree(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, 
     block_tables int32 [n_seqs, max_blocks], context_lens [n_seqs]; max_len bounds
     context_lens[r] + the sequence's nodes (a longer sequence is skipped and
     flagged; one with a page that is not there is flagged and its outputs are NaN).
-    ``scale`` defaults to D ** -0.5.  Returns out [N, HQ, D]."""
+    ``scale`` defaults to D ** -0.5.  fp32 sums and softmax; the probabilities enter the
+    second product with 16 bits where max_nodes * HQ / HKV is at most 16, else rounded
+    to bf16.  Returns out [N, HQ, D]."""
     dev = _one_device(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, parents)
     N, HQ, D, qs = _bf16_heads(q, "q")
     assert k_cache.dim() == 4
