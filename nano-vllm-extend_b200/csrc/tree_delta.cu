@@ -20,10 +20,11 @@
 // columns by 8 nodes, so few nodes waste little.  The results' layout is that of the
 // next product's A operand (nodes 2t, 2t + 1 as its k = t, t + 4), so X, d and o
 // never leave the warp's registers.  X is bf16 with fp32 sums: q and k are exact,
-// S_0 enters as two parts of 8 bits each (cutting it to one tf32 part of 11 bits, no
-// instruction per element, saves 2 us of 99); A, M and d meet in tf32, two parts of
-// 11 bits each (hi hi + lo hi + hi lo).  Norms, decays and the substitution within
-// eight nodes are fp32.
+// S_0 enters as two parts, each rounded: 2^-17 of an element is left out, which adds
+// 1e-4 to the 1.7e-3 (relative) of the output's rounding (all 24 bits, in three parts:
+// 107 us instead of 97; one tf32 part of 11 bits saves 2 of them); A, M and d meet in
+// tf32, two parts of 11 bits each (hi hi + lo hi + hi lo).  Norms, decays and the
+// substitution within eight nodes are fp32.
 //
 // The chain of a unit (one sequence and v-head) is long and mostly latency:
 // norms, decays, gram factors, X, substitution, norm.  So the states come by TMA
@@ -103,20 +104,6 @@ __device__ __forceinline__ uint4 load8(const bf16* p) {
 
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
-
-// The upper halves of two fp32 words: (x, y) cut to a bf16 pair.
-__device__ __forceinline__ uint32_t cut2(float x, float y) {
-  return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-}
-// What that leaves of each.
-__device__ __forceinline__ void rest2(float x, float y, float& rx, float& ry) {
-  const unsigned long long h = tc::f2pack(
-      __uint_as_float((__float_as_uint(x) & 0xffff0000u) ^ 0x80000000u),
-      __uint_as_float((__float_as_uint(y) & 0xffff0000u) ^ 0x80000000u));
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(tc::f2pack(x, y)), "l"(h));
-  tc::f2unpack(r, rx, ry);
-}
 
 // Substitution within eight nodes (lane t of a quad holds nodes 2t, 2t + 1; r[0],
 // r[1] of one column, r[2], r[3] of the next): node i's d to the quad, then into the
@@ -520,19 +507,13 @@ __global__ void __launch_bounds__(TreeDelta<D, TN>::NT* TreeDelta<D, TN>::GROUPS
             if constexpr (VC == 4) *reinterpret_cast<float4*>(s[j]) = *reinterpret_cast<const float4*>(p);
             else *reinterpret_cast<float2*>(s[j]) = *reinterpret_cast<const float2*>(p);
           }
-          float l[4][VC];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < VC; e += 2) rest2(s[j][e], s[j][e + 1], l[j][e], l[j][e + 1]);
           uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = (e >> 1) * 2, col = 2 * mt + (e & 1);
-              hi[mt][e] = cut2(s[j][col], s[j + 1][col]);
-              lo[mt][e] = cut2(l[j][col], l[j + 1][col]);
+              mm::split2(s[j][col], s[j + 1][col], hi[mt][e], lo[mt][e]);
             }
 #pragma unroll
           for (int t8 = 0; t8 < 2 * KT; t8 += 2) {

@@ -31,3 +31,21 @@ def test_attention_of_few_rows(ops, D, HQ, HKV, nodes, ctx):  # noqa: F811
     err = np.abs(host(out) - ref)
     assert (err <= tol).all(), f"{(err > tol).sum()} of {err.size}, worst {(err / tol).max():.2f}"
     assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("D,nodes", [(128, 8), (64, 8), (128, 16), (64, 30), (128, 64), (64, 64)])
+def test_stored_states(ops, D, nodes):  # noqa: F811
+    """q over states that cancel but for their low bits: entries of 1 + 2^-8 + 2^-15 - 2^-23
+    against -(1 + 2^-8).  Both parts rounded leave 2^-17 of an entry at most, both cut 2^-15."""
+    c = Gdn(1, 2, D, [nodes, 1], seed=nodes, chain=True)
+    c.pool[:, 1, :, 0::2] = 1 + 2.0 ** -8 + 2.0 ** -15 - 2.0 ** -23
+    c.pool[:, 1, :, 1::2] = -(1 + 2.0 ** -8)
+    c.y[:, :D] = 1.0                                    # q
+    c.beta[:] = 0.0                                     # no node changes the state
+    c.g[:] = 0.0
+    c.upload()
+    ref = c.delta_ref(False)
+    size = D ** -0.5 * D ** 0.5 * 1.01                  # sum of |S| |q|: D entries of D^-1/2 D^-1/2
+    err = np.abs(host(c.delta(ops, False)) - ref)
+    tol = U * np.abs(ref) + (2.0 ** -17 + 2.0 ** -18) * size
+    assert (err <= tol).all(), f"worst {(err / tol).max():.2f} of the tolerance"
