@@ -324,11 +324,13 @@ int gdn_decode_fused_static(const void* mixed, int64_t mixed_row_stride,
  *  - parents: int32 [n_tokens]; a row's parent as a number within its sequence,
  *    smaller than its own, or -1 for a node that follows the stored context
  *    directly.  A node sees the context, its ancestors and itself.
- *  - max_nodes bounds every sequence's rows, at most GDN_MAX_TREE_NODES.
+ *  - max_nodes bounds every sequence's rows, at most GDN_MAX_TREE_NODES (0: nothing
+ *    is computed or flagged, but for the slot map's rows).
  *  - A malformed sequence (cu_seqlens, or more than max_nodes rows) is skipped
  *    and flagged GDN_STATUS_BAD_SEQLEN; a parent or accepted node that is not one
  *    is flagged GDN_STATUS_BAD_TREE, outputs of its sequence are then
- *    unspecified and its state is left alone.  Nothing is read out of bounds.
+ *    unspecified and its state is left alone (gdn_commit_tree looks at the trees
+ *    that it takes something of).  Nothing is read out of bounds.
  *  - A row that holds NaN or infinities makes its own outputs and its
  *    descendants' NaN (or infinite), never those of other nodes: in the conv the
  *    channel that holds them; in the delta rule without the norm the value column

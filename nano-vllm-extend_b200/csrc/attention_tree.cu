@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(32 * (WM * WN + 1), Attn<D, WM, WN>::CTAS)
 // us).  The TMA producer keeps ST - 1 further tiles under way, and one more warp brings the
 // next segment's queries (a box of whole nodes' heads) and its nodes' ancestors: what a
 // segment does once is what is left above the memory traffic (queries through registers
-// when the segment began: 105 us, now 90; a longer context costs 6.3 TB/s).
+// when the segment began: 105 us, now 92; a longer context costs 6.3 TB/s).
 //
 // O is corrected only when a row's maximum has grown by more than 2^8 since its last
 // correction: until then its probabilities are measured against the older maximum, which

@@ -17,8 +17,11 @@
 // shuffle sum.  All arithmetic is fp32, rounded once at the end.
 //
 // NH: 6 where that many rows fill the GPU anyway (8.3k rows of 16 + 4 + 4 heads x 128:
-// 1 head 35 us, 2 28, 4 26, 6 24, 8 27; floor 16), else 2, which spread a small call
-// over more SMs (128 rows: 2.6 us where 6 take 4.2).
+// 1 head 35 us, 2 28, 4 26, 6 24, 8 29; floor 16), else 2, which spread a small call
+// over more SMs (128 rows: 2.6 us where 6 take 4.2).  The rule does not look at the number
+// of heads, and where six do not divide it lanes are without one: 8 heads (25k rows) 32.8 us
+// where NH = 4 takes 27.7, 10 heads (20k) 27.2 where 5 takes 25.1, 7 heads (29k) 35.5 where 8
+// takes 27.4; 12 and 24 heads are best with 6.
 #include "mma_util.cuh"
 #include "tree.cuh"
 

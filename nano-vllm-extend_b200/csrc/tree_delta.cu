@@ -20,8 +20,8 @@
 // columns by 8 nodes, so few nodes waste little.  The results' layout is that of the
 // next product's A operand (nodes 2t, 2t + 1 as its k = t, t + 4), so X, d and o
 // never leave the warp's registers.  X is bf16 with fp32 sums: q and k are exact,
-// S_0 enters as two parts, each rounded: 2^-17 of an element is left out, which adds
-// 1e-4 to the 1.7e-3 (relative) of the output's rounding (all 24 bits, in three parts:
+// S_0 enters as two parts, each rounded: 2^-17 of an element is left out, which moves
+// outputs by 5e-5 relative, where their own rounding is 1.7e-3 (all 24 bits, in three parts:
 // 107 us instead of 97; one tf32 part of 11 bits saves 2 of them); A, M and d meet in
 // tf32, two parts of 11 bits each (hi hi + lo hi + hi lo).  Norms, decays and the
 // substitution within eight nodes are fp32.
@@ -34,7 +34,7 @@
 // each a whole unit.  A buffer is refilled as soon as its group has formed X.  Rows,
 // values and gates of the next unit are copied into shared memory a unit ahead
 // (cp.async): as loads into registers they made every other wait of the warp a wait
-// for memory (a warp has six scoreboards), 115 us where this takes 99.  Measured
+// for memory (a warp has six scoreboards), 115 us where this took 99.  Measured
 // so, 256 sequences x 32 heads of 3 to 8 nodes, the floor being 89 us: state loaded
 // into registers by its own CTA, two CTAs an SM, 160-228 us (the loads stand still
 // while a CTA computes); the ring with two groups of eight warps 174 (1000
